@@ -43,6 +43,7 @@ c_int32 = ctypes.c_int32
 c_size_t = ctypes.c_size_t
 c_float = ctypes.c_float
 c_uint64 = ctypes.c_uint64
+c_int64 = ctypes.c_int64
 
 
 class MxExpertPtrs(ctypes.Structure):
@@ -122,6 +123,46 @@ class MxFullAttnWeights(ctypes.Structure):
 class MxFullAttnViews(ctypes.Structure):
     _fields_ = [("h32", c_void_p), ("h16", c_void_p), ("qg", c_void_p), ("k", c_void_p),
                 ("v", c_void_p), ("act", c_void_p), ("y", c_void_p)]
+
+
+class MxKvCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("n_pages", c_int32), ("page_size", c_int32), ("n_kv_heads", c_int32),
+                ("head_dim", c_int32), ("dtype", c_int32)]
+
+
+class MxPagedBatch(ctypes.Structure):
+    _fields_ = [("q_start", c_void_p), ("kv_len", c_void_p), ("pages", c_void_p),
+                ("n_seqs", c_int32), ("max_pages", c_int32), ("rows", c_int32),
+                ("max_q", c_int32), ("max_kv", c_int32)]
+
+
+class MxKvRows(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+                ("q_norm_w", c_void_p), ("k_norm_w", c_void_p), ("ldq", c_int64),
+                ("ldk", c_int64), ("ldv", c_int64), ("ldqo", c_int64), ("n_heads", c_int32),
+                ("rotary_dim", c_int32), ("x_dtype", c_int32), ("param_dtype", c_int32),
+                ("rope_theta", ctypes.c_double), ("eps", c_float)]
+
+
+class MxPagedAttn(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("gate", c_void_p), ("ldq", c_int64),
+                ("ldo", c_int64), ("ldg", c_int64), ("n_heads", c_int32), ("scale", c_float)]
+
+
+class MxPagePool(ctypes.Structure):
+    _fields_ = [("base", c_void_p), ("page_bytes", c_size_t), ("n_pages", c_int32)]
+
+
+class MxGatedDelta(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("g", c_void_p),
+                ("beta", c_void_p), ("o", c_void_p), ("state", c_void_p), ("slot_in", c_void_p),
+                ("slot_out", c_void_p), ("q_start", c_void_p), ("ldq", c_int64),
+                ("ldk", c_int64), ("ldv", c_int64), ("ldo", c_int64), ("n_slots", c_int32),
+                ("n_seqs", c_int32), ("rows", c_int32), ("max_q", c_int32),
+                ("n_k_heads", c_int32), ("n_v_heads", c_int32), ("head_dim_k", c_int32),
+                ("head_dim_v", c_int32), ("x_dtype", c_int32), ("qk_norm", c_int32),
+                ("scale", c_float)]
 
 
 class MxDeviceInfo(ctypes.Structure):
@@ -219,6 +260,15 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mx_gated_delta_scan_ws": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                                               c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                               c_size_t, c_void_p]),
+    "mx_kv_append": (ctypes.c_int, [P(MxKvCache), P(MxPagedBatch), P(MxKvRows), c_void_p]),
+    "mx_paged_attn_workspace_size": (ctypes.c_int, [P(MxKvCache), P(MxPagedBatch), c_int32,
+                                                    P(c_size_t)]),
+    "mx_paged_attn": (ctypes.c_int, [P(MxKvCache), P(MxPagedBatch), P(MxPagedAttn), c_void_p,
+                                     c_size_t, c_void_p]),
+    "mx_copy_pages": (ctypes.c_int, [P(MxPagePool), c_int32, c_void_p, c_void_p, c_int32,
+                                     c_void_p]),
+    "mx_gated_delta_rule_workspace_size": (ctypes.c_int, [P(MxGatedDelta), P(c_size_t)]),
+    "mx_gated_delta_rule": (ctypes.c_int, [P(MxGatedDelta), c_void_p, c_size_t, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -483,6 +483,162 @@ int mx_gated_delta_scan_ws(const float* q, const float* kb, const float* v,
                            int32_t head_dim_k, int32_t head_dim_v, float* o, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* =================================================================================== *
+ * Serving memory: what the sequences of a server carry from one call to the next, and  *
+ * the operators on it.  No counterpart in the reference, which runs every token over   *
+ * its whole prefix (its executors keep neither keys nor a recurrent state).            *
+ * =================================================================================== */
+
+/* The keys and values of one layer, in pages of page_size tokens:
+ * k, v [n_pages, n_kv_heads, page_size, head_dim] of dtype F32, F16 or I8 (16-byte aligned);
+ * int8 rows stand for int8 * scale with one fp32 scale per row in k_scale, v_scale
+ * [n_pages, n_kv_heads, page_size] (16-byte aligned; NULL for the other types).
+ * page_size: 16, 32, 64, 128 or 256.  head_dim: a multiple of 8 (I8: 16), <= 256.      */
+typedef struct MxKvCache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+} MxKvCache;
+
+/* The sequences of one call (device arrays).  Sequence b has the rows q_start[b] ..
+ * q_start[b + 1] - 1 of the call's row arrays as its newest tokens and kv_len[b] tokens in the
+ * cache, the new ones among them: row i of it is at position kv_len[b] - rows of b + i.  The
+ * token at position p lies in row p % page_size of page pages[b][p / page_size]; an id
+ * outside [0, n_pages) is no page: nothing is written to it and its keys take no part.
+ * q_start ascends from 0; a sequence may have no rows, and rows from q_start[n_seqs] on belong
+ * to nobody and are left as they are.  n_seqs <= 65535, rows < 2^24.  max_q and max_kv (at least the most rows
+ * and the most cached tokens of a sequence) choose the launch; `rows` (at least
+ * q_start[n_seqs]) bounds it.                                                           */
+typedef struct MxPagedBatch {
+  const int32_t* q_start; /* [n_seqs + 1]                                               */
+  const int32_t* kv_len;  /* [n_seqs]                                                   */
+  const int32_t* pages;   /* [n_seqs, max_pages]                                        */
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t rows;
+  int32_t max_q;
+  int32_t max_kv;
+} MxPagedBatch;
+
+/* New rows for the cache.  q, k, v: rows of x_dtype (F32 / F16), head after head, row
+ * strides in elements.  Per head of q and k: y = x / sqrt(mean(x^2) + eps) * norm weight (where
+ * one is given), then the rotate-half rotary embedding of the first rotary_dim dims at the
+ * row's position, angles formed in 64 bits (position * theta^(-2 j / rotary_dim)).  q goes
+ * to q_out (F32 with an F32 cache, else F16; q and q_out NULL: no queries), k and v to their
+ * pages; int8 rows get scale max|row| / 127 (1 for a row of zeros).  Rows at a negative
+ * position are left out.                                                               */
+typedef struct MxKvRows {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  const void* q_norm_w; /* [head_dim] of param_dtype or NULL                            */
+  const void* k_norm_w;
+  int64_t ldq;
+  int64_t ldk;
+  int64_t ldv;
+  int64_t ldqo;
+  int32_t n_heads;
+  int32_t rotary_dim;  /* even, 0 .. head_dim                                           */
+  int32_t x_dtype;
+  int32_t param_dtype;
+  double rope_theta;
+  float eps;
+} MxKvRows;
+int mx_kv_append(const MxKvCache* cache, const MxPagedBatch* batch, const MxKvRows* rows,
+                 void* stream);
+
+/* Attention of the batch's rows over the cache:
+ *   out = sum_j softmax_j(scale q . k_j) v_j over the keys up to the row's own position,
+ * times sigmoid(gate) where a gate is given; zeros for a row that sees no key.  q and out:
+ * rows of n_heads * head_dim, F32 with an F32 cache, else F16; gate fp32; row strides in
+ * elements (ldq, ldo, ldg), head after head.  Key/value head of query head h:
+ * h / (n_heads / n_kv_heads).  Fp16 and int8 caches: products of fp16 operands with fp32
+ * sums (probabilities rounded to fp16); fp32 caches: fp32 throughout.  q and gate 16-byte
+ * aligned with row strides that keep it, out likewise.                                 */
+typedef struct MxPagedAttn {
+  const void* q;
+  void* out;
+  const float* gate;
+  int64_t ldq;
+  int64_t ldo;
+  int64_t ldg;
+  int32_t n_heads;
+  float scale;
+} MxPagedAttn;
+/* Bytes of workspace of such a call (16-byte aligned; partial results of split key ranges).
+ * Calls that may overlap need a workspace each.                                        */
+int mx_paged_attn_workspace_size(const MxKvCache* cache, const MxPagedBatch* batch,
+                                 int32_t n_heads, size_t* nbytes);
+int mx_paged_attn(const MxKvCache* cache, const MxPagedBatch* batch, const MxPagedAttn* args,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages (cache pages, scale pages, state slots) copied inside each of n_pools pools: page
+ * dst[i] of a pool becomes page src[i], i < n_copies.  The pools array is read on the host during
+ * the call; src and dst are device arrays.  page_bytes a multiple of 16, base 16-byte aligned.
+ * A pair with an id outside [0, n_pages) is left out.  No page may be a dst twice, or a dst and
+ * another pair's src.                                                                  */
+typedef struct MxPagePool {
+  void* base;
+  size_t page_bytes;
+  int32_t n_pages;
+} MxPagePool;
+int mx_copy_pages(const MxPagePool* pools, int32_t n_pools, const int32_t* src,
+                  const int32_t* dst, int32_t n_copies, void* stream);
+
+/* The gated delta rule over a ragged batch, from and to state slots.  Per value head (its
+ * key head: head / (n_v_heads / n_k_heads)), with S [head_dim_k, head_dim_v]:
+ *   S' = exp(g_t) S;  u = beta_t (v_t - k_t^T S');  S = S' + k_t u^T;  o_t = scale q_t^T S
+ * and, with qk_norm, q_t and k_t first divided by sqrt(sum of squares + 1e-6).  (The scan
+ * above, mx_gated_delta_scan, is the reference's recurrence: it adds beta k v^T without
+ * taking k^T S away, starts at zero and drops its state.)  q, k [rows, n_k_heads head_dim_k], v, o
+ * [rows, n_v_heads head_dim_v] of x_dtype (F32 / F16) with row strides in elements; g (<= 0)
+ * and beta fp32 [rows, n_v_heads] contiguous; state fp32 [n_slots, n_v_heads, head_dim_k,
+ * head_dim_v], 16-byte aligned.  Sequence b (rows q_start[b] .. q_start[b + 1] - 1) starts
+ * from slot slot_in[b], or from zeros where that is outside [0, n_slots), and leaves its state
+ * in slot_out[b], or nowhere where that is outside.  A slot may be one sequence's in and out;
+ * no slot may be out of two sequences, or out of one and in of another.  head_dim_k and
+ * head_dim_v: multiples of 4, <= 256.  rows, max_q and rows past q_start[n_seqs] as in
+ * MxPagedBatch.                                                                        */
+typedef struct MxGatedDelta {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;
+  const float* beta;
+  void* o;
+  float* state;
+  const int32_t* slot_in;  /* [n_seqs]                                                  */
+  const int32_t* slot_out; /* [n_seqs]                                                  */
+  const int32_t* q_start;  /* [n_seqs + 1]                                              */
+  int64_t ldq;
+  int64_t ldk;
+  int64_t ldv;
+  int64_t ldo;
+  int32_t n_slots;
+  int32_t n_seqs;
+  int32_t rows;
+  int32_t max_q;
+  int32_t n_k_heads;
+  int32_t n_v_heads;
+  int32_t head_dim_k;
+  int32_t head_dim_v;
+  int32_t x_dtype;
+  int32_t qk_norm;
+  float scale;
+} MxGatedDelta;
+/* Workspace (16-byte aligned) of such a call: 0 where the recurrence runs token by token.
+ * Calls that may overlap need a workspace each.                                        */
+int mx_gated_delta_rule_workspace_size(const MxGatedDelta* args, size_t* nbytes);
+int mx_gated_delta_rule(const MxGatedDelta* args, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,204 @@
+"""The gated delta rule on the GPU against float64, token by token.
+
+Tolerances: a state or an output is a sum of products over the head dim, formed in fp32 (2^-24 of the
+sum of absolute values per rounding, head_dim roundings at most), and the delta rule with beta in
+(0, 1) and unit keys does not grow a state: normwise (2 dk + 64) x 2^-24 for a few chunks'
+chain.  Fp16 outputs are rounded once more (2^-11 normwise)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import _serving as sv
+from moe_mi355x.delta_rule import GatedDeltaRunner, delta_args
+
+pytestmark = pytest.mark.gpu
+
+
+def say(msg):
+    print(f"[gpu] {msg}", flush=True)
+
+
+def make(rng, news, nk, nv, dk, dv, dtype, pad=0, decay=0.3, norm=True):
+    rows = sum(news) + pad
+    dt = sv.DT[dtype]
+    q, k, v = (rng.standard_normal((rows, h, d)) for h, d in ((nk, dk), (nk, dk), (nv, dv)))
+    q, k, v = (a / (1 + np.exp(-a)) for a in (q, k, v))  # as behind the short convolution
+    if not norm:
+        q, k = (a / np.sqrt((a * a).sum(-1, keepdims=True) + 1e-6) for a in (q, k))
+    g = (-np.abs(rng.standard_normal((rows, nv))) * decay).astype(np.float32)
+    beta = (1 / (1 + np.exp(-rng.standard_normal((rows, nv))))).astype(np.float32)
+    return q.astype(dt), k.astype(dt), v.astype(dt), g, beta
+
+
+def run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, slot_in, slot_out, norm=True,
+        pads=(0, 0, 0, 0), max_q=None, scale=None):
+    q, k, v, g, beta = x
+    rows = len(g)
+
+    def wide(a, p, fill=5.0):
+        w = np.full((rows, a.shape[1] * a.shape[2] + p), fill, a.dtype)
+        w[:, :a.shape[1] * a.shape[2]] = a.reshape(rows, -1)
+        return w
+
+    start = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    o0 = wide(np.full((rows, nv, dv), 5.0, sv.DT[dtype]), pads[3])
+    with sv.Arrays(mi355x, stream) as ar:
+        po, ps = ar.put(o0), ar.put(state)
+        args = delta_args(q=ar.put(wide(q, pads[0])), k=ar.put(wide(k, pads[1])),
+                          v=ar.put(wide(v, pads[2])), g=ar.put(g), beta=ar.put(beta), o=po,
+                          state=ps, slot_in=ar.put(np.array(slot_in, np.int32)),
+                          slot_out=ar.put(np.array(slot_out, np.int32)), q_start=ar.put(start),
+                          n_slots=len(state), n_seqs=len(news), rows=rows,
+                          max_q=max_q or max([1, *news]), n_k_heads=nk, n_v_heads=nv, head_dim_k=dk,
+                          head_dim_v=dv, dtype=dtype, qk_norm=norm, scale=scale,
+                          ldq=nk * dk + pads[0], ldk=nk * dk + pads[1], ldv=nv * dv + pads[2],
+                          ldo=nv * dv + pads[3])
+        runner = GatedDeltaRunner(mi355x)
+        runner.reserve(args)
+        try:
+            runner.forward_device(args, stream)
+            o, s = ar.get(po, o0), ar.get(ps, state)
+        finally:
+            mi355x.synchronize_stream(stream)
+            runner.close()
+    assert np.all(o[:, nv * dv:] == 5.0) and np.all(o[start[-1]:] == 5.0)
+    return o[:, :nv * dv].reshape(rows, nv, dv), s
+
+
+def want_of(x, news, nk, nv, dk, dv, state, slot_in, slot_out, scale, norm=True):
+    q, k, v, g, beta = x
+    o = np.zeros((sum(news), nv, dv))
+    s = state.astype(np.float64)
+    r = 0
+    for b, n in enumerate(news):
+        for h in range(nv):
+            first = state[slot_in[b], h] if 0 <= slot_in[b] < len(state) else np.zeros((dk, dv))
+            at = slice(r, r + n)
+            hk = h // (nv // nk)
+            o[at, h], last = sv.delta_rule(q[at, hk], k[at, hk], v[at, h], g[at, h], beta[at, h],
+                                           first, scale, norm)
+            if 0 <= slot_out[b] < len(state):
+                s[slot_out[b], h] = last
+        r += n
+    return o, s
+
+
+def off(a, b):
+    return np.linalg.norm(a - b) / max(np.linalg.norm(b), 1e-30)
+
+
+CASES = [  # key heads, value heads, dk, dv, rows per sequence
+    (2, 2, 128, 128, [1]),
+    (2, 4, 128, 128, [1, 1, 1, 1, 1]),
+    (1, 3, 64, 64, [2, 1, 5]),
+    (2, 2, 32, 40, [7]),
+    (1, 2, 4, 4, [9]),
+    (1, 1, 256, 64, [3, 1]),
+    (2, 2, 96, 128, [70]),
+    (1, 2, 256, 256, [100]),
+    (2, 4, 128, 128, [64]),
+    (2, 4, 128, 128, [65, 63, 1, 0, 128]),
+    (1, 2, 128, 128, [33]),
+    (4, 4, 64, 64, [200, 17]),
+    (1, 3, 64, 128, [130, 64]),
+    (2, 2, 128, 64, [127]),
+    (1, 2, 128, 128, [700]),
+    (16, 32, 128, 128, [150, 300]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("nk,nv,dk,dv,news", CASES)
+def test_delta_rule_matches_float64(mi355x, stream, nk, nv, dk, dv, news, dtype):
+    say(f"delta rule heads={nk}/{nv} dk={dk} dv={dv} rows={news} {dtype}")
+    rng = np.random.default_rng(dk + dv + len(news))
+    x = make(rng, news, nk, nv, dk, dv, dtype, pad=2)
+    n = len(news)
+    state = (rng.standard_normal((2 * n + 1, nv, dk, dv)) * 0.3).astype(np.float32)
+    ids = rng.permutation(2 * n)
+    slot_in, slot_out = list(ids[:n]), list(ids[n:])
+    if n > 1:
+        slot_in[1] = -1           # a fresh sequence
+        slot_out[0] = slot_in[0]  # in place
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, slot_in, slot_out)
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, slot_in, slot_out, dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    eo, es = off(o[:sum(news)], wo), off(s, ws)
+    print(f"    normwise err o {eo:.2e} state {es:.2e}", flush=True)
+    assert es <= tol and eo <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+    keep = [i for i in range(2 * n + 1) if i not in slot_out]
+    assert np.array_equal(s[keep], state[keep])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("decay,news", [(30.0, [130, 3]), (0.0, [200]), (1e-4, [300]), (400.0, [70])])
+def test_decays(mi355x, stream, decay, news, dtype):
+    """No decay, hardly any, and decays that wipe the state out in a token."""
+    say(f"delta rule, decay scale {decay}, {dtype}")
+    nk, nv, dk, dv = 1, 2, 128, 128
+    rng = np.random.default_rng(int(decay) + 1)
+    x = make(rng, news, nk, nv, dk, dv, dtype, decay=decay)
+    if decay == 400.0:
+        x[3][5, 0], x[3][20, 1], x[3][64, 0] = -np.inf, -3e38, -np.inf
+    state = rng.standard_normal((2, nv, dk, dv)).astype(np.float32)
+    io = list(range(len(news)))
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, io, io)
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, io, io, dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    assert off(s, ws) <= tol and off(o, wo) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("news", [[1, 3], [90, 200]])
+def test_repeated_keys(mi355x, stream, news, dtype):
+    """The same key token after token with beta near one: the state holds the newest value, and the
+    products within a chunk are as far from small as they come."""
+    say(f"delta rule with one key, rows={news} {dtype}")
+    nk, nv, dk, dv = 1, 2, 64, 128
+    rng = np.random.default_rng(8)
+    q, k, v, g, beta = make(rng, news, nk, nv, dk, dv, dtype, decay=0.01)
+    k[:] = k[:1]
+    beta[:] = 0.999
+    state = np.zeros((2, nv, dk, dv), np.float32)
+    x = (q, k, v, g, beta)
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, [0, 1], [0, 1])
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, [0, 1], [0, 1], dk ** -0.5)
+    # each of the chunk's 64 rows is formed from the 63 before it, with factors near one
+    tol = 64 * (2 * dk + 64) * 2.0 ** -24
+    assert off(s, ws) <= tol and off(o, wo) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("news", [[1, 2], [40, 100]])
+def test_strides_scale_and_no_norm(mi355x, stream, news, dtype):
+    say(f"delta rule, strided rows={news} {dtype}")
+    nk, nv, dk, dv = 2, 4, 64, 64
+    rng = np.random.default_rng(4)
+    x = make(rng, news, nk, nv, dk, dv, dtype, pad=1, norm=False)
+    state = rng.standard_normal((3, nv, dk, dv)).astype(np.float32)
+    for pads in ((8, 16, 24, 8), (3, 1, 5, 7)):
+        o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, [0, 5], [2, -1], norm=False,
+                   pads=pads, scale=0.7)
+        wo, ws = want_of(x, news, nk, nv, dk, dv, state, [0, 5], [2, -1], 0.7, norm=False)
+        tol = (2 * dk + 64) * 2.0 ** -24
+        assert off(s, ws) <= tol
+        assert off(o[:sum(news)], wo) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+
+
+def test_a_prompt_in_pieces_is_the_prompt_at_once(mi355x, stream):
+    """Chunks of a prompt and then single tokens, carried through a slot, against one call."""
+    say("delta rule, a prompt in pieces")
+    nk, nv, dk, dv, T = 2, 4, 128, 128, 260
+    rng = np.random.default_rng(13)
+    x = make(rng, [T], nk, nv, dk, dv, "float32")
+    zero = np.zeros((1, nv, dk, dv), np.float32)
+    o, s = run(mi355x, stream, x, [T], nk, nv, dk, dv, "float32", zero, [0], [0])
+    st, parts, at = zero, [], 0
+    for n in (100, 64, 1, 1, 90, 1, 3):
+        po, st = run(mi355x, stream, tuple(a[at:at + n] for a in x), [n], nk, nv, dk, dv, "float32", st,
+                     [0], [0])
+        parts.append(po)
+        at += n
+    tol = 2 * (2 * dk + 64) * 2.0 ** -24
+    assert at == T and off(np.concatenate(parts), o) <= tol and off(st, s) <= tol
