@@ -10,8 +10,6 @@ struct PkCache {
   float* ks;
   float* vs;
   int n_pages, ps, ps_log, nkv, hd, dt;
-  long head_stride;  // bytes of one head's rows in a page
-  long page_stride;  // bytes of a page
 };
 struct PkBatch {
   const int* q_start;
@@ -58,8 +56,6 @@ static inline PkCache pk_cache(const MxKvCache* c) {
   k.nkv = c->n_kv_heads;
   k.hd = c->head_dim;
   k.dt = c->dtype;
-  k.head_stride = (long)k.ps * k.hd * pk_esz(k.dt);
-  k.page_stride = k.head_stride * k.nkv;
   return k;
 }
 

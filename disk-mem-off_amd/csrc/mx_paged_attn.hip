@@ -1,10 +1,52 @@
 // Attention of new rows over a paged key/value cache (mx_paged_attn).
+//
+// Rows.  All query heads of a key/value head read the same keys, so the rows of a sequence and
+// key/value head are counted token-major with the head inside: row r is token r / G, head r % G
+// of the group (G = n_heads / n_kv_heads).  A decode step of one token fills G rows, a chunk of
+// n tokens n G, and a row tile takes consecutive rows.
+//
+// Products.  Per 32 keys (two sub-tiles of 16, each inside one page):
+//   S^T = K Q^T   (A = 16 key rows from memory order, B = 16 query rows): lane (j, g) = (lane %
+//                 16, lane / 16) gets S[key 4 g + r][row j], so a row's softmax is in its lanes
+//   O^T += V^T P  (A = 16 dims x 32 keys, B = the lane's own probabilities): the k-slot (g, e)
+//                 stands for key 4 g + e of sub-tile 0 (e < 4) and key 4 g + e - 4 of sub-tile 1.
+// Values lie row-major in the pages; the transposing LDS reads (ds_read_b64_tr) give a lane the
+// 8 keys of one dim.
+//
+// Softmax in the base-2 domain with a lazy reference: a row's reference m moves only when a tile's
+// maximum passes it by more than kTau, so probabilities stay below 2^kTau (fp16 holds them)
+// and the accumulators are rescaled on few tiles.  Statistics and sums are fp32; the probabilities
+// are rounded to fp16 for the second product.
+//
+// Int8 pages: with a score s in the base-2 domain and the value row's scale w, the weight that
+// meets the int8 values is 2^s w = 2^(s + log2 w); its reference is taken over s + log2 w, the
+// accumulators take 2^(s + log2 w - m) and the row sum the same divided by w (fp32), so no
+// range of scales leaves fp16's.
+//
+// What is masked stays out: scores of keys past the row, past the cache or on no page are
+// replaced before the maximum; value rows no row of the wave sees are replaced by zeros, and
+// non-finite values that only some rows of a tile see (a NaN in the newest token) are taken out
+// of the matrix product and added to the rows that see them one by one.
 #include <math.h>
 
+#include <type_traits>
+
 #include "mx_common.h"
+#include "mx_lds_copy.h"
 #include "mx_paged.h"
 
 namespace {
+
+constexpr float kTau = 8.f;
+constexpr float kLow = -3.0e38f;  // a reference below every score
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef __amdgpu_buffer_rsrc_t pa_rsrc_t;
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef int int2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ int pa_ceil(int a, int b) { return (a + b - 1) / b; }
 
 struct PaArgs {
   const void* q;
@@ -15,64 +57,1059 @@ struct PaArgs {
   float scale;
 };
 
-// One wave per (row, head): the keys one after another, the dims over the lanes.
-template <typename XT, int DT>
-__global__ __launch_bounds__(64) void k_pa_simple(PkCache c, PkBatch b, PaArgs a) {
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int seq = __builtin_amdgcn_readfirstlane(pk_seq_of(b.q_start, b.n_seqs, t));
-  if (seq >= b.n_seqs) return;
-  const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1];
-  const int pos = b.kv_len[seq] - (q1 - q0) + (t - q0);
-  const int kvh = h / a.group;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-  const XT* qr = (const XT*)a.q + (long)t * a.ldq + (long)h * c.hd;
+// Key ranges: split z covers keys [z len, (z + 1) len).  A row tile whose keys fit one range
+// writes its result; the others leave sums (relative to their reference) for k_pa_join.
+struct PaSplit {
+  int len, n;
+  float* po;    // [n][rows][nh][hd]
+  float2* ml;   // [n][rows][nh]: reference, sum
+};
+
+// What a row tile is.
+struct PaTile {
+  int seq, row0, nrows;  // first row; rows of the sequence and head
+  int first;             // q_start of the sequence
+  int pos0;              // position of the sequence's row 0
+  int kend;              // keys its last row sees
+};
+
+// Tile `idx` of the batch's row tiles of RT rows (every sequence has ceil(rows G / RT), in order);
+// false past the last.  64 lanes sum the sequences' tiles, then look inside one lane's
+// share: one round for 64 sequences, two for 4096.  Wave-uniform; callers converged.
+template <int RT>
+__device__ __forceinline__ bool pa_find_tile(const PkBatch& b, const PkCache& c, int group, int idx,
+                                             int kmax, PaTile* t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = b.n_seqs, before = 0;
+  while (true) {
+    const int per = (hi - lo + 63) >> 6;
+    const int s0 = lo + lane * per, s1 = min(hi, s0 + per);
+    int sum = 0;
+    for (int s = s0; s < s1; ++s)
+      sum += (int)(((long)(b.q_start[s + 1] - b.q_start[s]) * group + RT - 1) / RT);
+    int incl = sum;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) q[e] = lane + 64 * e < c.hd ? (float)qr[lane + 64 * e] * a.scale : 0.f;
-  float m = -INFINITY, l = 0.f;
-  const int n = min(pos + 1, b.max_pages * c.ps);
-  for (int j = 0; j < n; ++j) {
-    const int page = b.pages[(long)seq * b.max_pages + (j >> c.ps_log)];
-    if (page < 0 || page >= c.n_pages) continue;
-    const long row = ((long)page * c.nkv + kvh) * c.ps + (j & (c.ps - 1));
-    float s = 0.f, v[4];
+    for (int o = 1; o < 64; o *= 2) {
+      const int up = __shfl_up(incl, o);
+      if (lane >= o) incl += up;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > idx);
+    if (!past) return false;
+    const int l = __builtin_ctzll(past);
+    before += __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(sum, l);
+    lo = lo + l * per;
+    if (per == 1) break;
+    hi = min(hi, lo + per);
+  }
+  t->seq = lo;
+  t->first = __builtin_amdgcn_readfirstlane(b.q_start[lo]);
+  const int m = __builtin_amdgcn_readfirstlane(b.q_start[lo + 1]) - t->first;
+  const int len = __builtin_amdgcn_readfirstlane(b.kv_len[lo]);
+  t->row0 = (idx - before) * RT;
+  t->nrows = m * group;
+  t->pos0 = len - m;
+  const int last = min(t->row0 + RT, t->nrows) - 1;
+  t->kend = max(0, min(t->pos0 + last / group + 1, kmax));
+  return true;
+}
+
+__device__ __forceinline__ pa_rsrc_t pa_rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
+}
+
+// Both operands of a lane swap: v_permlane16_swap exchanges the odd 16-lane rows of x with
+// the even ones of y, v_permlane32_swap the upper half of x with the lower half of y.  With x = y
+// = v the two hold v of the lane and of its partner.  (The compiler's builtins return x alone:
+// a maximum over both results of one is folded away.)  s_nop: the swap's operands were just
+// written.
+__device__ __forceinline__ void pa_swap16(float& x, float& y) {
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
+__device__ __forceinline__ void pa_swap32(float& x, float& y) {
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
+// Max and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float pa_rowmax(float v) {
+  float x = v, y = v;
+  pa_swap16(x, y);
+  x = y = fmaxf(x, y);
+  pa_swap32(x, y);
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ float pa_rowsum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// 8 int8 -> 8 fp16 (mx_i8_to_f16 of half the width).
+__device__ __forceinline__ half8_t pa_i8x8(int2_t v) {
+  const half2_t bias = {(half_t)1152.0f, (half_t)1152.0f};
+  half2_t h[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = lane + 64 * e;
-      v[e] = 0.f;
-      if (d >= c.hd) continue;
-      const long at = row * c.hd + d;
-      if constexpr (DT == MX_DT_I8) {
-        s += q[e] * ((float)((const int8_t*)c.k)[at] * c.ks[row]);
-        v[e] = (float)((const int8_t*)c.v)[at] * c.vs[row];
-      } else {
-        s += q[e] * (float)((const XT*)c.k)[at];
-        v[e] = (float)((const XT*)c.v)[at];
+  for (int d = 0; d < 2; ++d) {
+    const uint32_t u = (uint32_t)v[d] ^ 0x80808080u;
+    h[2 * d] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+    h[2 * d + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+  }
+  return (half8_t){h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+
+// ------------------------------------------------------------------------------------
+// LDS tiles of 32 rows of RB bytes (RB = 64 .. 512, the padded row), row-major, a row's 16-byte
+// chunks permuted by an XOR so that the fragment reads use every bank once: 8 lanes of a
+// 16-byte read take one chunk of 8 consecutive rows (keys: chunk ^ row % 8), 16 lanes of an 8-byte
+// transposing read take 32 bytes of 4 rows (fp16 values: chunk ^ 2 (row % 4)) or 16 bytes of 8
+// rows (int8 values: chunk ^ the row's number among the 16 that two groups of lanes read).
+// A copy instruction fills 1 KiB, whole rows: the permutation stays inside a row, so it reads
+// whole rows of the page in order.  Rows of fewer than RB bytes: the chunks past the row repeat
+// its last one (the queries are zero there, and no output is stored).
+// ------------------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ int pa_vxor(int row) {  // row of the 32
+  if constexpr (DT == MX_DT_I8) return (row & 3) | ((row >> 4) & 1) << 2 | ((row >> 2) & 1) << 3;
+  return 2 * (row & 3);
+}
+
+// Byte offset in a 16-row sub-tile of the page that copy instruction `i` (of RB / 64) loads on this
+// lane for row-major rows of rb bytes; XORs by `x(row)`.
+template <int RB, typename X>
+__device__ __forceinline__ uint32_t pa_copy_off(int i, int lane, int rb, X x) {
+  constexpr int CPR = RB / 16, RPI = 1024 / RB;
+  const int row = i * RPI + lane / CPR;
+  const int chunk = ((lane % CPR) ^ x(row)) & (CPR - 1);
+  return (uint32_t)(row * rb + min(chunk * 16, rb - 16));
+}
+
+// One lane's value fragment f (16 dims x 32 keys) of a tile at byte offset `base` of the wave's
+// LDS: the XOR of the chunk number is the XOR of address bits, rows are RB-aligned.
+template <int DT>
+__device__ __forceinline__ int pa_vlane(int rb_pad, int lane) {
+  const int j = lane & 15, g = lane >> 4;
+  if constexpr (DT == MX_DT_I8) {
+    const int rr = j >> 1, row = rr < 4 ? 4 * g + rr : 16 + 4 * g + rr - 4;
+    return row * rb_pad + ((pa_vxor<DT>(row) * 16) & (rb_pad - 1)) + 8 * (j & 1);
+  }
+  const int row = 4 * g + (j >> 2);
+  return row * rb_pad + (((pa_vxor<DT>(row) + ((j & 3) >> 1)) * 16) & (rb_pad - 1)) + 8 * (j & 1);
+}
+
+typedef __attribute__((address_space(3))) short4_t pa_lds_s4;
+typedef __attribute__((address_space(3))) int2_t pa_lds_i2;
+
+template <int RB, int DT>
+__device__ __forceinline__ half8_t pa_vfrag(const char* tile, int vlane, int f) {
+  if constexpr (DT == MX_DT_I8) {
+    const int2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((pa_lds_i2*)(tile + (vlane ^ (f * 16))));
+    return pa_i8x8(v);
+  } else {
+    const char* p = tile + (vlane ^ (f * 32));
+    const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)p);
+    const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)(p + 16 * RB));
+    const half4_t x = __builtin_bit_cast(half4_t, a), y = __builtin_bit_cast(half4_t, b);
+    return (half8_t){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  }
+}
+
+// A fragment of a masked tile: keys no row of the wave sees become zeros (keep: 16-bit masks
+// of the lane's 8 keys), and with fp16 values non-finite ones do too, noted in `odd`.
+template <int DT>
+__device__ __forceinline__ half8_t pa_clean(half8_t v, const uint32_t (&keep)[4], uint32_t& odd) {
+  int4_t u = __builtin_bit_cast(int4_t, v);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    uint32_t w = (uint32_t)u[d] & keep[d];
+    if constexpr (DT != MX_DT_I8) {
+      const uint32_t lo = (w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+      const uint32_t hi = (w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+      odd |= lo | hi;
+      w &= ~(lo | hi);
+    }
+    u[d] = (int)w;
+  }
+  return __builtin_bit_cast(half8_t, u);
+}
+
+// The non-finite values that pa_clean took out of a tile, added to the rows that see them (fp16
+// values only; rare).  p: the row's probabilities in k-slot order; lim: the last key of the tile
+// that the lane's row sees; seen: keys on a page (bit per key).
+template <int RB, int NF>
+__device__ __forceinline__ void pa_add_odd(const char* tile, half8_t p, int lim, uint32_t seen,
+                                        float4_t (&o)[NF]) {
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  for (int key = 0; key < 32; ++key) {
+    if (!((seen >> key) & 1)) continue;
+    const int src = ((key & 15) >> 2) * 16 + j, e = (key >> 4) * 4 + (key & 3);
+    half_t pe = p[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) pe = i == e ? p[i] : pe;
+    const float pk = __shfl((float)pe, src);
+    const int row = key * RB, x = pa_vxor<MX_DT_F16>(key) * 16;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      // dims 16 f + 4 g ..: chunk 2 f + g / 2, its half g % 2
+      const half4_t v = *(const half4_t*)(tile + row + (((32 * f + 16 * (g >> 1)) ^ x) & (RB - 1)) + 8 * (g & 1));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool bad = (__builtin_bit_cast(unsigned short, v[r]) & 0x7C00) == 0x7C00;
+        if (bad && key <= lim) o[f][r] += pk * (float)v[r];
       }
     }
-    s = mx_wave_sum(s);
-    const float mn = fmaxf(m, s), al = m == mn ? 1.f : expf(m - mn), p = s == mn ? 1.f : expf(s - mn);
-    m = mn;
-    l = l * al + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * al + p * v[e];
   }
-  XT* orow = (XT*)a.out + (long)t * a.ldo + (long)h * c.hd;
+}
+
+// Two sub-tiles' key scales and value scales on this lane's keys (int8 pages).
+struct PaScales {
+  float4 ks[2], vs[2];
+};
+
+// One 32-key step of a row set: scores sc (raw dots) -> probabilities, running reference and
+// sum, accumulators rescaled where the reference moved.  lim: last key of the tile (relative)
+// that the row sees, relative to 4 g; `on`: bits of the sub-tiles that are on a page.
+template <int DT, bool MASK, int NF>
+__device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const PaScales& q8, int lim,
+                                              int on, float& mrun, float& lrun, float4_t (&o)[NF]) {
+  float s[8], inv[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 64 * e;
-    if (d >= c.hd) continue;
-    float r = l > 0.f ? o[e] / l : 0.f;
-    if (l != l) r = l;
-    if (a.gate) r *= mx_sigmoid(a.gate[(long)t * a.ldg + (long)h * c.hd + d]);
-    orow[d] = (XT)r;
+  for (int b = 0; b < 2; ++b) {
+    const float kq[4] = {q8.ks[b].x, q8.ks[b].y, q8.ks[b].z, q8.ks[b].w};
+    const float vq[4] = {q8.vs[b].x, q8.vs[b].y, q8.vs[b].z, q8.vs[b].w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool out = MASK && (16 * b + r > lim || !((on >> b) & 1));
+      float v;
+      if constexpr (DT == MX_DT_I8) {
+        const float w = fmaxf(vq[r], 1e-30f);
+        inv[4 * b + r] = out ? 0.f : __builtin_amdgcn_rcpf(w);
+        v = __builtin_fmaf(sc[b][r], rs * kq[r], __builtin_amdgcn_logf(w));
+      } else {
+        v = sc[b][r] * rs;
+      }
+      s[4 * b + r] = out ? -INFINITY : v;
+    }
   }
+  float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                   fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+  mt = pa_rowmax(mt);
+  const bool up = mt > mrun + kTau;
+  if (__builtin_amdgcn_ballot_w64(up)) {
+    const float mnew = up ? mt : mrun;
+    const float alpha = __builtin_amdgcn_exp2f(mrun - mnew);  // 1 where it stays
+    lrun *= alpha;
+    mrun = mnew;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[f] *= alpha;
+  }
+  half8_t p;
+  float ps = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = __builtin_amdgcn_exp2f(s[e] - mrun);
+    if constexpr (DT == MX_DT_I8) ps = __builtin_fmaf(v, inv[e], ps);
+    else ps += v;
+    p[e] = (half_t)v;
+  }
+  lrun += ps;
+  return p;
+}
+
+// The page ids of 64 sub-tiles, one per lane, and which of them are pages.
+struct PaIds {
+  int id;
+  uint64_t on;
+};
+__device__ __forceinline__ PaIds pa_ids(const PkBatch& b, const PkCache& c, int seq, int key, int stop) {
+  PaIds r;
+  const int pi = key >> c.ps_log;
+  r.id = key < stop && pi < b.max_pages ? b.pages[(long)seq * b.max_pages + pi] : -1;
+  const bool ok = r.id >= 0 && r.id < c.n_pages;
+  if (!ok) r.id = 0;
+  r.on = __builtin_amdgcn_ballot_w64(ok);
+  return r;
+}
+
+// ------------------------------------------------------------------------------------
+// k_pa_keys: a tile of 16 rows, its keys dealt to the block's 4 waves 32 at a time.  For decode
+// steps, bound by the bytes of the pages.  A wave's tiles are its own: keys straight into MFMA
+// registers (16 rows x 64 bytes per load), values by copies into two LDS buffers of the wave, the
+// next tile's of both in flight while one computes, no barrier until the waves' sums are put
+// together at the end.
+// ------------------------------------------------------------------------------------
+constexpr int kKeysRows = 16;
+constexpr int kKeysMax = 4096;  // keys of a split: 64 sub-tile page ids per wave
+
+template <int RB, int DT>
+__global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+  constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
+  constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16;
+  constexpr int NL = RB / 64;             // 1 KiB pieces per 16 rows
+  constexpr int TILE = 32 * RB;
+  __shared__ __align__(1024) char lds[4 * 2 * TILE];
+  __shared__ float sm[4][16], sl[4][16];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, z = blockIdx.z;
+  PaTile t;
+  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
+  if (!pa_find_tile<kKeysRows>(b, c, a.group, blockIdx.x, kmax, &t)) return;
+  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
+  if (k0 >= k1 && z > 0) return;
+  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+
+  const int row = min(t.row0 + j, t.nrows - 1);
+  const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
+  const int pos = t.pos0 + tok;
+  const int rb = c.hd * ES;
+  const float rs = a.scale * kLog2e;
+
+  // Queries: B fragments.  Fp16 pages: chunk cc holds dims 32 cc + 8 g ..; int8 pages (16 dims per
+  // 16-byte load): chunk pair (2 i, 2 i + 1) dims 64 i + 16 g .. + 7 and + 8 .. + 15.
+  half8_t qf[NC];
+  const half_t* qrow = (const half_t*)a.q + (long)(t.first + tok) * a.ldq + (long)hq * c.hd;
+  auto qdim = [&](int cc) { return DT == MX_DT_I8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g; };
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc) qf[cc] = *(const half8_t*)(qrow + min(qdim(cc), c.hd - 8));
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc)
+    if (qdim(cc) >= c.hd) qf[cc] = (half8_t)(half_t)0.f;
+
+  const int ntile = pa_ceil(max(0, k1 - k0), 32);
+  const int nw = ntile > wave ? (ntile - 1 - wave) / 4 + 1 : 0;
+  // lane l: the page of sub-tile l % 2 of the wave's tile l / 2
+  const PaIds ids = pa_ids(b, c, t.seq, k0 + 32 * (wave + 4 * (lane >> 1)) + 16 * (lane & 1), k1);
+  char* const buf = lds + wave * 2 * TILE;
+  uint32_t voff[NL][2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      voff[i][s] = pa_copy_off<RB>(i, lane, rb, [&](int r) { return pa_vxor<DT>(16 * s + r); });
+  auto row_of = [&](int i, int s) {  // the sub-tile's first row in a pool
+    const int id = __builtin_amdgcn_readlane(ids.id, 2 * i + s);
+    const int key = k0 + 32 * (wave + 4 * i) + 16 * s;
+    return (((long)id * c.nkv + kvh) << c.ps_log) + (key & (c.ps - 1));
+  };
+  auto issue_v = [&](int i) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const pa_rsrc_t r = pa_rsrc(c.v + row_of(i, s) * rb, 16 * rb);
+#pragma unroll
+      for (int n = 0; n < NL; ++n)
+        mx_copy_to_lds16(r, buf + (i & 1) * TILE + s * 16 * RB + n * 1024, voff[n][s]);
+    }
+  };
+  constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte loads per key row and lane
+  int4_t kr[2][NK];
+  PaScales q8;
+  auto load_k = [&](int i) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const long at = row_of(i, s);
+      const char* p = c.k + at * rb;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) kr[s][n] = *(const int4_t*)(p + (uint32_t)(j * rb + min(64 * n + 16 * g, rb - 16)));
+      if constexpr (DT == MX_DT_I8) {
+        q8.ks[s] = *(const float4*)(c.ks + at + 4 * g);
+        q8.vs[s] = *(const float4*)(c.vs + at + 4 * g);
+      }
+    }
+  };
+  const int vlane = pa_vlane<DT>(RB, lane);
+  float4_t o[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) o[f] = (float4_t){0.f, 0.f, 0.f, 0.f};
+  float mrun = kLow, lrun = 0.f;
+
+  // The last key that every row of the tile sees (rows past the last repeat it).
+  const int all = t.pos0 + t.row0 / a.group;
+  if (nw > 0) {
+    issue_v(0);
+    load_k(0);
+  }
+  for (int i = 0; i < nw; ++i) {
+    if (i + 1 < nw) issue_v(i + 1);
+    float4_t sc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        if constexpr (DT == MX_DT_I8) {
+          half8_t lo, hi;
+          mx_i8_to_f16(kr[s][n], lo, hi);
+          x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qf[2 * n], x[0], 0, 0, 0);
+          x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qf[2 * n + 1], x[1], 0, 0, 0);
+        } else {
+          x[n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kr[s][n]), qf[n],
+                                                            x[n & 1], 0, 0, 0);
+        }
+      }
+      sc[s] = x[0] + x[1];
+    }
+    const PaScales w8 = q8;
+    const int tk = k0 + 32 * (wave + 4 * i);  // first key of the tile
+    const int on = (int)(ids.on >> (2 * i)) & 3;
+    if (i + 1 < nw) load_k(i + 1);
+    const bool mask = tk + 31 > all || on != 3;
+    const int lim = pos - tk;
+    half8_t p;
+    if (mask) p = pa_softmax<DT, true>(sc, rs, w8, lim - 4 * g, on, mrun, lrun, o);
+    else p = pa_softmax<DT, false>(sc, rs, w8, lim, on, mrun, lrun, o);
+    // This tile's values have landed; the next tile's copies and key loads may be in flight.
+    int4_t pw = __builtin_bit_cast(int4_t, p);
+    if (i + 1 < nw) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(pw) : "n"(2 * NL + 2 * NK) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" : "+v"(pw) : : "memory");
+    p = __builtin_bit_cast(half8_t, pw);
+    const char* tile = buf + (i & 1) * TILE;
+    if (!mask) {
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(tile, vlane, f), p, o[f], 0, 0, 0);
+    } else {
+      const int top = min(t.kend - 1, 1 << 30) - tk;  // the last key any row sees
+      uint32_t keep[4], odd = 0;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
+        const bool ok = (on >> s) & 1;
+        keep[d] = (ok && k <= top ? 0xFFFFu : 0u) | (ok && k + 1 <= top ? 0xFFFF0000u : 0u);
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<DT>(pa_vfrag<RB, DT>(tile, vlane, f), keep, odd),
+                                                      p, o[f], 0, 0, 0);
+      if constexpr (DT != MX_DT_I8)
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+          const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
+          pa_add_odd<RB, NF>(tile, p, lim, seen, o);
+        }
+    }
+  }
+  lrun = pa_rowsum(lrun);
+
+  // The waves' sums, relative to the largest reference of each row.
+  if (g == 0) {
+    sm[wave][j] = mrun;
+    sl[wave][j] = lrun;
+  }
+  __syncthreads();
+  const float m = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j]));
+  const float mine = __builtin_amdgcn_exp2f(mrun - m);
+  float* const part = (float*)(lds + wave * 2 * TILE);  // [16 rows][DP], the wave's own buffers
+  static_assert(16 * DP * 4 <= 2 * TILE, "the sums fit the wave's buffers");
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const float4_t v = o[f] * mine;
+    *(float4_t*)(part + j * DP + 16 * f + 4 * g) = v;
+  }
+  __syncthreads();
+  constexpr int D4 = DP / 4;
+  for (int i = tid; i < 16 * D4; i += 256) {
+    const int r = i / D4, d = 4 * (i % D4);
+    if (t.row0 + r >= t.nrows || d >= c.hd) continue;
+    float4_t s = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f, mr = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      s += *(const float4_t*)((const float*)(lds + w * 2 * TILE) + r * DP + d);
+      l += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mr);
+    }
+    const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
+    const long tr = t.first + rt;
+    if (nsp > 1) {
+      const long at = ((long)z * b.rows + tr) * a.nh + h;
+      *(float4_t*)(sp.po + at * c.hd + d) = s;
+      if (d == 0) sp.ml[at] = make_float2(mr, l);
+      continue;
+    }
+    s *= l == 0.f ? 0.f : 1.f / l;
+    if (a.gate) {
+      const float4 gv = *(const float4*)(a.gate + tr * a.ldg + (long)h * c.hd + d);
+      s = (float4_t){s[0] * mx_sigmoid(gv.x), s[1] * mx_sigmoid(gv.y), s[2] * mx_sigmoid(gv.z),
+                     s[3] * mx_sigmoid(gv.w)};
+    }
+    *(half4_t*)((half_t*)a.out + tr * a.ldo + (long)h * c.hd + d) =
+        (half4_t){(half_t)s[0], (half_t)s[1], (half_t)s[2], (half_t)s[3]};
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// k_pa_join: the partial sums of a row's key ranges, one wave per (row, head).
+// ------------------------------------------------------------------------------------
+template <int RT, typename OT>
+__global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+  const int lane = threadIdx.x & 63;
+  const int item = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int t = item / a.nh, h = item - t * a.nh;
+  if (t >= b.rows) return;
+  const int seq = __builtin_amdgcn_readfirstlane(pk_seq_of(b.q_start, b.n_seqs, t));
+  if (seq >= b.n_seqs) return;
+  const int q0 = b.q_start[seq], m = b.q_start[seq + 1] - q0, len = b.kv_len[seq];
+  const int r = (t - q0) * a.group + h % a.group, nrows = m * a.group;
+  const int last = min(r / RT * RT + RT, nrows) - 1;
+  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
+  const int kend = max(0, min(len - m + last / a.group + 1, kmax));
+  const int n = pa_ceil(kend, sp.len);
+  if (n <= 1) return;
+  const long step = (long)b.rows * a.nh, at = (long)t * a.nh + h;
+  float mr = kLow;
+  for (int z = 0; z < n; ++z) mr = fmaxf(mr, sp.ml[at + z * step].x);
+  float l = 0.f;
+  float4_t s = {0.f, 0.f, 0.f, 0.f};
+  const int d = min(4 * lane, c.hd - 4);
+  for (int z = 0; z < n; ++z) {
+    const float2 ml = sp.ml[at + z * step];
+    const float w = __builtin_amdgcn_exp2f(ml.x - mr);
+    l += w * ml.y;
+    s += w * *(const float4_t*)(sp.po + (at + z * step) * c.hd + d);
+  }
+  if (4 * lane >= c.hd) return;
+  s *= l == 0.f ? 0.f : 1.f / l;
+  if (a.gate) {
+    const float4 gv = *(const float4*)(a.gate + (long)t * a.ldg + (long)h * c.hd + d);
+    s = (float4_t){s[0] * mx_sigmoid(gv.x), s[1] * mx_sigmoid(gv.y), s[2] * mx_sigmoid(gv.z),
+                   s[3] * mx_sigmoid(gv.w)};
+  }
+  OT* o = (OT*)a.out + (long)t * a.ldo + (long)h * c.hd + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (OT)s[e];
+}
+
+// ------------------------------------------------------------------------------------
+// k_pa_rows: a tile of 64 QS rows (16 QS per wave), every key tile shared by the block's 4 waves.
+// For chunks of new tokens, bound by the matrix instructions.  Key and value tiles of 32 keys are
+// copied straight into two LDS buffers by the buffer loads' LDS mode; a wave's copies of tile t + 1
+// are issued behind the barrier that opens tile t.  Each fragment read from LDS feeds QS query
+// sets.  A wave computes up to its own last key and then only keeps the copies going.
+//
+// Row tiles of a key/value head run on the XCDs that its keys are dealt to, the longest (last)
+// ones first.
+// ------------------------------------------------------------------------------------
+#ifndef PA_PD
+#define PA_PD 2  // LDS fragment reads in flight ahead of the MFMAs
+#endif
+
+template <int RB, int DT, int QS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
+  constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
+  constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16, CPR = RB / 16;
+  constexpr int NL = RB / 64;             // 1 KiB pieces per 16 rows
+  constexpr int FPW = NL;                 // copies per wave and tile (4 NL pieces, 4 waves)
+  constexpr int TILE = 64 * RB;           // keys, then values
+  constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte fragment reads per key row and lane
+  constexpr int RT = 64 * QS;
+  __shared__ __align__(1024) char lds[2 * TILE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4;
+  int kvh, idx;
+  {
+    const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    if (8 % c.nkv == 0) {
+      const int per = 8 / c.nkv;
+      kvh = x / per;
+      idx = i * per + x % per;
+    } else if (c.nkv % 8 == 0) {
+      const int per = c.nkv / 8;
+      kvh = x * per + i % per;
+      idx = i / per;
+    } else {
+      kvh = blockIdx.x % c.nkv;
+      idx = blockIdx.x / c.nkv;
+    }
+    idx = ntiles - 1 - idx;
+  }
+  if (idx < 0) return;
+  const int z = blockIdx.z;
+  PaTile t;
+  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
+  if (!pa_find_tile<RT>(b, c, a.group, idx, kmax, &t)) return;
+  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
+  if (k0 >= k1 && z > 0) return;
+  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+  const int ntile = pa_ceil(max(0, k1 - k0), 32);
+
+  const int rb = c.hd * ES;
+  const float rs = a.scale * kLog2e;
+  // Copies: piece wave + 4 i of the tile's 4 NL (key pieces of both sub-tiles, then values).
+  uint32_t off[FPW];
+#pragma unroll
+  for (int i = 0; i < FPW; ++i) {
+    const int p = wave + 4 * i, n = p % NL, s = p / NL % 2;
+    off[i] = p < 2 * NL ? pa_copy_off<RB>(n, lane, rb, [](int r) { return r & 7; })
+                        : pa_copy_off<RB>(n, lane, rb, [&](int r) { return pa_vxor<DT>(16 * s + r); });
+  }
+  PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * lane, k1);
+  PaIds ids2 = pa_ids(b, c, t.seq, k0 + 1024 + 16 * lane, k1);
+  auto row_of = [&](int kt, int s) {  // the sub-tile's first row in a pool
+    const int id = __builtin_amdgcn_readlane(ids.id, 2 * (kt & 31) + s);
+    return (((long)id * c.nkv + kvh) << c.ps_log) + ((k0 + 32 * kt + 16 * s) & (c.ps - 1));
+  };
+  PaScales q8n;
+  auto issue = [&](int kt) {
+    char* buf = lds + (kt & 1) * TILE;
+    const long at0 = row_of(kt, 0), at1 = row_of(kt, 1);
+#pragma unroll
+    for (int i = 0; i < FPW; ++i) {
+      const int p = wave + 4 * i;
+      const long at = (p / NL) % 2 ? at1 : at0;
+      const pa_rsrc_t r = pa_rsrc((p < 2 * NL ? c.k : c.v) + at * rb, 16 * rb);
+      mx_copy_to_lds16(r, buf + p * 1024, off[i]);
+    }
+    if constexpr (DT == MX_DT_I8) {
+      const long r0 = at0 + 4 * g, r1 = at1 + 4 * g;
+      q8n.ks[0] = *(const float4*)(c.ks + r0);
+      q8n.ks[1] = *(const float4*)(c.ks + r1);
+      q8n.vs[0] = *(const float4*)(c.vs + r0);
+      q8n.vs[1] = *(const float4*)(c.vs + r1);
+    }
+  };
+  if (ntile > 0) issue(0);
+  int on_next = (int)(ids.on & 3);
+
+  int pos[QS], tok[QS], hq[QS];
+  half8_t qf[QS][NC];
+  auto qdim = [&](int cc) { return DT == MX_DT_I8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g; };
+  const int w0 = t.row0 + wave * 16 * QS;  // the wave's first row
+#pragma unroll
+  for (int u = 0; u < QS; ++u) {
+    const int row = min(w0 + 16 * u + j, t.nrows - 1);
+    tok[u] = row / a.group;
+    hq[u] = kvh * a.group + row - tok[u] * a.group;
+    pos[u] = t.pos0 + tok[u];
+    const half_t* qrow = (const half_t*)a.q + (long)(t.first + tok[u]) * a.ldq + (long)hq[u] * c.hd;
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) qf[u][cc] = *(const half8_t*)(qrow + min(qdim(cc), c.hd - 8));
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc)
+      if (qdim(cc) >= c.hd) qf[u][cc] = (half8_t)(half_t)0.f;
+  }
+  // The keys that every row of the wave sees end at `all`, those that any sees at `any`.
+  const int lastrow = min(w0 + 16 * QS, t.nrows) - 1;
+  const int all = t.pos0 + min(w0, t.nrows - 1) / a.group;
+  const int any = min(t.pos0 + lastrow / a.group, t.kend - 1);
+  const int nt_w = w0 < t.nrows ? min(ntile, max(0, any + 1 - k0 + 31) / 32) : 0;
+
+  float4_t o[QS][NF];
+  float mrun[QS], lrun[QS];
+#pragma unroll
+  for (int u = 0; u < QS; ++u) {
+    mrun[u] = kLow;
+    lrun[u] = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[u][f] = (float4_t){0.f, 0.f, 0.f, 0.f};
+  }
+  const int klane = j * RB + ((g ^ (j & 7)) & (CPR - 1)) * 16;
+  const int vlane = pa_vlane<DT>(RB, lane);
+
+  auto advance = [&](int kt) {  // tile kt + 1 on its way
+    if (kt + 1 >= ntile) return;
+    if (((kt + 1) & 31) == 0) {
+      ids = ids2;
+      ids2 = pa_ids(b, c, t.seq, k0 + 32 * (kt + 33) + 16 * lane, k1);
+    }
+    issue(kt + 1);
+    on_next = (int)(ids.on >> (2 * ((kt + 1) & 31))) & 3;
+  };
+  int kt = 0;
+  for (; kt < nt_w; ++kt) {
+    mx_wait_copies_and_barrier<0>();
+    const int on = on_next;
+    const PaScales q8 = q8n;
+    advance(kt);
+    const int tk = k0 + 32 * kt;
+    const bool mask = tk + 31 > all || on != 3;
+    const char* kb = lds + (kt & 1) * TILE;
+    const char* vb = kb + 32 * RB;
+    auto kfrag = [&](int i) {  // step i: sub-tile i % 2, 16-byte piece i / 2
+      return *(const int4_t*)(kb + (i & 1) * 16 * RB + (klane ^ (64 * (i >> 1))));
+    };
+    float4_t sc[QS][2];
+#pragma unroll
+    for (int u = 0; u < QS; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) sc[u][s] = (float4_t){0.f, 0.f, 0.f, 0.f};
+    int4_t fr[PA_PD];
+#pragma unroll
+    for (int i = 0; i < PA_PD && i < 2 * NK; ++i) fr[i] = kfrag(i);
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i) {
+      const int4_t kf = fr[i % PA_PD];
+      if (i + PA_PD < 2 * NK) fr[i % PA_PD] = kfrag(i + PA_PD);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (DT == MX_DT_I8) {
+        half8_t lo, hi;
+        mx_i8_to_f16(kf, lo, hi);
+#pragma unroll
+        for (int u = 0; u < QS; ++u)
+          sc[u][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qf[u][2 * (i >> 1)], sc[u][i & 1], 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < QS; ++u)
+          sc[u][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qf[u][2 * (i >> 1) + 1], sc[u][i & 1], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < QS; ++u)
+          sc[u][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kf), qf[u][i >> 1],
+                                                                sc[u][i & 1], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    half8_t p[QS];
+    if (!mask) {
+#pragma unroll
+      for (int u = 0; u < QS; ++u) p[u] = pa_softmax<DT, false>(sc[u], rs, q8, 0, 3, mrun[u], lrun[u], o[u]);
+      half8_t vf = pa_vfrag<RB, DT>(vb, vlane, 0);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const half8_t v = vf;
+        if (f + 1 < NF) vf = pa_vfrag<RB, DT>(vb, vlane, f + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < QS; ++u)
+          o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < QS; ++u)
+        p[u] = pa_softmax<DT, true>(sc[u], rs, q8, pos[u] - tk - 4 * g, on, mrun[u], lrun[u], o[u]);
+      uint32_t keep[4], odd = 0;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
+        const bool ok = (on >> s) & 1;
+        keep[d] = (ok && k <= any - tk ? 0xFFFFu : 0u) | (ok && k + 1 <= any - tk ? 0xFFFF0000u : 0u);
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const half8_t v = pa_clean<DT>(pa_vfrag<RB, DT>(vb, vlane, f), keep, odd);
+#pragma unroll
+        for (int u = 0; u < QS; ++u)
+          o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (DT != MX_DT_I8)
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+          const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
+#pragma unroll
+          for (int u = 0; u < QS; ++u) pa_add_odd<RB, NF>(vb, p[u], pos[u] - tk, seen, o[u]);
+        }
+    }
+  }
+  for (; kt < ntile; ++kt) {
+    mx_wait_copies_and_barrier<0>();
+    advance(kt);
+  }
+#pragma unroll
+  for (int u = 0; u < QS; ++u) {
+    const float l = pa_rowsum(lrun[u]);
+    if (w0 + 16 * u + j >= t.nrows) continue;
+    const long tr = t.first + tok[u];
+    if (nsp > 1) {
+      const long at = ((long)z * b.rows + tr) * a.nh + hq[u];
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int d = 16 * f + 4 * g;
+        if (d < c.hd) *(float4_t*)(sp.po + at * c.hd + d) = o[u][f];
+      }
+      if (g == 0) sp.ml[at] = make_float2(mrun[u], l);
+      continue;
+    }
+    const float il = l == 0.f ? 0.f : 1.f / l;
+    const float* gate = a.gate ? a.gate + tr * a.ldg + (long)hq[u] * c.hd : nullptr;
+    half_t* orow = (half_t*)a.out + tr * a.ldo + (long)hq[u] * c.hd;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const int d = 16 * f + 4 * g;
+      if (d >= c.hd) continue;
+      float4_t v = o[u][f] * il;
+      if (gate) {
+        const float4 gv = *(const float4*)(gate + d);
+        v = (float4_t){v[0] * mx_sigmoid(gv.x), v[1] * mx_sigmoid(gv.y), v[2] * mx_sigmoid(gv.z),
+                       v[3] * mx_sigmoid(gv.w)};
+      }
+      *(half4_t*)(orow + d) = (half4_t){(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// k_pa_f32: fp32 pages on v_mfma_f32_16x16x4_f32 (full fp32 products and sums), k_pa_keys' way: 16
+// rows, keys dealt to the waves 16 at a time, keys in registers, values through the wave's LDS
+// buffers.  The MFMA k-slot of lane group g at step r is key 4 g + r on both operands.
+// ------------------------------------------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+  constexpr int RB = DP * 4, NC = DP / 16, NL = RB / 64, CPR = RB / 16;
+  constexpr int TILE = 16 * RB;
+  __shared__ __align__(1024) char lds[4 * 2 * TILE];
+  __shared__ float sm[4][16], sl[4][16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, z = blockIdx.z;
+  PaTile t;
+  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
+  if (!pa_find_tile<kKeysRows>(b, c, a.group, blockIdx.x, kmax, &t)) return;
+  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
+  if (k0 >= k1 && z > 0) return;
+  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+  const int row = min(t.row0 + j, t.nrows - 1);
+  const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
+  const int pos = t.pos0 + tok;
+  const int rb = c.hd * 4;
+  const float rs = a.scale * kLog2e;
+  float4 qf[NC];
+  const float* qrow = (const float*)a.q + (long)(t.first + tok) * a.ldq + (long)hq * c.hd;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) qf[n] = *(const float4*)(qrow + min(16 * n + 4 * g, c.hd - 4));
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+    if (16 * n + 4 * g >= c.hd) qf[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+  const int ntile = pa_ceil(max(0, k1 - k0), 16);
+  const int nw = ntile > wave ? (ntile - 1 - wave) / 4 + 1 : 0;
+  const PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * (wave + 4 * lane), k1);
+  char* const buf = lds + wave * 2 * TILE;
+  uint32_t voff[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    // rows of a copy: 64 / CPR; value chunks XORed by 4 (row / 4), so the four rows of a read
+    // lie in different banks
+    const int r = i * (64 / CPR) + lane / CPR;
+    voff[i] = (uint32_t)(r * rb + min(((lane % CPR) ^ ((r & 12) & (CPR - 1))) * 16, rb - 16));
+  }
+  auto base_of = [&](int i) {  // byte offset of the tile's first row in a pool
+    const int key = k0 + 16 * (wave + 4 * i);
+    const long row = (((long)__builtin_amdgcn_readlane(ids.id, i) * c.nkv + kvh) << c.ps_log) + (key & (c.ps - 1));
+    return row * rb;
+  };
+  auto issue_v = [&](int i) {
+    const pa_rsrc_t r = pa_rsrc(c.v + base_of(i), 16 * rb);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) mx_copy_to_lds16(r, buf + (i & 1) * TILE + n * 1024, voff[n]);
+  };
+  float4 kr[NC];
+  auto load_k = [&](int i) {
+    const char* p = c.k + base_of(i);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) kr[n] = *(const float4*)(p + (uint32_t)(j * rb + min(64 * n + 16 * g, rb - 16)));
+  };
+  // value of key 4 g + r, dim 16 f + j
+  const int vlane = 4 * g * RB + (((j >> 2) ^ ((4 * g) & (CPR - 1))) * 16) + 4 * (j & 3);
+  float4_t o[NC];
+#pragma unroll
+  for (int f = 0; f < NC; ++f) o[f] = (float4_t){0.f, 0.f, 0.f, 0.f};
+  float mrun = kLow, lrun = 0.f;
+  const int all = t.pos0 + t.row0 / a.group;
+  if (nw > 0) {
+    issue_v(0);
+    load_k(0);
+  }
+  for (int i = 0; i < nw; ++i) {
+    if (i + 1 < nw) issue_v(i + 1);
+    float4_t x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      x[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[n].x, qf[n].x, x[0], 0, 0, 0);
+      x[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[n].y, qf[n].y, x[1], 0, 0, 0);
+      x[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[n].z, qf[n].z, x[2], 0, 0, 0);
+      x[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[n].w, qf[n].w, x[3], 0, 0, 0);
+    }
+    const float4_t sc = (x[0] + x[1]) + (x[2] + x[3]);
+    const int tk = k0 + 16 * (wave + 4 * i);
+    const bool on = (ids.on >> i) & 1;
+    if (i + 1 < nw) load_k(i + 1);
+    const bool mask = tk + 15 > all || !on;
+    const int lim = pos - tk;
+    float4_t s = sc * rs;
+    if (mask) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * g + r > lim || !on) s[r] = -INFINITY;
+    }
+    const float mt = pa_rowmax(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const bool up = mt > mrun + kTau;
+    if (__builtin_amdgcn_ballot_w64(up)) {
+      const float mnew = up ? mt : mrun;
+      const float alpha = __builtin_amdgcn_exp2f(mrun - mnew);
+      lrun *= alpha;
+      mrun = mnew;
+#pragma unroll
+      for (int f = 0; f < NC; ++f) o[f] *= alpha;
+    }
+    float4_t p;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(s[r] - mrun);
+    lrun += (p[0] + p[1]) + (p[2] + p[3]);
+    if (i + 1 < nw) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(p) : "n"(NL + NC) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" : "+v"(p) : : "memory");
+    const char* tile = buf + (i & 1) * TILE;
+    const int top = t.kend - 1 - tk;  // the last key any row sees
+    bool odd = false;
+#pragma unroll
+    for (int f = 0; f < NC; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = *(const float*)(tile + (vlane ^ (f * 64)) + r * RB);
+        if (mask) {
+          const bool fin = (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u;
+          const bool in = on && 4 * g + r <= top;
+          odd |= in && !fin;
+          v = in && fin ? v : 0.f;
+        }
+        o[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[r], o[f], 0, 0, 0);
+      }
+    if (__builtin_amdgcn_ballot_w64(odd)) {  // non-finite values that only some rows see
+      for (int key = 0; key < 16; ++key) {
+        const int e = key & 3;
+        const float pe = e == 0 ? p[0] : e == 1 ? p[1] : e == 2 ? p[2] : p[3];
+        const float pk = __shfl(pe, (key >> 2) * 16 + j);
+        const int x16 = ((key & 12) & (CPR - 1)) * 16;
+#pragma unroll
+        for (int f = 0; f < NC; ++f) {
+          const float4_t v = *(const float4_t*)(tile + key * RB + ((64 * f + 16 * g) ^ x16));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool bad = (__builtin_bit_cast(uint32_t, v[r]) & 0x7F800000u) == 0x7F800000u;
+            if (bad && key <= lim) o[f][r] += pk * v[r];
+          }
+        }
+      }
+    }
+  }
+  lrun = pa_rowsum(lrun);
+  if (g == 0) {
+    sm[wave][j] = mrun;
+    sl[wave][j] = lrun;
+  }
+  __syncthreads();
+  const float m = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j]));
+  const float mine = __builtin_amdgcn_exp2f(mrun - m);
+  float* const part = (float*)buf;
+#pragma unroll
+  for (int f = 0; f < NC; ++f) {
+    const float4_t v = o[f] * mine;
+    *(float4_t*)(part + j * DP + 16 * f + 4 * g) = v;
+  }
+  __syncthreads();
+  constexpr int D4 = DP / 4;
+  for (int i = tid; i < 16 * D4; i += 256) {
+    const int r = i / D4, d = 4 * (i % D4);
+    if (t.row0 + r >= t.nrows || d >= c.hd) continue;
+    float4_t s = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f, mr = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      s += *(const float4_t*)((const float*)(lds + w * 2 * TILE) + r * DP + d);
+      l += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mr);
+    }
+    const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
+    const long tr = t.first + rt;
+    if (nsp > 1) {
+      const long at = ((long)z * b.rows + tr) * a.nh + h;
+      *(float4_t*)(sp.po + at * c.hd + d) = s;
+      if (d == 0) sp.ml[at] = make_float2(mr, l);
+      continue;
+    }
+    s *= l == 0.f ? 0.f : 1.f / l;
+    if (a.gate) {
+      const float4 gv = *(const float4*)(a.gate + tr * a.ldg + (long)h * c.hd + d);
+      s = (float4_t){s[0] * mx_sigmoid(gv.x), s[1] * mx_sigmoid(gv.y), s[2] * mx_sigmoid(gv.z),
+                     s[3] * mx_sigmoid(gv.w)};
+    }
+    *(float4_t*)((float*)a.out + tr * a.ldo + (long)h * c.hd + d) = s;
+  }
+}
+
+// ---- the launch ----------------------------------------------------------------------
+
+enum PaKind { kKeys, kRows1, kRows2, kF32 };
+
+struct PaPlan {
+  PaKind kind;
+  int rt, ntiles;  // rows per tile, at most so many tiles
+  int len, n;      // keys per split, splits
+  size_t bytes;    // workspace
+};
+
+// Kernel, row tile and key split of a call, from its sizes alone.
+int plan(const MxKvCache* c, const MxPagedBatch* b, int nh, PaPlan* p) {
+  const int group = nh / c->n_kv_heads;
+  const long max_q = b->max_q < b->rows ? b->max_q : b->rows;
+  const long seqs = b->n_seqs, rows = (long)b->rows * group;
+  if (rows >= (1l << 30)) return MX_ERR_UNSUPPORTED;
+  p->kind = c->dtype == MX_DT_F32 ? kF32 : max_q * group <= kKeysRows ? kKeys : kRows1;
+  if (p->kind == kRows1 && (rows / 128 + seqs) * c->n_kv_heads >= 256) p->kind = kRows2;
+  p->rt = p->kind == kRows1 ? 64 : p->kind == kRows2 ? 128 : kKeysRows;
+  const long tiles = max_q * group <= p->rt ? seqs : rows / p->rt + seqs;
+  if (tiles * c->n_kv_heads >= (1l << 24)) return MX_ERR_UNSUPPORTED;
+  p->ntiles = (int)tiles;
+  const long blocks = tiles * c->n_kv_heads;
+  const bool own = p->kind == kKeys || p->kind == kF32;
+  const long want = own ? 1024 : 512;     // blocks
+  const long least = own ? 256 : 1024;    // keys of a split
+  const long keys = b->max_kv > 0 ? b->max_kv : 1;
+  long n = blocks < want ? (want + blocks - 1) / blocks : 1;
+  long len = (keys + n - 1) / n;
+  if (len < least) len = least;
+  if (own && len > kKeysMax) len = kKeysMax;
+  len = (len + 127) / 128 * 128;
+  n = (keys + len - 1) / len;
+  if (n > 65535) return MX_ERR_UNSUPPORTED;
+  p->len = (int)len;
+  p->n = (int)n;
+  p->bytes = 0;
+  if (n > 1) p->bytes = mx_align_up((size_t)n * b->rows * nh * c->head_dim * 4, 256) + (size_t)n * b->rows * nh * 8;
+  return MX_OK;
+}
+
+template <int DT>
+int launch(const PaPlan& p, const PkCache& c, const PkBatch& b, const PaArgs& a, const PaSplit& sp, hipStream_t s) {
+  const dim3 grid(p.ntiles, c.nkv, p.n);
+  mx_clear_error();
+  if constexpr (DT == MX_DT_F32) {
+    auto* kern = c.hd <= 32 ? k_pa_f32<32> : c.hd <= 64 ? k_pa_f32<64> : c.hd <= 128 ? k_pa_f32<128> : k_pa_f32<256>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp);
+  } else {
+    constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
+    const int rb = c.hd * ES;
+    if (p.kind == kKeys) {
+      auto* kern = rb <= 64 ? k_pa_keys<64, DT> : rb <= 128 ? k_pa_keys<128, DT> : k_pa_keys<256, DT>;
+      if constexpr (ES == 2)
+        if (rb > 256) kern = k_pa_keys<512, DT>;
+      hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp);
+    } else {
+      // blocks of a head's XCDs come in whole rounds
+      const int nb = 8 % c.nkv == 0   ? 8 * mx_ceil_div(p.ntiles, 8 / c.nkv)
+                     : c.nkv % 8 == 0 ? p.ntiles * c.nkv
+                                      : p.ntiles * c.nkv;
+      auto* kern = p.kind == kRows1
+                       ? (rb <= 64 ? k_pa_rows<64, DT, 1> : rb <= 128 ? k_pa_rows<128, DT, 1> : k_pa_rows<256, DT, 1>)
+                       : (rb <= 64 ? k_pa_rows<64, DT, 2> : rb <= 128 ? k_pa_rows<128, DT, 2> : k_pa_rows<256, DT, 2>);
+      if constexpr (ES == 2)
+        if (rb > 256) kern = p.kind == kRows1 ? k_pa_rows<512, DT, 1> : k_pa_rows<512, DT, 2>;
+      hipLaunchKernelGGL(kern, dim3(nb, 1, p.n), dim3(256), 0, s, c, b, a, sp, p.ntiles);
+    }
+  }
+  MX_TRY(mx_launch_status());
+  if (p.n == 1) return MX_OK;
+  typedef typename std::conditional<DT == MX_DT_F32, float, half_t>::type OT;
+  auto* join = p.rt == 64 ? k_pa_join<64, OT> : p.rt == 128 ? k_pa_join<128, OT> : k_pa_join<16, OT>;
+  hipLaunchKernelGGL(join, dim3((unsigned)(((long)b.rows * a.nh + 3) / 4)), dim3(256), 0, s, c, b, a, sp);
+  return mx_launch_status();
 }
 
 int check(const MxKvCache* cache, const MxPagedBatch* batch, int n_heads) {
   MX_TRY(pk_check_cache(cache));
   MX_TRY(pk_check_batch(batch));
   if (n_heads <= 0 || n_heads % cache->n_kv_heads) return MX_ERR_INVALID;
-  return n_heads > 65535 ? MX_ERR_UNSUPPORTED : MX_OK;
+  return n_heads > 65535 || (long)n_heads * batch->rows >= (1l << 26) ? MX_ERR_UNSUPPORTED : MX_OK;
 }
 
 }  // namespace
@@ -82,6 +1119,10 @@ extern "C" int mx_paged_attn_workspace_size(const MxKvCache* cache, const MxPage
   if (!nbytes) return MX_ERR_INVALID;
   MX_TRY(check(cache, batch, n_heads));
   *nbytes = 0;
+  if (batch->rows == 0 || batch->n_seqs == 0) return MX_OK;
+  PaPlan p;
+  MX_TRY(plan(cache, batch, n_heads, &p));
+  *nbytes = p.bytes;
   return MX_OK;
 }
 
@@ -97,15 +1138,20 @@ extern "C" int mx_paged_attn(const MxKvCache* cache, const MxPagedBatch* batch,
       args->ldq * esz % 16 || args->ldo * esz % 16 || (args->gate && args->ldg * 4 % 16))
     return MX_ERR_ALIGNMENT;
   if (batch->rows == 0 || batch->n_seqs == 0) return MX_OK;
+  PaPlan p;
+  MX_TRY(plan(cache, batch, args->n_heads, &p));
+  if (p.bytes) {
+    if (!workspace || workspace_bytes < p.bytes) return MX_ERR_WORKSPACE;
+    if (!mx_aligned16(workspace)) return MX_ERR_ALIGNMENT;
+  }
   const PkCache c = pk_cache(cache);
   const PkBatch b = pk_batch(batch);
   const PaArgs a{args->q, args->out, args->gate, args->ldq, args->ldo, args->ldg, args->n_heads,
                  args->n_heads / cache->n_kv_heads, args->scale};
+  const size_t ml = mx_align_up((size_t)p.n * b.rows * a.nh * c.hd * 4, 256);
+  const PaSplit sp{p.len, p.n, (float*)workspace, (float2*)((char*)workspace + ml)};
   const hipStream_t s = (hipStream_t)stream;
-  auto* kern = cache->dtype == MX_DT_F32   ? k_pa_simple<float, MX_DT_F32>
-               : cache->dtype == MX_DT_F16 ? k_pa_simple<half_t, MX_DT_F16>
-                                           : k_pa_simple<half_t, MX_DT_I8>;
-  mx_clear_error();
-  hipLaunchKernelGGL(kern, dim3(b.rows, a.nh), dim3(64), 0, s, c, b, a);
-  return mx_launch_status();
+  return cache->dtype == MX_DT_F32   ? launch<MX_DT_F32>(p, c, b, a, sp, s)
+         : cache->dtype == MX_DT_F16 ? launch<MX_DT_F16>(p, c, b, a, sp, s)
+                                     : launch<MX_DT_I8>(p, c, b, a, sp, s);
 }
