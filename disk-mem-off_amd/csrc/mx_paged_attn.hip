@@ -159,14 +159,14 @@ __device__ __forceinline__ half8_t pa_i8x8(int2_t v) {
 // chunks permuted by an XOR so that the fragment reads use every bank once: 8 lanes of a
 // 16-byte read take one chunk of 8 consecutive rows (keys: chunk ^ row % 8), 16 lanes of an 8-byte
 // transposing read take 32 bytes of 4 rows (fp16 values: chunk ^ 2 (row % 4)) or 16 bytes of 8
-// rows (int8 values: chunk ^ the row's number among the 16 that two groups of lanes read).
+// rows (int8 values: chunk ^ the row's number among those 8).
 // A copy instruction fills 1 KiB, whole rows: the permutation stays inside a row, so it reads
 // whole rows of the page in order.  Rows of fewer than RB bytes: the chunks past the row repeat
 // its last one (the queries are zero there, and no output is stored).
 // ------------------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ int pa_vxor(int row) {  // row of the 32
-  if constexpr (DT == MX_DT_I8) return (row & 3) | ((row >> 4) & 1) << 2 | ((row >> 2) & 1) << 3;
+  if constexpr (DT == MX_DT_I8) return (row & 3) | ((row >> 4) & 1) << 2;
   return 2 * (row & 3);
 }
 
@@ -180,29 +180,46 @@ __device__ __forceinline__ uint32_t pa_copy_off(int i, int lane, int rb, X x) {
   return (uint32_t)(row * rb + min(chunk * 16, rb - 16));
 }
 
-// One lane's value fragment f (16 dims x 32 keys) of a tile at byte offset `base` of the wave's
-// LDS: the XOR of the chunk number is the XOR of address bits, rows are RB-aligned.
-template <int DT>
-__device__ __forceinline__ int pa_vlane(int rb_pad, int lane) {
-  const int j = lane & 15, g = lane >> 4;
-  if constexpr (DT == MX_DT_I8) {
-    const int rr = j >> 1, row = rr < 4 ? 4 * g + rr : 16 + 4 * g + rr - 4;
-    return row * rb_pad + ((pa_vxor<DT>(row) * 16) & (rb_pad - 1)) + 8 * (j & 1);
-  }
-  const int row = 4 * g + (j >> 2);
-  return row * rb_pad + (((pa_vxor<DT>(row) + ((j & 3) >> 1)) * 16) & (rb_pad - 1)) + 8 * (j & 1);
+// A register's value the compiler knows nothing of: what is worked out from it is worked out
+// here, per tile, and holds no registers across the loop.
+__device__ __forceinline__ int pa_opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
+
+// One lane's reads of a tile's value fragments (16 dims x 32 keys each): the XOR touches the low
+// bits of a fragment's number only, so a few addresses and constant offsets serve all of
+// them.
+template <int RB, int DT>
+struct PaV {
+  static constexpr int STEP = DT == MX_DT_I8 ? 16 : 32;       // bytes of a fragment in a row
+  static constexpr int NB = (DT == MX_DT_I8 ? 8 : 4) * STEP <= RB ? (DT == MX_DT_I8 ? 8 : 4) : RB / STEP;
+  const char* at[NB];
+  // The lane's place in a tile, fragment 0 (the others: an XOR with f STEP).
+  static __device__ __forceinline__ int lane_at(int lane) {
+    const int j = lane & 15, g = lane >> 4;
+    const int rr = j >> 1;
+    const int row = DT == MX_DT_I8 ? (rr < 4 ? 4 * g + rr : 16 + 4 * g + rr - 4) : 4 * g + (j >> 2);
+    const int chunk = DT == MX_DT_I8 ? 0 : (j & 3) >> 1;
+    return row * RB + ((chunk ^ pa_vxor<DT>(row)) & (RB / 16 - 1)) * 16 + 8 * (j & 1);
+  }
+  __device__ __forceinline__ PaV(const char* tile, int lane_at) {
+    const int v = pa_opaque(lane_at);
+#pragma unroll
+    for (int e = 0; e < NB; ++e) at[e] = tile + (v ^ (e * STEP));
+  }
+  __device__ __forceinline__ const char* operator()(int f) const { return at[f % NB] + f / NB * NB * STEP; }
+};
 
 typedef __attribute__((address_space(3))) short4_t pa_lds_s4;
 typedef __attribute__((address_space(3))) int2_t pa_lds_i2;
 
 template <int RB, int DT>
-__device__ __forceinline__ half8_t pa_vfrag(const char* tile, int vlane, int f) {
+__device__ __forceinline__ half8_t pa_vfrag(const PaV<RB, DT>& vl, int f) {
+  const char* p = vl(f);
   if constexpr (DT == MX_DT_I8) {
-    const int2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((pa_lds_i2*)(tile + (vlane ^ (f * 16))));
-    return pa_i8x8(v);
+    return pa_i8x8(__builtin_amdgcn_ds_read_tr8_b64_v2i32((pa_lds_i2*)p));
   } else {
-    const char* p = tile + (vlane ^ (f * 32));
     const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)p);
     const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)(p + 16 * RB));
     const half4_t x = __builtin_bit_cast(half4_t, a), y = __builtin_bit_cast(half4_t, b);
@@ -234,25 +251,28 @@ __device__ __forceinline__ half8_t pa_clean(half8_t v, const uint32_t (&keep)[4]
 // that the lane's row sees; seen: keys on a page (bit per key).
 template <int RB, int NF>
 __device__ __forceinline__ void pa_add_odd(const char* tile, half8_t p, int lim, uint32_t seen,
-                                        float4_t (&o)[NF]) {
-  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+                                           float4_t (&o)[NF]) {
+  const int4_t pi = __builtin_bit_cast(int4_t, p);
+#pragma nounroll
   for (int key = 0; key < 32; ++key) {
     if (!((seen >> key) & 1)) continue;
-    const int src = ((key & 15) >> 2) * 16 + j, e = (key >> 4) * 4 + (key & 3);
-    half_t pe = p[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) pe = i == e ? p[i] : pe;
-    const float pk = __shfl((float)pe, src);
-    const int row = key * RB, x = pa_vxor<MX_DT_F16>(key) * 16;
+    const int lane = pa_opaque(threadIdx.x & 63), j = lane & 15, g = lane >> 4;
+    const int src = ((key & 15) >> 2) * 16 + j, d = (key >> 4) * 2 + ((key >> 1) & 1);
+    const int pw = __shfl(d == 0 ? pi[0] : d == 1 ? pi[1] : d == 2 ? pi[2] : pi[3], src);
+    const half2_t ph = __builtin_bit_cast(half2_t, pw);
+    const float pk = key <= lim ? (float)((key & 1) ? ph[1] : ph[0]) : 0.f;
+    // dims 16 f + 4 g ..: chunk 2 f + g / 2, its half g % 2
+    const char* row = tile + key * RB + 8 * (g & 1);
+    const int x = pa_vxor<MX_DT_F16>(key) * 16 ^ 16 * (g >> 1);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-      // dims 16 f + 4 g ..: chunk 2 f + g / 2, its half g % 2
-      const half4_t v = *(const half4_t*)(tile + row + (((32 * f + 16 * (g >> 1)) ^ x) & (RB - 1)) + 8 * (g & 1));
+      const half4_t v = *(const half4_t*)(row + ((32 * f ^ pa_opaque(x)) & (RB - 1)));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const bool bad = (__builtin_bit_cast(unsigned short, v[r]) & 0x7C00) == 0x7C00;
         if (bad && key <= lim) o[f][r] += pk * (float)v[r];
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -343,7 +363,8 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16;
   constexpr int NL = RB / 64;             // 1 KiB pieces per 16 rows
   constexpr int TILE = 32 * RB;
-  __shared__ __align__(1024) char lds[4 * 2 * TILE];
+  __shared__ __align__(1024) char lds0[4 * TILE];  // one variable per buffer (see k_pa_rows)
+  __shared__ __align__(1024) char lds1[4 * TILE];
   __shared__ float sm[4][16], sl[4][16];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -361,7 +382,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
   const int pos = t.pos0 + tok;
   const int rb = c.hd * ES;
-  const float rs = a.scale * kLog2e;
+  const float rs = mx_readlane(a.scale * kLog2e, 0);  // uniform: a scalar register
 
   // Queries: B fragments.  Fp16 pages: chunk cc holds dims 32 cc + 8 g ..; int8 pages (16 dims per
   // 16-byte load): chunk pair (2 i, 2 i + 1) dims 64 i + 16 g .. + 7 and + 8 .. + 15.
@@ -378,7 +399,8 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   const int nw = ntile > wave ? (ntile - 1 - wave) / 4 + 1 : 0;
   // lane l: the page of sub-tile l % 2 of the wave's tile l / 2
   const PaIds ids = pa_ids(b, c, t.seq, k0 + 32 * (wave + 4 * (lane >> 1)) + 16 * (lane & 1), k1);
-  char* const buf = lds + wave * 2 * TILE;
+  char* const buf0 = lds0 + wave * TILE;
+  char* const buf1 = lds1 + wave * TILE;
   uint32_t voff[NL][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -390,13 +412,12 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     const int key = k0 + 32 * (wave + 4 * i) + 16 * s;
     return (((long)id * c.nkv + kvh) << c.ps_log) + (key & (c.ps - 1));
   };
-  auto issue_v = [&](int i) {
+  auto issue_v = [&](int i, char* buf) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const pa_rsrc_t r = pa_rsrc(c.v + row_of(i, s) * rb, 16 * rb);
 #pragma unroll
-      for (int n = 0; n < NL; ++n)
-        mx_copy_to_lds16(r, buf + (i & 1) * TILE + s * 16 * RB + n * 1024, voff[n][s]);
+      for (int n = 0; n < NL; ++n) mx_copy_to_lds16(r, buf + s * 16 * RB + n * 1024, voff[n][s]);
     }
   };
   constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte loads per key row and lane
@@ -415,7 +436,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
       }
     }
   };
-  const int vlane = pa_vlane<DT>(RB, lane);
+  const int vlane = PaV<RB, DT>::lane_at(lane);
   float4_t o[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) o[f] = (float4_t){0.f, 0.f, 0.f, 0.f};
@@ -423,13 +444,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
 
   // The last key that every row of the tile sees (rows past the last repeat it).
   const int all = t.pos0 + t.row0 / a.group;
-  if (nw > 0) {
-    issue_v(0);
-    load_k(0);
-  }
-  for (int i = 0; i < nw; ++i) {
-    if (i + 1 < nw) issue_v(i + 1);
-    float4_t sc[2];
+  auto scores = [&](float4_t (&sc)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       float4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -447,44 +462,67 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
       }
       sc[s] = x[0] + x[1];
     }
+  };
+  // A tile with a tile behind it that every row sees whole.  The next tile's copies and loads are
+  // issued without a branch, so the waits for this tile's leave them in flight.
+  auto whole = [&](const char* tile, char* next, int i) {
+    issue_v(i + 1, next);
+    float4_t sc[2];
+    scores(sc);
+    const PaScales w8 = q8;
+    load_k(i + 1);
+    half8_t p = pa_softmax<DT, false>(sc, rs, w8, 0, 3, mrun, lrun, o);
+    // This tile's values have landed (they were issued before its keys).
+    int4_t pw = __builtin_bit_cast(int4_t, p);
+    asm volatile("s_waitcnt vmcnt(%1)" : "+v"(pw) : "n"(2 * NL + 2 * NK) : "memory");
+    p = __builtin_bit_cast(half8_t, pw);
+    const PaV<RB, DT> vt(tile, vlane);
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(vt, f), p, o[f], 0, 0, 0);
+  };
+  if (nw > 0) {
+    issue_v(0, buf0);
+    load_k(0);
+  }
+  int i = 0;
+  auto plain = [&]() {  // tiles i and i + 1
+    return k0 + 32 * (wave + 4 * i + 4) + 31 <= all && ((ids.on >> (2 * i)) & 15) == 15;
+  };
+  for (; i + 2 < nw && plain(); i += 2) {
+    whole(buf0, buf1, i);
+    whole(buf1, buf0, i + 1);
+  }
+  for (; i < nw; ++i) {
+    char* const tile = i & 1 ? buf1 : buf0;
+    if (i + 1 < nw) issue_v(i + 1, i & 1 ? buf0 : buf1);
+    float4_t sc[2];
+    scores(sc);
     const PaScales w8 = q8;
     const int tk = k0 + 32 * (wave + 4 * i);  // first key of the tile
     const int on = (int)(ids.on >> (2 * i)) & 3;
     if (i + 1 < nw) load_k(i + 1);
-    const bool mask = tk + 31 > all || on != 3;
     const int lim = pos - tk;
-    half8_t p;
-    if (mask) p = pa_softmax<DT, true>(sc, rs, w8, lim - 4 * g, on, mrun, lrun, o);
-    else p = pa_softmax<DT, false>(sc, rs, w8, lim, on, mrun, lrun, o);
-    // This tile's values have landed; the next tile's copies and key loads may be in flight.
-    int4_t pw = __builtin_bit_cast(int4_t, p);
-    if (i + 1 < nw) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(pw) : "n"(2 * NL + 2 * NK) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" : "+v"(pw) : : "memory");
-    p = __builtin_bit_cast(half8_t, pw);
-    const char* tile = buf + (i & 1) * TILE;
-    if (!mask) {
+    const half8_t p = pa_softmax<DT, true>(sc, rs, w8, lim - 4 * g, on, mrun, lrun, o);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const PaV<RB, DT> vt(tile, vlane);
+    const int top = t.kend - 1 - tk;  // the last key any row sees
+    uint32_t keep[4], odd = 0;
 #pragma unroll
-      for (int f = 0; f < NF; ++f)
-        o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(tile, vlane, f), p, o[f], 0, 0, 0);
-    } else {
-      const int top = min(t.kend - 1, 1 << 30) - tk;  // the last key any row sees
-      uint32_t keep[4], odd = 0;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
-        const bool ok = (on >> s) & 1;
-        keep[d] = (ok && k <= top ? 0xFFFFu : 0u) | (ok && k + 1 <= top ? 0xFFFF0000u : 0u);
-      }
-#pragma unroll
-      for (int f = 0; f < NF; ++f)
-        o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<DT>(pa_vfrag<RB, DT>(tile, vlane, f), keep, odd),
-                                                      p, o[f], 0, 0, 0);
-      if constexpr (DT != MX_DT_I8)
-        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-          const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
-          pa_add_odd<RB, NF>(tile, p, lim, seen, o);
-        }
+    for (int d = 0; d < 4; ++d) {
+      const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
+      const bool ok = (on >> s) & 1;
+      keep[d] = (ok && k <= top ? 0xFFFFu : 0u) | (ok && k + 1 <= top ? 0xFFFF0000u : 0u);
     }
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<DT>(pa_vfrag<RB, DT>(vt, f), keep, odd), p, o[f],
+                                                    0, 0, 0);
+    if constexpr (DT != MX_DT_I8)
+      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+        const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
+        pa_add_odd<RB, NF>(tile, p, lim, seen, o);
+      }
   }
   lrun = pa_rowsum(lrun);
 
@@ -496,8 +534,11 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   __syncthreads();
   const float m = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j]));
   const float mine = __builtin_amdgcn_exp2f(mrun - m);
-  float* const part = (float*)(lds + wave * 2 * TILE);  // [16 rows][DP], the wave's own buffers
-  static_assert(16 * DP * 4 <= 2 * TILE, "the sums fit the wave's buffers");
+  // [16 rows][DP] per wave: waves 0, 1 in the first buffer, 2, 3 in the second
+  static_assert(2 * 16 * DP * 4 <= 4 * TILE, "the sums fit the buffers");
+  auto part_of = [&](int w) { return (float*)(w < 2 ? lds0 : lds1) + (w & 1) * 16 * DP; };
+  __syncthreads();
+  float* const part = part_of(wave);
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const float4_t v = o[f] * mine;
@@ -512,7 +553,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     float l = 0.f, mr = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      s += *(const float4_t*)((const float*)(lds + w * 2 * TILE) + r * DP + d);
+      s += *(const float4_t*)(part_of(w) + r * DP + d);
       l += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mr);
     }
     const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
@@ -600,7 +641,10 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   constexpr int TILE = 64 * RB;           // keys, then values
   constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte fragment reads per key row and lane
   constexpr int RT = 64 * QS;
-  __shared__ __align__(1024) char lds[2 * TILE];
+  // One variable per buffer: the compiler then knows that a read of one does not wait for copies
+  // into the other (a transposing read waits for every copy it may meet).
+  __shared__ __align__(1024) char lds0[TILE];
+  __shared__ __align__(1024) char lds1[TILE];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -633,15 +677,15 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   const int ntile = pa_ceil(max(0, k1 - k0), 32);
 
   const int rb = c.hd * ES;
-  const float rs = a.scale * kLog2e;
-  // Copies: piece wave + 4 i of the tile's 4 NL (key pieces of both sub-tiles, then values).
-  uint32_t off[FPW];
-#pragma unroll
-  for (int i = 0; i < FPW; ++i) {
-    const int p = wave + 4 * i, n = p % NL, s = p / NL % 2;
-    off[i] = p < 2 * NL ? pa_copy_off<RB>(n, lane, rb, [](int r) { return r & 7; })
-                        : pa_copy_off<RB>(n, lane, rb, [&](int r) { return pa_vxor<DT>(16 * s + r); });
-  }
+  const float rs = mx_readlane(a.scale * kLog2e, 0);  // uniform: a scalar register
+  // Copies: piece wave + 4 i of the tile's 4 NL (key pieces of both sub-tiles, then values).  A
+  // wave's pieces of a sub-tile (NL > 4: two) are 4 pieces, 8 rows, apart: the same lane
+  // offsets.  Int8 values' XOR depends on the sub-tile.
+  const int n0 = wave % NL;
+  const uint32_t offk = pa_copy_off<RB>(n0, lane, rb, [](int r) { return r & 7; });
+  uint32_t offv[2];
+  offv[0] = pa_copy_off<RB>(n0, lane, rb, [](int r) { return pa_vxor<DT>(r); });
+  offv[1] = DT == MX_DT_I8 ? pa_copy_off<RB>(n0, lane, rb, [](int r) { return pa_vxor<DT>(16 + r); }) : offv[0];
   PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * lane, k1);
   PaIds ids2 = pa_ids(b, c, t.seq, k0 + 1024 + 16 * lane, k1);
   auto row_of = [&](int kt, int s) {  // the sub-tile's first row in a pool
@@ -649,15 +693,17 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     return (((long)id * c.nkv + kvh) << c.ps_log) + ((k0 + 32 * kt + 16 * s) & (c.ps - 1));
   };
   PaScales q8n;
-  auto issue = [&](int kt) {
-    char* buf = lds + (kt & 1) * TILE;
+  auto issue = [&](int kt, char* buf) {
     const long at0 = row_of(kt, 0), at1 = row_of(kt, 1);
 #pragma unroll
     for (int i = 0; i < FPW; ++i) {
-      const int p = wave + 4 * i;
-      const long at = (p / NL) % 2 ? at1 : at0;
-      const pa_rsrc_t r = pa_rsrc((p < 2 * NL ? c.k : c.v) + at * rb, 16 * rb);
-      mx_copy_to_lds16(r, buf + p * 1024, off[i]);
+      // piece wave + 4 i: key or value, its sub-tile, its rows (8 behind the lane offset's, or not)
+      const bool key = NL >= 2 ? i < FPW / 2 : wave < 2;
+      const bool second = NL >= 4 ? (4 * i / NL) % 2 : NL == 2 ? wave >= 2 : wave & 1;
+      const int more = NL > 4 && (4 * i) % NL >= 4 ? 8 * rb : 0;
+      const pa_rsrc_t r = pa_rsrc((key ? c.k : c.v) + (second ? at1 : at0) * rb, 16 * rb);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (mx_lds_void*)(buf + (wave + 4 * i) * 1024), 16,
+                                               key ? offk : second ? offv[1] : offv[0], more, 0, 0);
     }
     if constexpr (DT == MX_DT_I8) {
       const long r0 = at0 + 4 * g, r1 = at1 + 4 * g;
@@ -667,20 +713,24 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
       q8n.vs[1] = *(const float4*)(c.vs + r1);
     }
   };
-  if (ntile > 0) issue(0);
+  if (ntile > 0) issue(0, lds0);
   int on_next = (int)(ids.on & 3);
 
-  int pos[QS], tok[QS], hq[QS];
   half8_t qf[QS][NC];
   auto qdim = [&](int cc) { return DT == MX_DT_I8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g; };
   const int w0 = t.row0 + wave * 16 * QS;  // the wave's first row
+  // Token (of the sequence) and head of the lane's row in set u: worked out where they are needed,
+  // behind a barrier to the compiler, so that they hold no registers in between.
+  auto where = [&](int u, int& tok, int& hq) {
+    const int row = min(w0 + 16 * u + pa_opaque(j), t.nrows - 1);
+    tok = row / a.group;
+    hq = kvh * a.group + row - tok * a.group;
+  };
 #pragma unroll
   for (int u = 0; u < QS; ++u) {
-    const int row = min(w0 + 16 * u + j, t.nrows - 1);
-    tok[u] = row / a.group;
-    hq[u] = kvh * a.group + row - tok[u] * a.group;
-    pos[u] = t.pos0 + tok[u];
-    const half_t* qrow = (const half_t*)a.q + (long)(t.first + tok[u]) * a.ldq + (long)hq[u] * c.hd;
+    int tok, hq;
+    where(u, tok, hq);
+    const half_t* qrow = (const half_t*)a.q + (long)(t.first + tok) * a.ldq + (long)hq * c.hd;
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) qf[u][cc] = *(const half8_t*)(qrow + min(qdim(cc), c.hd - 8));
 #pragma unroll
@@ -702,32 +752,26 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[u][f] = (float4_t){0.f, 0.f, 0.f, 0.f};
   }
+  // key piece n of a row lies at (klane ^ 64 (n % 2)) + 64 (n - n % 2)
   const int klane = j * RB + ((g ^ (j & 7)) & (CPR - 1)) * 16;
-  const int vlane = pa_vlane<DT>(RB, lane);
+  const int vlane = PaV<RB, DT>::lane_at(lane);
 
-  auto advance = [&](int kt) {  // tile kt + 1 on its way
-    if (kt + 1 >= ntile) return;
+  auto advance = [&](int kt, char* buf) {  // tile kt + 1 (there is one) on its way
     if (((kt + 1) & 31) == 0) {
       ids = ids2;
       ids2 = pa_ids(b, c, t.seq, k0 + 32 * (kt + 33) + 16 * lane, k1);
     }
-    issue(kt + 1);
+    issue(kt + 1, buf);
     on_next = (int)(ids.on >> (2 * ((kt + 1) & 31))) & 3;
   };
-  int kt = 0;
-  for (; kt < nt_w; ++kt) {
-    mx_wait_copies_and_barrier<0>();
-    const int on = on_next;
-    const PaScales q8 = q8n;
-    advance(kt);
-    const int tk = k0 + 32 * kt;
-    const bool mask = tk + 31 > all || on != 3;
-    const char* kb = lds + (kt & 1) * TILE;
-    const char* vb = kb + 32 * RB;
-    auto kfrag = [&](int i) {  // step i: sub-tile i % 2, 16-byte piece i / 2
-      return *(const int4_t*)(kb + (i & 1) * 16 * RB + (klane ^ (64 * (i >> 1))));
+  // Scores of tile kt (its copies have landed): step i is sub-tile i % 2, 16-byte piece i / 2.
+  auto scores = [&](const char* kb, float4_t (&sc)[QS][2]) {
+    const int kl = pa_opaque(klane);
+    const char* const ka[2] = {kb + kl, kb + (kl ^ (CPR > 4 ? 64 : 0))};
+    auto kfrag = [&](int i) {
+      const int n = i >> 1;
+      return *(const int4_t*)(ka[n & 1] + (i & 1) * 16 * RB + 64 * (n & ~1));
     };
-    float4_t sc[QS][2];
 #pragma unroll
     for (int u = 0; u < QS; ++u)
 #pragma unroll
@@ -757,59 +801,99 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // Three loops, so that no accumulator is merged behind a branch: the tiles that every row of the
+  // wave sees whole (in pairs, one per buffer), the ones from the first masked tile on, and those
+  // only other waves need.
+  auto whole = [&](const char* kb, char* next, int kt) {
+    mx_wait_copies_and_barrier<0>();
+    const PaScales q8 = q8n;
+    advance(kt, next);
+    float4_t sc[QS][2];
+    scores(kb, sc);
+    const PaV<RB, DT> vt(kb + 32 * RB, vlane);
+    half8_t vf = pa_vfrag<RB, DT>(vt, 0);
     half8_t p[QS];
-    if (!mask) {
 #pragma unroll
-      for (int u = 0; u < QS; ++u) p[u] = pa_softmax<DT, false>(sc[u], rs, q8, 0, 3, mrun[u], lrun[u], o[u]);
-      half8_t vf = pa_vfrag<RB, DT>(vb, vlane, 0);
+    for (int u = 0; u < QS; ++u) p[u] = pa_softmax<DT, false>(sc[u], rs, q8, 0, 3, mrun[u], lrun[u], o[u]);
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const half8_t v = vf;
-        if (f + 1 < NF) vf = pa_vfrag<RB, DT>(vb, vlane, f + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < QS; ++u)
-          o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
+    for (int f = 0; f < NF; ++f) {
+      const half8_t v = vf;
+      if (f + 1 < NF) vf = pa_vfrag<RB, DT>(vt, f + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < QS; ++u)
-        p[u] = pa_softmax<DT, true>(sc[u], rs, q8, pos[u] - tk - 4 * g, on, mrun[u], lrun[u], o[u]);
-      uint32_t keep[4], odd = 0;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
-        const bool ok = (on >> s) & 1;
-        keep[d] = (ok && k <= any - tk ? 0xFFFFu : 0u) | (ok && k + 1 <= any - tk ? 0xFFFF0000u : 0u);
-      }
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const half8_t v = pa_clean<DT>(pa_vfrag<RB, DT>(vb, vlane, f), keep, odd);
-#pragma unroll
-        for (int u = 0; u < QS; ++u)
-          o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if constexpr (DT != MX_DT_I8)
-        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-          const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int u = 0; u < QS; ++u) pa_add_odd<RB, NF>(vb, p[u], pos[u] - tk, seen, o[u]);
-        }
+        o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // Page ids of tiles kt and kt + 1 (kt even) lie in one load of ids, whose bits are at hand once
+  // tile kt is on its way.
+  int kt = 0;
+  const int seen = all + 1 - k0;  // keys of the range that every row of the wave sees
+  auto both_on = [&]() { return ((ids.on >> (2 * (kt & 31))) & 15) == 15; };
+  for (; kt + 2 < ntile && kt + 2 <= nt_w && 32 * kt + 64 <= seen && both_on(); kt += 2) {
+    whole(lds0, lds1, kt);
+    whole(lds1, lds0, kt + 1);
+  }
+  int pos[QS];
+#pragma unroll
+  for (int u = 0; u < QS; ++u) {
+    int hq;
+    where(u, pos[u], hq);
+    pos[u] += t.pos0;
+  }
+  for (; kt < nt_w; ++kt) {
+    mx_wait_copies_and_barrier<0>();
+    const int on = on_next;
+    const PaScales q8 = q8n;
+    if (kt + 1 < ntile) advance(kt, kt & 1 ? lds0 : lds1);
+    const int tk = k0 + 32 * kt;
+    const char* kb = kt & 1 ? lds1 : lds0;
+    const char* vb = kb + 32 * RB;
+    float4_t sc[QS][2];
+    scores(kb, sc);
+    const PaV<RB, DT> vt(vb, vlane);
+    half8_t p[QS];
+#pragma unroll
+    for (int u = 0; u < QS; ++u)
+      p[u] = pa_softmax<DT, true>(sc[u], rs, q8, pos[u] - tk - 4 * g, on, mrun[u], lrun[u], o[u]);
+    uint32_t keep[4], odd = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
+      const bool ok = (on >> s) & 1;
+      keep[d] = (ok && k <= any - tk ? 0xFFFFu : 0u) | (ok && k + 1 <= any - tk ? 0xFFFF0000u : 0u);
+    }
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const half8_t v = pa_clean<DT>(pa_vfrag<RB, DT>(vt, f), keep, odd);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < QS; ++u)
+        o[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[u], o[u][f], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (DT != MX_DT_I8)
+      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+        const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
+#pragma unroll
+        for (int u = 0; u < QS; ++u) pa_add_odd<RB, NF>(vb, p[u], pos[u] - tk, seen, o[u]);
+      }
   }
   for (; kt < ntile; ++kt) {
     mx_wait_copies_and_barrier<0>();
-    advance(kt);
+    if (kt + 1 < ntile) advance(kt, kt & 1 ? lds0 : lds1);
   }
 #pragma unroll
   for (int u = 0; u < QS; ++u) {
     const float l = pa_rowsum(lrun[u]);
     if (w0 + 16 * u + j >= t.nrows) continue;
-    const long tr = t.first + tok[u];
+    int tok, hq;
+    where(u, tok, hq);
+    const long tr = t.first + tok;
     if (nsp > 1) {
-      const long at = ((long)z * b.rows + tr) * a.nh + hq[u];
+      const long at = ((long)z * b.rows + tr) * a.nh + hq;
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         const int d = 16 * f + 4 * g;
@@ -819,8 +903,8 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
       continue;
     }
     const float il = l == 0.f ? 0.f : 1.f / l;
-    const float* gate = a.gate ? a.gate + tr * a.ldg + (long)hq[u] * c.hd : nullptr;
-    half_t* orow = (half_t*)a.out + tr * a.ldo + (long)hq[u] * c.hd;
+    const float* gate = a.gate ? a.gate + tr * a.ldg + (long)hq * c.hd : nullptr;
+    half_t* orow = (half_t*)a.out + tr * a.ldo + (long)hq * c.hd;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const int d = 16 * f + 4 * g;
@@ -861,7 +945,7 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
   const int pos = t.pos0 + tok;
   const int rb = c.hd * 4;
-  const float rs = a.scale * kLog2e;
+  const float rs = mx_readlane(a.scale * kLog2e, 0);  // uniform: a scalar register
   float4 qf[NC];
   const float* qrow = (const float*)a.q + (long)(t.first + tok) * a.ldq + (long)hq * c.hd;
 #pragma unroll
@@ -909,8 +993,10 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
     issue_v(0);
     load_k(0);
   }
-  for (int i = 0; i < nw; ++i) {
-    if (i + 1 < nw) issue_v(i + 1);
+  // `more`: a tile follows, issued without a branch, so that the waits leave it in flight.
+  auto step = [&](int i, auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    if constexpr (MORE) issue_v(i + 1);
     float4_t x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = (float4_t){0.f, 0.f, 0.f, 0.f};
@@ -924,7 +1010,7 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
     const float4_t sc = (x[0] + x[1]) + (x[2] + x[3]);
     const int tk = k0 + 16 * (wave + 4 * i);
     const bool on = (ids.on >> i) & 1;
-    if (i + 1 < nw) load_k(i + 1);
+    if constexpr (MORE) load_k(i + 1);
     const bool mask = tk + 15 > all || !on;
     const int lim = pos - tk;
     float4_t s = sc * rs;
@@ -947,7 +1033,7 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
 #pragma unroll
     for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(s[r] - mrun);
     lrun += (p[0] + p[1]) + (p[2] + p[3]);
-    if (i + 1 < nw) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(p) : "n"(NL + NC) : "memory");
+    if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(p) : "n"(NL + NC) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" : "+v"(p) : : "memory");
     const char* tile = buf + (i & 1) * TILE;
     const int top = t.kend - 1 - tk;  // the last key any row sees
@@ -982,7 +1068,9 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
         }
       }
     }
-  }
+  };
+  for (int i = 0; i + 1 < nw; ++i) step(i, std::true_type{});
+  if (nw > 0) step(nw - 1, std::false_type{});
   lrun = pa_rowsum(lrun);
   if (g == 0) {
     sm[wave][j] = mrun;
