@@ -203,10 +203,9 @@ struct PaV {
     const int chunk = DT == MX_DT_I8 ? 0 : (j & 3) >> 1;
     return row * RB + ((chunk ^ pa_vxor<DT>(row)) & (RB / 16 - 1)) * 16 + 8 * (j & 1);
   }
-  __device__ __forceinline__ PaV(const char* tile, int lane_at) {
-    const int v = pa_opaque(lane_at);
+  __device__ __forceinline__ PaV(const char* tile, int place) {
 #pragma unroll
-    for (int e = 0; e < NB; ++e) at[e] = tile + (v ^ (e * STEP));
+    for (int e = 0; e < NB; ++e) at[e] = tile + (place ^ (e * STEP));
   }
   __device__ __forceinline__ const char* operator()(int f) const { return at[f % NB] + f / NB * NB * STEP; }
 };
@@ -476,7 +475,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     int4_t pw = __builtin_bit_cast(int4_t, p);
     asm volatile("s_waitcnt vmcnt(%1)" : "+v"(pw) : "n"(2 * NL + 2 * NK) : "memory");
     p = __builtin_bit_cast(half8_t, pw);
-    const PaV<RB, DT> vt(tile, vlane);
+    const PaV<RB, DT> vt(tile, pa_opaque(vlane));
 #pragma unroll
     for (int f = 0; f < NF; ++f)
       o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(vt, f), p, o[f], 0, 0, 0);
@@ -505,7 +504,7 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     const int lim = pos - tk;
     const half8_t p = pa_softmax<DT, true>(sc, rs, w8, lim - 4 * g, on, mrun, lrun, o);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const PaV<RB, DT> vt(tile, vlane);
+    const PaV<RB, DT> vt(tile, pa_opaque(vlane));
     const int top = t.kend - 1 - tk;  // the last key any row sees
     uint32_t keep[4], odd = 0;
 #pragma unroll
@@ -752,9 +751,12 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[u][f] = (float4_t){0.f, 0.f, 0.f, 0.f};
   }
-  // key piece n of a row lies at (klane ^ 64 (n % 2)) + 64 (n - n % 2)
-  const int klane = j * RB + ((g ^ (j & 7)) & (CPR - 1)) * 16;
-  const int vlane = PaV<RB, DT>::lane_at(lane);
+  // Key piece n of a row lies at (place ^ 64 (n % 2)) + 64 (n - n % 2).
+  auto key_place = [&]() {
+    const int l = pa_opaque(threadIdx.x), jj = l & 15, gg = (l >> 4) & 3;
+    return jj * RB + ((gg ^ (jj & 7)) & (CPR - 1)) * 16;
+  };
+  auto value_place = [&]() { return PaV<RB, DT>::lane_at(pa_opaque(threadIdx.x & 63)); };
 
   auto advance = [&](int kt, char* buf) {  // tile kt + 1 (there is one) on its way
     if (((kt + 1) & 31) == 0) {
@@ -766,7 +768,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   };
   // Scores of tile kt (its copies have landed): step i is sub-tile i % 2, 16-byte piece i / 2.
   auto scores = [&](const char* kb, float4_t (&sc)[QS][2]) {
-    const int kl = pa_opaque(klane);
+    const int kl = key_place();
     const char* const ka[2] = {kb + kl, kb + (kl ^ (CPR > 4 ? 64 : 0))};
     auto kfrag = [&](int i) {
       const int n = i >> 1;
@@ -811,7 +813,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     advance(kt, next);
     float4_t sc[QS][2];
     scores(kb, sc);
-    const PaV<RB, DT> vt(kb + 32 * RB, vlane);
+    const PaV<RB, DT> vt(kb + 32 * RB, value_place());
     half8_t vf = pa_vfrag<RB, DT>(vt, 0);
     half8_t p[QS];
 #pragma unroll
@@ -853,7 +855,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     const char* vb = kb + 32 * RB;
     float4_t sc[QS][2];
     scores(kb, sc);
-    const PaV<RB, DT> vt(vb, vlane);
+    const PaV<RB, DT> vt(vb, value_place());
     half8_t p[QS];
 #pragma unroll
     for (int u = 0; u < QS; ++u)
@@ -1133,7 +1135,10 @@ int plan(const MxKvCache* c, const MxPagedBatch* b, int nh, PaPlan* p) {
   const long seqs = b->n_seqs, rows = (long)b->rows * group;
   if (rows >= (1l << 30)) return MX_ERR_UNSUPPORTED;
   p->kind = c->dtype == MX_DT_F32 ? kF32 : max_q * group <= kKeysRows ? kKeys : kRows1;
-  if (p->kind == kRows1 && (rows / 128 + seqs) * c->n_kv_heads >= 256) p->kind = kRows2;
+  // Two query sets per wave halve the LDS reads per product; int8 heads over 128 dims would spill.
+  if (p->kind == kRows1 && !(c->dtype == MX_DT_I8 && c->head_dim > 128) &&
+      (rows / 128 + seqs) * c->n_kv_heads >= 256)
+    p->kind = kRows2;
   p->rt = p->kind == kRows1 ? 64 : p->kind == kRows2 ? 128 : kKeysRows;
   const long tiles = max_q * group <= p->rt ? seqs : rows / p->rt + seqs;
   if (tiles * c->n_kv_heads >= (1l << 24)) return MX_ERR_UNSUPPORTED;
@@ -1177,11 +1182,12 @@ int launch(const PaPlan& p, const PkCache& c, const PkBatch& b, const PaArgs& a,
       const int nb = 8 % c.nkv == 0   ? 8 * mx_ceil_div(p.ntiles, 8 / c.nkv)
                      : c.nkv % 8 == 0 ? p.ntiles * c.nkv
                                       : p.ntiles * c.nkv;
-      auto* kern = p.kind == kRows1
-                       ? (rb <= 64 ? k_pa_rows<64, DT, 1> : rb <= 128 ? k_pa_rows<128, DT, 1> : k_pa_rows<256, DT, 1>)
-                       : (rb <= 64 ? k_pa_rows<64, DT, 2> : rb <= 128 ? k_pa_rows<128, DT, 2> : k_pa_rows<256, DT, 2>);
-      if constexpr (ES == 2)
+      auto* kern = rb <= 64 ? k_pa_rows<64, DT, 1> : rb <= 128 ? k_pa_rows<128, DT, 1> : k_pa_rows<256, DT, 1>;
+      if (p.kind == kRows2) kern = rb <= 64 ? k_pa_rows<64, DT, 2> : k_pa_rows<128, DT, 2>;
+      if constexpr (ES == 2) {
+        if (p.kind == kRows2 && rb > 128) kern = k_pa_rows<256, DT, 2>;
         if (rb > 256) kern = p.kind == kRows1 ? k_pa_rows<512, DT, 1> : k_pa_rows<512, DT, 2>;
+      }
       hipLaunchKernelGGL(kern, dim3(nb, 1, p.n), dim3(256), 0, s, c, b, a, sp, p.ntiles);
     }
   }
