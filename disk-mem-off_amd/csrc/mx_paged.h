@@ -15,7 +15,7 @@ struct PkBatch {
   const int* q_start;
   const int* kv_len;
   const int* pages;
-  int n_seqs, max_pages, rows;
+  int n_seqs, max_pages, rows, max_kv;
 };
 
 static inline int pk_esz(int dt) { return dt == MX_DT_F32 ? 4 : dt == MX_DT_F16 ? 2 : 1; }
@@ -60,7 +60,8 @@ static inline PkCache pk_cache(const MxKvCache* c) {
 }
 
 static inline PkBatch pk_batch(const MxPagedBatch* b) {
-  return PkBatch{b->q_start, b->kv_len, b->pages, b->n_seqs, b->max_pages, b->rows};
+  return PkBatch{b->q_start, b->kv_len, b->pages, b->n_seqs, b->max_pages, b->rows,
+                 b->max_kv};
 }
 
 // The sequence that row t belongs to: the last b with q_start[b] <= t, or n where t is past

@@ -57,60 +57,218 @@ struct PaArgs {
   float scale;
 };
 
-// Key ranges: split z covers keys [z len, (z + 1) len).  A row tile whose keys fit one range
-// writes its result; the others leave sums (relative to their reference) for k_pa_join.
-struct PaSplit {
-  int len, n;
-  float* po;    // [n][rows][nh][hd]
-  float2* ml;   // [n][rows][nh]: reference, sum
+// A register's value the compiler knows nothing of: what is worked out from it is worked out
+// here, per tile, and holds no registers across the loop.
+__device__ __forceinline__ int pa_opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+__device__ __forceinline__ int pa_opaque_s(int v) {  // a uniform one
+  asm volatile("" : "+s"(v));
+  return v;
+}
+// The lane's number, from the execution mask: it holds no register where it is not needed.
+__device__ __forceinline__ int pa_lane() {
+  return pa_opaque(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)));
+}
+
+// Work items.  A call's rows are cut into row tiles (RT rows of one sequence and key/value head) and
+// a tile's keys into ranges of `len` keys; an item is one range of one tile.  Every block works
+// the same schedule out of the batch's lengths: len such that about `target` items of equal
+// size come out (sum over the tiles of their keys / target, within [least, most]), the items in
+// order of sequence, range, tile (last tile first).  The blocks of a head take its items in turn.
+// An item whose tile fits one range writes its rows; the others leave sums, relative to their
+// reference, in the slot of their number for k_pa_join.
+struct PaSched {
+  int target, least, most;
+  int slots;     // at most so many items of a head
+  float* po;     // [nkv][slots][RT][hd]
+  float2* ml;    // [nkv][slots][RT]: reference, sum
+  int4_t* rows;  // [rows][nh]: where a row's first partial sum lies in them, the step to the next, how many
 };
 
-// What a row tile is.
+// A sequence's part, one sequence per lane.
+struct PaSeq {
+  int q0, m, len;   // first row, rows, cached tokens
+  int tiles, keys;  // row tiles; keys its last row sees
+  int items;
+};
+
+struct PaWork {
+  int len, items;   // keys per range, items of a head
+  PaSeq own;        // up to 64 sequences: the lane's, and the items before its end
+  int incl;
+};
+
+// What an item is.
 struct PaTile {
   int seq, row0, nrows;  // first row; rows of the sequence and head
   int first;             // q_start of the sequence
   int pos0;              // position of the sequence's row 0
-  int kend;              // keys its last row sees
+  int kend;              // keys the tile's last row sees
+  int k0;                // first key of the range
+  int ranges;            // ranges of the tile
+  int tiles;             // tiles of the sequence
 };
 
-// Tile `idx` of the batch's row tiles of RT rows (every sequence has ceil(rows G / RT), in order);
-// false past the last.  64 lanes sum the sequences' tiles, then look inside one lane's
-// share: one round for 64 sequences, two for 4096.  Wave-uniform; callers converged.
 template <int RT>
-__device__ __forceinline__ bool pa_find_tile(const PkBatch& b, const PkCache& c, int group, int idx,
-                                             int kmax, PaTile* t) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = b.n_seqs, before = 0;
-  while (true) {
-    const int per = (hi - lo + 63) >> 6;
-    const int s0 = lo + lane * per, s1 = min(hi, s0 + per);
-    int sum = 0;
-    for (int s = s0; s < s1; ++s)
-      sum += (int)(((long)(b.q_start[s + 1] - b.q_start[s]) * group + RT - 1) / RT);
-    int incl = sum;
+__device__ __forceinline__ PaSeq pa_seq(const PkBatch& b, const PkCache& c, int group, int s) {
+  PaSeq q;
+  const bool in = s < b.n_seqs;
+  const int at = in ? s : 0;
+  q.q0 = b.q_start[at];
+  q.m = in ? min(b.q_start[at + 1], b.rows) - q.q0 : 0;
+  q.len = b.kv_len[at];
+  q.tiles = q.m > 0 ? (int)(((long)q.m * group + RT - 1) / RT) : 0;
+  q.keys = (int)max(0l, min((long)min(q.len, b.max_kv), (long)b.max_pages << c.ps_log));
+  return q;
+}
+
+__device__ __forceinline__ int pa_scan(int v) {  // inclusive, over the wave
+  const int lane = pa_lane();
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const int up = __shfl_up(incl, o);
-      if (lane >= o) incl += up;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > idx);
-    if (!past) return false;
-    const int l = __builtin_ctzll(past);
-    before += __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(sum, l);
-    lo = lo + l * per;
-    if (per == 1) break;
-    hi = min(hi, lo + per);
+  for (int o = 1; o < 64; o *= 2) {
+    const int up = __shfl_up(v, o);
+    if (lane >= o) v += up;
   }
-  t->seq = lo;
-  t->first = __builtin_amdgcn_readfirstlane(b.q_start[lo]);
-  const int m = __builtin_amdgcn_readfirstlane(b.q_start[lo + 1]) - t->first;
-  const int len = __builtin_amdgcn_readfirstlane(b.kv_len[lo]);
-  t->row0 = (idx - before) * RT;
+  return v;
+}
+
+__device__ __forceinline__ int pa_items(const PaSeq& q, int len) {
+  return q.tiles * max(1, pa_ceil(q.keys, len));
+}
+
+// The schedule (wave-uniform but for `own`; callers converged).
+template <int RT>
+__device__ __forceinline__ PaWork pa_schedule(const PkBatch& b, const PkCache& c, const PaSched& sp, int group) {
+  const int lane = pa_lane();
+  PaWork w;
+  w.own = pa_seq<RT>(b, c, group, lane);
+  float total = (float)w.own.tiles * (float)w.own.keys, tiles = (float)w.own.tiles;
+  for (int s = 64 + lane; s - lane < b.n_seqs; s += 64) {
+    const PaSeq q = pa_seq<RT>(b, c, group, s);
+    total += (float)q.tiles * (float)q.keys;
+    tiles += (float)q.tiles;
+  }
+  total = mx_wave_sum(total) * (float)c.nkv;
+  tiles = mx_wave_sum(tiles);
+  // Every tile rounds its last range up: half an item each is set aside for that.
+  const float room = max((float)sp.target - 0.5f * tiles * (float)c.nkv, 0.5f * (float)sp.target);
+  const float each = min(total / room, 1.0e9f);
+  w.len = max(sp.least, min(sp.most, ((int)each + 128) & ~127));
+  w.own.items = pa_items(w.own, w.len);
+  w.incl = pa_scan(w.own.items);
+  w.items = __builtin_amdgcn_readlane(w.incl, 63);
+  for (int s = 64 + lane; s - lane < b.n_seqs; s += 64)
+    w.items += __builtin_amdgcn_readlane(pa_scan(pa_items(pa_seq<RT>(b, c, group, s), w.len)), 63);
+  return w;
+}
+
+// The sequence that `pick` (a lane's cumulative measure past a sequence > it) points at, and
+// the items before it: 64 sequences at a time.
+template <int RT>
+__device__ __forceinline__ PaSeq pa_locate(const PkBatch& b, const PkCache& c, int group, const PaWork& w, int item,
+                                           int* seq, int* before) {
+  PaSeq q = w.own;
+  int incl = w.incl, base = 0, s0 = 0;
+  uint64_t past;
+  while (!(past = __builtin_amdgcn_ballot_w64(incl > item)) && s0 + 64 < b.n_seqs) {
+    s0 += 64;
+    base = __builtin_amdgcn_readlane(incl, 63);
+    q = pa_seq<RT>(b, c, group, s0 + pa_lane());
+    q.items = pa_items(q, w.len);
+    incl = base + pa_scan(q.items);
+  }
+  const int l = past ? __builtin_ctzll(past) : 63;
+  *seq = s0 + l;
+  *before = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(q.items, l);
+  PaSeq r;
+  r.q0 = __builtin_amdgcn_readlane(q.q0, l);
+  r.m = __builtin_amdgcn_readlane(q.m, l);
+  r.len = __builtin_amdgcn_readlane(q.len, l);
+  r.tiles = __builtin_amdgcn_readlane(q.tiles, l);
+  r.keys = __builtin_amdgcn_readlane(q.keys, l);
+  return r;
+}
+
+// Keys that the last row of a tile sees.
+template <int RT>
+__device__ __forceinline__ int pa_kend(const PaSeq& q, int row0, int group) {
+  const int last = min(row0 + RT, q.m * group) - 1;
+  return max(0, min(q.len - q.m + last / group + 1, q.keys));
+}
+
+// Item `item` < w.items of a head; false where nothing is to be done (a range behind the last key
+// that its tile sees).
+template <int RT>
+__device__ __forceinline__ bool pa_item(const PkBatch& b, const PkCache& c, int group, const PaWork& w, int item,
+                                        PaTile* t) {
+  int before;
+  const PaSeq q = pa_locate<RT>(b, c, group, w, item, &t->seq, &before);
+  const int z = (item - before) / q.tiles, tile = q.tiles - 1 - (item - before - z * q.tiles);
+  t->first = q.q0;
+  t->row0 = tile * RT;
+  t->nrows = q.m * group;
+  t->pos0 = q.len - q.m;
+  t->kend = pa_kend<RT>(q, t->row0, group);
+  t->k0 = z * w.len;
+  t->ranges = max(1, pa_ceil(t->kend, w.len));
+  t->tiles = q.tiles;
+  return z < t->ranges;
+}
+
+// The page ids of 64 sub-tiles, one per lane (the one that holds key `key`), and which of them
+// are pages.
+struct PaIds {
+  int id;
+  uint64_t on;
+};
+__device__ __forceinline__ PaIds pa_ids(const PkBatch& b, const PkCache& c, int seq, int key) {
+  PaIds r;
+  const int pi = key >> c.ps_log;
+  r.id = pi < b.max_pages ? b.pages[(long)seq * b.max_pages + pi] : -1;
+  const bool ok = r.id >= 0 && r.id < c.n_pages;
+  if (!ok) r.id = 0;
+  r.on = __builtin_amdgcn_ballot_w64(ok);
+  return r;
+}
+
+// The item of a block of a direct schedule's grid (sequence, head, range), with the page ids of its
+// range (lane: key k0 + `key`): few enough that all may be there; everything is loaded at once.
+__device__ __forceinline__ bool pa_direct(const PkBatch& b, const PkCache& c, int group, int len, int key, PaTile* t,
+                                          PaIds* ids) {
+  const int z = blockIdx.z, s = blockIdx.x;
+  const int q0 = b.q_start[s], q1 = min(b.q_start[s + 1], b.rows), have = b.kv_len[s];
+  *ids = pa_ids(b, c, s, z * len + key);
+  t->seq = s;
+  t->first = __builtin_amdgcn_readfirstlane(q0);
+  const int m = __builtin_amdgcn_readfirstlane(q1) - t->first, n = __builtin_amdgcn_readfirstlane(have);
+  t->row0 = 0;
   t->nrows = m * group;
-  t->pos0 = len - m;
-  const int last = min(t->row0 + RT, t->nrows) - 1;
-  t->kend = max(0, min(t->pos0 + last / group + 1, kmax));
-  return true;
+  t->pos0 = n - m;
+  t->kend = (int)max(0l, min((long)min(n, b.max_kv), (long)b.max_pages << c.ps_log));
+  t->k0 = z * len;
+  t->ranges = max(1, pa_ceil(t->kend, len));
+  return m > 0 && z < t->ranges;
+}
+
+// The head of a block and its place among the head's blocks (`per` of them).  A head's blocks sit
+// on as few of the 8 XCDs as there are to go round, so that its keys pass through their caches.
+__device__ __forceinline__ void pa_head_of(int nkv, int* kvh, int* place) {
+  const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  if (8 % nkv == 0) {
+    const int per = 8 / nkv;
+    *kvh = x / per;
+    *place = i * per + x % per;
+  } else if (nkv % 8 == 0) {
+    const int per = nkv / 8;
+    *kvh = x * per + i % per;
+    *place = i / per;
+  } else {
+    *kvh = blockIdx.x % nkv;
+    *place = blockIdx.x / nkv;
+  }
 }
 
 __device__ __forceinline__ pa_rsrc_t pa_rsrc(const void* base, int bytes) {
@@ -154,6 +312,21 @@ __device__ __forceinline__ half8_t pa_i8x8(int2_t v) {
   return (half8_t){h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
+// 16 int8 -> 16 fp16 of 1152 + q, exact: byte q + 128 under exponent 0x64 reads as 1024 + (q + 128).
+__device__ __forceinline__ void pa_i8_biased(int4_t v, half8_t& lo, half8_t& hi) {
+  int4_t a, b;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t u = (uint32_t)v[d] ^ 0x80808080u;
+    const int p0 = (int)__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const int p1 = (int)__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    (d < 2 ? a : b)[2 * (d & 1)] = p0;
+    (d < 2 ? a : b)[2 * (d & 1) + 1] = p1;
+  }
+  lo = __builtin_bit_cast(half8_t, a);
+  hi = __builtin_bit_cast(half8_t, b);
+}
+
 // ------------------------------------------------------------------------------------
 // LDS tiles of 32 rows of RB bytes (RB = 64 .. 512, the padded row), row-major, a row's 16-byte
 // chunks permuted by an XOR so that the fragment reads use every bank once: 8 lanes of a
@@ -178,13 +351,6 @@ __device__ __forceinline__ uint32_t pa_copy_off(int i, int lane, int rb, X x) {
   const int row = i * RPI + lane / CPR;
   const int chunk = ((lane % CPR) ^ x(row)) & (CPR - 1);
   return (uint32_t)(row * rb + min(chunk * 16, rb - 16));
-}
-
-// A register's value the compiler knows nothing of: what is worked out from it is worked out
-// here, per tile, and holds no registers across the loop.
-__device__ __forceinline__ int pa_opaque(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
 }
 
 // One lane's reads of a tile's value fragments (16 dims x 32 keys each): the XOR touches the low
@@ -226,15 +392,27 @@ __device__ __forceinline__ half8_t pa_vfrag(const PaV<RB, DT>& vl, int f) {
   }
 }
 
-// A fragment of a masked tile: keys no row of the wave sees become zeros (keep: 16-bit masks
-// of the lane's 8 keys), and with fp16 values non-finite ones do too, noted in `odd`.
-template <int DT>
+// 16-bit masks of the lane's 8 keys of a tile whose last seen key is `top` (relative) and whose
+// sub-tiles on a page are `on`.
+__device__ __forceinline__ void pa_keep(int top, int on, uint32_t (&keep)[4]) {
+  const int g = pa_lane() >> 4;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
+    const bool ok = (on >> s) & 1;
+    keep[d] = (ok && k <= top ? 0xFFFFu : 0u) | (ok && k + 1 <= top ? 0xFFFF0000u : 0u);
+  }
+}
+
+// A fragment of a masked fp16 tile: keys no row of the wave sees become zeros, and with ODD non-
+// finite values do too, noted in `odd`.  (Int8 values are finite: a weight of zero suffices.)
+template <bool ODD>
 __device__ __forceinline__ half8_t pa_clean(half8_t v, const uint32_t (&keep)[4], uint32_t& odd) {
   int4_t u = __builtin_bit_cast(int4_t, v);
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
     uint32_t w = (uint32_t)u[d] & keep[d];
-    if constexpr (DT != MX_DT_I8) {
+    if constexpr (ODD) {
       const uint32_t lo = (w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
       const uint32_t hi = (w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
       odd |= lo | hi;
@@ -255,7 +433,7 @@ __device__ __forceinline__ void pa_add_odd(const char* tile, half8_t p, int lim,
 #pragma nounroll
   for (int key = 0; key < 32; ++key) {
     if (!((seen >> key) & 1)) continue;
-    const int lane = pa_opaque(threadIdx.x & 63), j = lane & 15, g = lane >> 4;
+    const int lane = pa_lane(), j = lane & 15, g = lane >> 4;
     const int src = ((key & 15) >> 2) * 16 + j, d = (key >> 4) * 2 + ((key >> 1) & 1);
     const int pw = __shfl(d == 0 ? pi[0] : d == 1 ? pi[1] : d == 2 ? pi[2] : pi[3], src);
     const half2_t ph = __builtin_bit_cast(half2_t, pw);
@@ -331,51 +509,51 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
   return p;
 }
 
-// The page ids of 64 sub-tiles, one per lane, and which of them are pages.
-struct PaIds {
-  int id;
-  uint64_t on;
-};
-__device__ __forceinline__ PaIds pa_ids(const PkBatch& b, const PkCache& c, int seq, int key, int stop) {
-  PaIds r;
-  const int pi = key >> c.ps_log;
-  r.id = key < stop && pi < b.max_pages ? b.pages[(long)seq * b.max_pages + pi] : -1;
-  const bool ok = r.id >= 0 && r.id < c.n_pages;
-  if (!ok) r.id = 0;
-  r.on = __builtin_amdgcn_ballot_w64(ok);
-  return r;
-}
-
 // ------------------------------------------------------------------------------------
 // k_pa_keys: a tile of 16 rows, its keys dealt to the block's 4 waves 32 at a time.  For decode
-// steps, bound by the bytes of the pages.  A wave's tiles are its own: keys straight into MFMA
-// registers (16 rows x 64 bytes per load), values by copies into two LDS buffers of the wave, the
-// next tile's of both in flight while one computes, no barrier until the waves' sums are put
-// together at the end.
+// steps, bound by the bytes of the pages.  A wave's tiles are its own: one LDS buffer for keys,
+// one for values, filled by copies of whole rows (key rows read straight into MFMA registers
+// would be 16 rows x 16 bytes per quarter wave, a cache line each); the next tile's keys are on
+// their way from the moment this tile's scores are formed, its values from the moment this
+// tile's are used.  No barrier until the waves' sums are put together at the end.
 // ------------------------------------------------------------------------------------
 constexpr int kKeysRows = 16;
 constexpr int kKeysMax = 4096;  // keys of a split: 64 sub-tile page ids per wave
 
-template <int RB, int DT>
-__global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+template <int RB, int DT, bool DIRECT>
+__global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
   constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
-  constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16;
+  constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16, CPR = RB / 16;
   constexpr int NL = RB / 64;             // 1 KiB pieces per 16 rows
   constexpr int TILE = 32 * RB;
-  __shared__ __align__(1024) char lds0[4 * TILE];  // one variable per buffer (see k_pa_rows)
-  __shared__ __align__(1024) char lds1[4 * TILE];
+  __shared__ __align__(1024) char ldsk[4 * TILE];  // one variable per buffer (see k_pa_rows)
+  __shared__ __align__(1024) char ldsv[4 * TILE];
   __shared__ float sm[4][16], sl[4][16];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, z = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kvh = blockIdx.y, first = 0;
+  PaWork work;
+  if constexpr (DIRECT) {  // one item per block, slot by range and sequence
+    first = blockIdx.z * b.n_seqs + blockIdx.x;
+    work.len = sp.least;
+  } else {
+    pa_head_of(c.nkv, &kvh, &first);
+    work = pa_schedule<kKeysRows>(b, c, sp, a.group);
+    work.items = min(work.items, sp.slots);
+  }
+  for (int item = first; DIRECT || item < work.items; item += per) {
+  // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
+  const int lane = pa_lane(), tid = 64 * wave + lane, j = lane & 15, g = lane >> 4;
   PaTile t;
-  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
-  if (!pa_find_tile<kKeysRows>(b, c, a.group, blockIdx.x, kmax, &t)) return;
-  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
-  if (k0 >= k1 && z > 0) return;
-  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+  PaIds ids;  // lane l: the page of sub-tile l % 2 of the wave's tile l / 2
+  const int mine = 32 * (wave + 4 * (lane >> 1)) + 16 * (lane & 1);
+  if constexpr (DIRECT) {
+    if (!pa_direct(b, c, a.group, work.len, mine, &t, &ids)) return;
+  } else {
+    if (!pa_item<kKeysRows>(b, c, a.group, work, item, &t)) continue;
+    ids = pa_ids(b, c, t.seq, t.k0 + mine);
+  }
+  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
 
   const int row = min(t.row0 + j, t.nrows - 1);
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
@@ -390,139 +568,146 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   auto qdim = [&](int cc) { return DT == MX_DT_I8 ? 64 * (cc >> 1) + 16 * g + 8 * (cc & 1) : 32 * cc + 8 * g; };
 #pragma unroll
   for (int cc = 0; cc < NC; ++cc) qf[cc] = *(const half8_t*)(qrow + min(qdim(cc), c.hd - 8));
-#pragma unroll
-  for (int cc = 0; cc < NC; ++cc)
-    if (qdim(cc) >= c.hd) qf[cc] = (half8_t)(half_t)0.f;
-
   const int ntile = pa_ceil(max(0, k1 - k0), 32);
   const int nw = ntile > wave ? (ntile - 1 - wave) / 4 + 1 : 0;
-  // lane l: the page of sub-tile l % 2 of the wave's tile l / 2
-  const PaIds ids = pa_ids(b, c, t.seq, k0 + 32 * (wave + 4 * (lane >> 1)) + 16 * (lane & 1), k1);
-  char* const buf0 = lds0 + wave * TILE;
-  char* const buf1 = lds1 + wave * TILE;
-  uint32_t voff[NL][2];
+  char* const kbuf = ldsk + wave * TILE;
+  char* const vbuf = ldsv + wave * TILE;
+  uint32_t koff[NL], voff[NL][2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int i = 0; i < NL; ++i) {
+    koff[i] = pa_copy_off<RB>(i, lane, rb, [](int r) { return r & 7; });
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
+    for (int s = 0; s < 2; ++s)
       voff[i][s] = pa_copy_off<RB>(i, lane, rb, [&](int r) { return pa_vxor<DT>(16 * s + r); });
+  }
   auto row_of = [&](int i, int s) {  // the sub-tile's first row in a pool
     const int id = __builtin_amdgcn_readlane(ids.id, 2 * i + s);
     const int key = k0 + 32 * (wave + 4 * i) + 16 * s;
     return (((long)id * c.nkv + kvh) << c.ps_log) + (key & (c.ps - 1));
   };
-  auto issue_v = [&](int i, char* buf) {
+  PaScales q8n;
+  auto issue_k = [&](int i) {
+    const long at0 = row_of(i, 0), at1 = row_of(i, 1);
+    if constexpr (DT == MX_DT_I8) {  // ahead of the copies: the waits below count those alone
+      q8n.ks[0] = *(const float4*)(c.ks + at0 + 4 * g);
+      q8n.ks[1] = *(const float4*)(c.ks + at1 + 4 * g);
+      q8n.vs[0] = *(const float4*)(c.vs + at0 + 4 * g);
+      q8n.vs[1] = *(const float4*)(c.vs + at1 + 4 * g);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const pa_rsrc_t r = pa_rsrc(c.k + (s ? at1 : at0) * rb, 16 * rb);
+#pragma unroll
+      for (int n = 0; n < NL; ++n) mx_copy_to_lds16(r, kbuf + s * 16 * RB + n * 1024, koff[n]);
+    }
+  };
+  auto issue_v = [&](int i) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const pa_rsrc_t r = pa_rsrc(c.v + row_of(i, s) * rb, 16 * rb);
 #pragma unroll
-      for (int n = 0; n < NL; ++n) mx_copy_to_lds16(r, buf + s * 16 * RB + n * 1024, voff[n][s]);
+      for (int n = 0; n < NL; ++n) mx_copy_to_lds16(r, vbuf + s * 16 * RB + n * 1024, voff[n][s]);
     }
   };
-  constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte loads per key row and lane
-  int4_t kr[2][NK];
-  PaScales q8;
-  auto load_k = [&](int i) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const long at = row_of(i, s);
-      const char* p = c.k + at * rb;
-#pragma unroll
-      for (int n = 0; n < NK; ++n) kr[s][n] = *(const int4_t*)(p + (uint32_t)(j * rb + min(64 * n + 16 * g, rb - 16)));
-      if constexpr (DT == MX_DT_I8) {
-        q8.ks[s] = *(const float4*)(c.ks + at + 4 * g);
-        q8.vs[s] = *(const float4*)(c.vs + at + 4 * g);
-      }
-    }
-  };
+  constexpr int NK = DT == MX_DT_I8 ? NC / 2 : NC;  // 16-byte fragment reads per key row and lane
   const int vlane = PaV<RB, DT>::lane_at(lane);
+  const int klane = j * RB + ((g ^ (j & 7)) & (CPR - 1)) * 16;
   float4_t o[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) o[f] = (float4_t){0.f, 0.f, 0.f, 0.f};
   float mrun = kLow, lrun = 0.f;
 
-  // The last key that every row of the tile sees (rows past the last repeat it).
-  const int all = t.pos0 + t.row0 / a.group;
-  auto scores = [&](float4_t (&sc)[2]) {
+  if (nw > 0) {
+    issue_k(0);
+    issue_v(0);
+  }
+  __builtin_amdgcn_sched_barrier(0);  // the queries, loaded ahead of the copies, are not waited for before
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc)
+    if (qdim(cc) >= c.hd) qf[cc] = (half8_t)(half_t)0.f;
+  // Int8 keys meet the queries as 1152 + q (pa_i8_biased): 1152 times the sum of the row's queries
+  // comes off the score.
+  float bias = 0.f;
+  if constexpr (DT == MX_DT_I8) {
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bias += (float)qf[cc][e];
+    bias = -1152.f * pa_rowsum(bias);
+  }
+  // The last key that every row of the tile sees (rows past the last repeat it), and that any does.
+  const int all = t.pos0 + t.row0 / a.group, any = t.kend - 1;
+  // MORE: a tile follows.  Its copies are issued without a branch, so that the compiler's own waits
+  // leave them in flight too.
+  auto step = [&](int i, auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    // Keys of this tile: all but the value copies behind them.
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+    const PaScales q8 = q8n;
+    float4_t sc[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      float4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const char* p0 = kbuf + klane + s * 16 * RB;
+      const char* p1 = kbuf + (klane ^ (CPR > 4 ? 64 : 0)) + s * 16 * RB;
+      float4_t x[2] = {{bias, bias, bias, bias}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
+        const int4_t kf = *(const int4_t*)((n & 1 ? p1 : p0) + 64 * (n & ~1));
         if constexpr (DT == MX_DT_I8) {
           half8_t lo, hi;
-          mx_i8_to_f16(kr[s][n], lo, hi);
+          pa_i8_biased(kf, lo, hi);
           x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qf[2 * n], x[0], 0, 0, 0);
           x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qf[2 * n + 1], x[1], 0, 0, 0);
         } else {
-          x[n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kr[s][n]), qf[n],
-                                                            x[n & 1], 0, 0, 0);
+          x[n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kf), qf[n], x[n & 1], 0, 0, 0);
         }
       }
       sc[s] = x[0] + x[1];
     }
-  };
-  // A tile with a tile behind it that every row sees whole.  The next tile's copies and loads are
-  // issued without a branch, so the waits for this tile's leave them in flight.
-  auto whole = [&](const char* tile, char* next, int i) {
-    issue_v(i + 1, next);
-    float4_t sc[2];
-    scores(sc);
-    const PaScales w8 = q8;
-    load_k(i + 1);
-    half8_t p = pa_softmax<DT, false>(sc, rs, w8, 0, 3, mrun, lrun, o);
-    // This tile's values have landed (they were issued before its keys).
-    int4_t pw = __builtin_bit_cast(int4_t, p);
-    asm volatile("s_waitcnt vmcnt(%1)" : "+v"(pw) : "n"(2 * NL + 2 * NK) : "memory");
-    p = __builtin_bit_cast(half8_t, pw);
-    const PaV<RB, DT> vt(tile, pa_opaque(vlane));
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-      o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(vt, f), p, o[f], 0, 0, 0);
-  };
-  if (nw > 0) {
-    issue_v(0, buf0);
-    load_k(0);
-  }
-  int i = 0;
-  auto plain = [&]() {  // tiles i and i + 1
-    return k0 + 32 * (wave + 4 * i + 4) + 31 <= all && ((ids.on >> (2 * i)) & 15) == 15;
-  };
-  for (; i + 2 < nw && plain(); i += 2) {
-    whole(buf0, buf1, i);
-    whole(buf1, buf0, i + 1);
-  }
-  for (; i < nw; ++i) {
-    char* const tile = i & 1 ? buf1 : buf0;
-    if (i + 1 < nw) issue_v(i + 1, i & 1 ? buf0 : buf1);
-    float4_t sc[2];
-    scores(sc);
-    const PaScales w8 = q8;
+    // The scores are formed (their registers pass through here): the buffer is free.
+    asm volatile("" : "+v"(sc[0]), "+v"(sc[1])::"memory");
+    if constexpr (MORE) issue_k(i + 1);
     const int tk = k0 + 32 * (wave + 4 * i);  // first key of the tile
     const int on = (int)(ids.on >> (2 * i)) & 3;
-    if (i + 1 < nw) load_k(i + 1);
+    const bool mask = tk + 31 > all || on != 3;
     const int lim = pos - tk;
-    const half8_t p = pa_softmax<DT, true>(sc, rs, w8, lim - 4 * g, on, mrun, lrun, o);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const PaV<RB, DT> vt(tile, pa_opaque(vlane));
-    const int top = t.kend - 1 - tk;  // the last key any row sees
-    uint32_t keep[4], odd = 0;
+    half8_t p;
+    if (mask) p = pa_softmax<DT, true>(sc, rs, q8, lim - 4 * g, on, mrun, lrun, o);
+    else p = pa_softmax<DT, false>(sc, rs, q8, lim, on, mrun, lrun, o);
+    // Values of this tile: all but the key copies behind them.
+    if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const PaV<RB, DT> vt(vbuf, pa_opaque(vlane));
+    if (DT == MX_DT_I8 || !mask) {  // (a weight of zero meets finite int8 values)
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
-      const bool ok = (on >> s) & 1;
-      keep[d] = (ok && k <= top ? 0xFFFFu : 0u) | (ok && k + 1 <= top ? 0xFFFF0000u : 0u);
-    }
+      for (int f = 0; f < NF; ++f)
+        o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_vfrag<RB, DT>(vt, f), p, o[f], 0, 0, 0);
+    } else {
+      uint32_t keep[4], odd = 0;
+      pa_keep(any - tk, on, keep);
+      if (all >= any) {  // one token: what one row does not see, none does
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
-      o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<DT>(pa_vfrag<RB, DT>(vt, f), keep, odd), p, o[f],
-                                                    0, 0, 0);
-    if constexpr (DT != MX_DT_I8)
-      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-        const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
-        pa_add_odd<RB, NF>(tile, p, lim, seen, o);
+        for (int f = 0; f < NF; ++f)
+          o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<false>(pa_vfrag<RB, DT>(vt, f), keep, odd), p,
+                                                        o[f], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pa_clean<true>(pa_vfrag<RB, DT>(vt, f), keep, odd), p,
+                                                        o[f], 0, 0, 0);
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+          const uint32_t seen = ((on & 1) ? 0xFFFFu : 0u) | ((on & 2) ? 0xFFFF0000u : 0u);
+          pa_add_odd<RB, NF>(vbuf, p, lim, seen, o);
+        }
       }
-  }
+    }
+    // Every value is read (the products hold them): the buffer is free.
+    asm volatile("" : "+v"(o[NF - 1])::"memory");
+    if constexpr (MORE) issue_v(i + 1);
+  };
+#pragma nounroll
+  for (int i = 0; i + 1 < nw; ++i) step(i, std::true_type{});
+  if (nw > 0) step(nw - 1, std::false_type{});
   lrun = pa_rowsum(lrun);
 
   // The waves' sums, relative to the largest reference of each row.
@@ -532,15 +717,15 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
   }
   __syncthreads();
   const float m = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j]));
-  const float mine = __builtin_amdgcn_exp2f(mrun - m);
+  const float weight = __builtin_amdgcn_exp2f(mrun - m);
   // [16 rows][DP] per wave: waves 0, 1 in the first buffer, 2, 3 in the second
   static_assert(2 * 16 * DP * 4 <= 4 * TILE, "the sums fit the buffers");
-  auto part_of = [&](int w) { return (float*)(w < 2 ? lds0 : lds1) + (w & 1) * 16 * DP; };
+  auto part_of = [&](int w) { return (float*)(w < 2 ? ldsk : ldsv) + (w & 1) * 16 * DP; };
   __syncthreads();
   float* const part = part_of(wave);
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
-    const float4_t v = o[f] * mine;
+    const float4_t v = o[f] * weight;
     *(float4_t*)(part + j * DP + 16 * f + 4 * g) = v;
   }
   __syncthreads();
@@ -557,9 +742,11 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     }
     const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
     const long tr = t.first + rt;
-    if (nsp > 1) {
-      const long at = ((long)z * b.rows + tr) * a.nh + h;
-      *(float4_t*)(sp.po + at * c.hd + d) = s;
+    const int at = (kvh * sp.slots + item) * kKeysRows + r;
+    if (k0 == 0 && d == 0)
+      sp.rows[tr * a.nh + h] = (int4_t){at, (DIRECT ? b.n_seqs : t.tiles) * kKeysRows, t.ranges, 0};
+    if (t.ranges > 1) {
+      *(float4_t*)(sp.po + (long)at * c.hd + d) = s;
       if (d == 0) sp.ml[at] = make_float2(mr, l);
       continue;
     }
@@ -572,37 +759,81 @@ __global__ __launch_bounds__(256) void k_pa_keys(PkCache c, PkBatch b, PaArgs a,
     *(half4_t*)((half_t*)a.out + tr * a.ldo + (long)h * c.hd + d) =
         (half4_t){(half_t)s[0], (half_t)s[1], (half_t)s[2], (half_t)s[3]};
   }
+  if constexpr (DIRECT) return;
+  __syncthreads();  // the buffers are free
+  }
 }
 
 // ------------------------------------------------------------------------------------
-// k_pa_join: the partial sums of a row's key ranges, one wave per (row, head).
+// k_pa_join: the partial sums of a row's key ranges; the first range's item has noted where they
+// lie.  One wave per (row, head), or WIDE, a block's four waves, a quarter of the ranges each: a
+// decode step has few rows of many ranges, whose sums were written by other XCDs and take a
+// microsecond or two to fetch (40 rows of up to 35 ranges: 11.4 us with one wave, 5.0 with four).
 // ------------------------------------------------------------------------------------
-template <int RT, typename OT>
-__global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+template <typename OT, bool WIDE>
+__global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a, PaSched sp) {
+  __shared__ float sml[4][2];
+  __shared__ __align__(16) float so[WIDE ? 4 : 1][256];
   const int lane = threadIdx.x & 63;
-  const int item = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int t = item / a.nh, h = item - t * a.nh;
-  if (t >= b.rows) return;
-  const int seq = __builtin_amdgcn_readfirstlane(pk_seq_of(b.q_start, b.n_seqs, t));
-  if (seq >= b.n_seqs) return;
-  const int q0 = b.q_start[seq], m = b.q_start[seq + 1] - q0, len = b.kv_len[seq];
-  const int r = (t - q0) * a.group + h % a.group, nrows = m * a.group;
-  const int last = min(r / RT * RT + RT, nrows) - 1;
-  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
-  const int kend = max(0, min(len - m + last / a.group + 1, kmax));
-  const int n = pa_ceil(kend, sp.len);
-  if (n <= 1) return;
-  const long step = (long)b.rows * a.nh, at = (long)t * a.nh + h;
-  float mr = kLow;
-  for (int z = 0; z < n; ++z) mr = fmaxf(mr, sp.ml[at + z * step].x);
-  float l = 0.f;
-  float4_t s = {0.f, 0.f, 0.f, 0.f};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = WIDE ? blockIdx.y : blockIdx.y * 4 + wave;
+  const int t = blockIdx.x;
+  if (h >= a.nh) return;
+  const int4_t where = sp.rows[(long)t * a.nh + h];
+  if (t >= b.q_start[b.n_seqs]) return;  // behind the last sequence
+  const int ranges = __builtin_amdgcn_readfirstlane(where[2]);
+  if (ranges <= 1) return;
+  // This wave's: every 4th range, or all of them.
+  constexpr int HOP = WIDE ? 4 : 1;
+  const int n = WIDE ? (ranges - wave + 3) / 4 : ranges;
+  const long at = __builtin_amdgcn_readfirstlane(where[0]) + (WIDE ? (long)wave * where[1] : 0);
+  const long step = (long)HOP * __builtin_amdgcn_readfirstlane(where[1]);
   const int d = min(4 * lane, c.hd - 4);
-  for (int z = 0; z < n; ++z) {
-    const float2 ml = sp.ml[at + z * step];
-    const float w = __builtin_amdgcn_exp2f(ml.x - mr);
-    l += w * ml.y;
-    s += w * *(const float4_t*)(sp.po + (at + z * step) * c.hd + d);
+  const float* po = sp.po + at * c.hd + d;
+  float mr = kLow, l = 0.f;
+  float4_t s = {0.f, 0.f, 0.f, 0.f};
+  // 64 ranges at a time: lane z holds range z's reference and sum, whose weights all lanes
+  // then read; 8 partial rows in flight.
+  for (int z0 = 0; z0 < n; z0 += 64) {
+    const int nz = min(64, n - z0);
+    float2 ml = make_float2(kLow, 0.f);
+    if (lane < nz) ml = sp.ml[at + (z0 + lane) * step];
+    float4_t v[8];
+    auto load = [&](int z) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (z + e < nz) v[e] = *(const float4_t*)(po + (z0 + z + e) * step * c.hd);
+    };
+    load(0);
+    const float top = fmaxf(mr, mx_wave_max(ml.x));
+    const float w = __builtin_amdgcn_exp2f(ml.x - top), old = __builtin_amdgcn_exp2f(mr - top);
+    l = l * old + mx_wave_sum(w * ml.y);
+    s *= old;
+    mr = top;
+    for (int z = 0; z < nz; z += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (z + e < nz) s += mx_readlane(w, z + e) * v[e];
+      load(z + 8);
+    }
+  }
+  if constexpr (WIDE) {
+    if (lane == 0) {
+      sml[wave][0] = mr;
+      sml[wave][1] = l;
+    }
+    *(float4_t*)(so[wave] + 4 * lane) = s;
+    __syncthreads();
+    if (wave) return;
+    const float top = fmaxf(fmaxf(sml[0][0], sml[1][0]), fmaxf(sml[2][0], sml[3][0]));
+    l = 0.f;
+    s = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sml[w][0] - top);
+      l += f * sml[w][1];
+      s += f * *(const float4_t*)(so[w] + 4 * lane);
+    }
   }
   if (4 * lane >= c.hd) return;
   s *= l == 0.f ? 0.f : 1.f / l;
@@ -611,9 +842,9 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
     s = (float4_t){s[0] * mx_sigmoid(gv.x), s[1] * mx_sigmoid(gv.y), s[2] * mx_sigmoid(gv.z),
                    s[3] * mx_sigmoid(gv.w)};
   }
-  OT* o = (OT*)a.out + (long)t * a.ldo + (long)h * c.hd + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = (OT)s[e];
+  typedef OT ot4_t __attribute__((ext_vector_type(4)));
+  *(ot4_t*)((OT*)a.out + (long)t * a.ldo + (long)h * c.hd + d) =
+      (ot4_t){(OT)s[0], (OT)s[1], (OT)s[2], (OT)s[3]};
 }
 
 // ------------------------------------------------------------------------------------
@@ -632,7 +863,7 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
 
 template <int RB, int DT, int QS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
+void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
   constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
   constexpr int DP = RB / ES, NC = DP / 32, NF = DP / 16, CPR = RB / 16;
   constexpr int NL = RB / 64;             // 1 KiB pieces per 16 rows
@@ -645,34 +876,22 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   __shared__ __align__(1024) char lds0[TILE];
   __shared__ __align__(1024) char lds1[TILE];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4;
-  int kvh, idx;
-  {
-    const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
-    if (8 % c.nkv == 0) {
-      const int per = 8 / c.nkv;
-      kvh = x / per;
-      idx = i * per + x % per;
-    } else if (c.nkv % 8 == 0) {
-      const int per = c.nkv / 8;
-      kvh = x * per + i % per;
-      idx = i / per;
-    } else {
-      kvh = blockIdx.x % c.nkv;
-      idx = blockIdx.x / c.nkv;
-    }
-    idx = ntiles - 1 - idx;
-  }
-  if (idx < 0) return;
-  const int z = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kvh, place;
+  pa_head_of(c.nkv, &kvh, &place);
+  for (int item = place;; item += per) {
+  // Worked out anew for every item: it would hold registers across the loops below.
+  PaSched now = sp;
+  now.target = pa_opaque_s(sp.target);
+  const int group = pa_opaque_s(a.group);
+  const PaWork work = pa_schedule<RT>(b, c, now, group);
+  if (item >= min(work.items, sp.slots)) return;
+  // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
+  const int lane = pa_lane(), j = lane & 15, g = lane >> 4;
   PaTile t;
-  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
-  if (!pa_find_tile<RT>(b, c, a.group, idx, kmax, &t)) return;
-  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
-  if (k0 >= k1 && z > 0) return;
-  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+  if (!pa_item<RT>(b, c, group, work, item, &t)) continue;
+  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
+  PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * lane);
   const int ntile = pa_ceil(max(0, k1 - k0), 32);
 
   const int rb = c.hd * ES;
@@ -685,8 +904,6 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   uint32_t offv[2];
   offv[0] = pa_copy_off<RB>(n0, lane, rb, [](int r) { return pa_vxor<DT>(r); });
   offv[1] = DT == MX_DT_I8 ? pa_copy_off<RB>(n0, lane, rb, [](int r) { return pa_vxor<DT>(16 + r); }) : offv[0];
-  PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * lane, k1);
-  PaIds ids2 = pa_ids(b, c, t.seq, k0 + 1024 + 16 * lane, k1);
   auto row_of = [&](int kt, int s) {  // the sub-tile's first row in a pool
     const int id = __builtin_amdgcn_readlane(ids.id, 2 * (kt & 31) + s);
     return (((long)id * c.nkv + kvh) << c.ps_log) + ((k0 + 32 * kt + 16 * s) & (c.ps - 1));
@@ -721,9 +938,10 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   // Token (of the sequence) and head of the lane's row in set u: worked out where they are needed,
   // behind a barrier to the compiler, so that they hold no registers in between.
   auto where = [&](int u, int& tok, int& hq) {
-    const int row = min(w0 + 16 * u + pa_opaque(j), t.nrows - 1);
-    tok = row / a.group;
-    hq = kvh * a.group + row - tok * a.group;
+    const int row = min(w0 + 16 * u + (pa_lane() & 15), t.nrows - 1);
+    const int group = pa_opaque_s(a.group);  // (its reciprocal, too)
+    tok = row / group;
+    hq = kvh * group + row - tok * group;
   };
 #pragma unroll
   for (int u = 0; u < QS; ++u) {
@@ -738,8 +956,8 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   }
   // The keys that every row of the wave sees end at `all`, those that any sees at `any`.
   const int lastrow = min(w0 + 16 * QS, t.nrows) - 1;
-  const int all = t.pos0 + min(w0, t.nrows - 1) / a.group;
-  const int any = min(t.pos0 + lastrow / a.group, t.kend - 1);
+  const int all = t.pos0 + min(w0, t.nrows - 1) / group;
+  const int any = min(t.pos0 + lastrow / group, t.kend - 1);
   const int nt_w = w0 < t.nrows ? min(ntile, max(0, any + 1 - k0 + 31) / 32) : 0;
 
   float4_t o[QS][NF];
@@ -753,16 +971,13 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
   }
   // Key piece n of a row lies at (place ^ 64 (n % 2)) + 64 (n - n % 2).
   auto key_place = [&]() {
-    const int l = pa_opaque(threadIdx.x), jj = l & 15, gg = (l >> 4) & 3;
+    const int l = pa_lane(), jj = l & 15, gg = l >> 4;
     return jj * RB + ((gg ^ (jj & 7)) & (CPR - 1)) * 16;
   };
-  auto value_place = [&]() { return PaV<RB, DT>::lane_at(pa_opaque(threadIdx.x & 63)); };
+  auto value_place = [&]() { return PaV<RB, DT>::lane_at(pa_lane()); };
 
   auto advance = [&](int kt, char* buf) {  // tile kt + 1 (there is one) on its way
-    if (((kt + 1) & 31) == 0) {
-      ids = ids2;
-      ids2 = pa_ids(b, c, t.seq, k0 + 32 * (kt + 33) + 16 * lane, k1);
-    }
+    if (((kt + 1) & 31) == 0) ids = pa_ids(b, c, t.seq, k0 + 32 * (kt + 1) + 16 * pa_lane());
     issue(kt + 1, buf);
     on_next = (int)(ids.on >> (2 * ((kt + 1) & 31))) & 3;
   };
@@ -859,17 +1074,13 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     half8_t p[QS];
 #pragma unroll
     for (int u = 0; u < QS; ++u)
-      p[u] = pa_softmax<DT, true>(sc[u], rs, q8, pos[u] - tk - 4 * g, on, mrun[u], lrun[u], o[u]);
+      p[u] = pa_softmax<DT, true>(sc[u], rs, q8, pos[u] - tk - 4 * (pa_lane() >> 4), on, mrun[u], lrun[u], o[u]);
     uint32_t keep[4], odd = 0;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const int s = d >> 1, k = 16 * s + 4 * g + 2 * (d & 1);
-      const bool ok = (on >> s) & 1;
-      keep[d] = (ok && k <= any - tk ? 0xFFFFu : 0u) | (ok && k + 1 <= any - tk ? 0xFFFF0000u : 0u);
-    }
+    pa_keep(any - tk, on, keep);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-      const half8_t v = pa_clean<DT>(pa_vfrag<RB, DT>(vt, f), keep, odd);
+      half8_t v = pa_vfrag<RB, DT>(vt, f);
+      if constexpr (DT != MX_DT_I8) v = pa_clean<true>(v, keep, odd);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < QS; ++u)
@@ -887,21 +1098,23 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     mx_wait_copies_and_barrier<0>();
     if (kt + 1 < ntile) advance(kt, kt & 1 ? lds0 : lds1);
   }
+  const int j1 = pa_lane() & 15, g1 = pa_lane() >> 4;
 #pragma unroll
   for (int u = 0; u < QS; ++u) {
     const float l = pa_rowsum(lrun[u]);
-    if (w0 + 16 * u + j >= t.nrows) continue;
+    if (w0 + 16 * u + j1 >= t.nrows) continue;
     int tok, hq;
     where(u, tok, hq);
     const long tr = t.first + tok;
-    if (nsp > 1) {
-      const long at = ((long)z * b.rows + tr) * a.nh + hq;
+    const int at = (kvh * sp.slots + item) * RT + (w0 - t.row0) + 16 * u + j1;
+    if (k0 == 0 && g1 == 0) sp.rows[tr * a.nh + hq] = (int4_t){at, t.tiles * RT, t.ranges, 0};
+    if (t.ranges > 1) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const int d = 16 * f + 4 * g;
-        if (d < c.hd) *(float4_t*)(sp.po + at * c.hd + d) = o[u][f];
+        const int d = 16 * f + 4 * g1;
+        if (d < c.hd) *(float4_t*)(sp.po + (long)at * c.hd + d) = o[u][f];
       }
-      if (g == 0) sp.ml[at] = make_float2(mrun[u], l);
+      if (g1 == 0) sp.ml[at] = make_float2(mrun[u], l);
       continue;
     }
     const float il = l == 0.f ? 0.f : 1.f / l;
@@ -909,7 +1122,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
     half_t* orow = (half_t*)a.out + tr * a.ldo + (long)hq * c.hd;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-      const int d = 16 * f + 4 * g;
+      const int d = 16 * f + 4 * g1;
       if (d >= c.hd) continue;
       float4_t v = o[u][f] * il;
       if (gate) {
@@ -920,6 +1133,8 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
       *(half4_t*)(orow + d) = (half4_t){(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
     }
   }
+  __syncthreads();  // the buffers are free
+  }
 }
 
 // ------------------------------------------------------------------------------------
@@ -927,22 +1142,36 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSplit sp, int ntiles) {
 // rows, keys dealt to the waves 16 at a time, keys in registers, values through the wave's LDS
 // buffers.  The MFMA k-slot of lane group g at step r is key 4 g + r on both operands.
 // ------------------------------------------------------------------------------------
-template <int DP>
-__global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, PaSplit sp) {
+template <int DP, bool DIRECT>
+__global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
   constexpr int RB = DP * 4, NC = DP / 16, NL = RB / 64, CPR = RB / 16;
   constexpr int TILE = 16 * RB;
   __shared__ __align__(1024) char lds[4 * 2 * TILE];
   __shared__ float sm[4][16], sl[4][16];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, z = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kvh = blockIdx.y, first = 0;
+  PaWork work;
+  if constexpr (DIRECT) {  // one item per block, slot by range and sequence
+    first = blockIdx.z * b.n_seqs + blockIdx.x;
+    work.len = sp.least;
+  } else {
+    pa_head_of(c.nkv, &kvh, &first);
+    work = pa_schedule<kKeysRows>(b, c, sp, a.group);
+    work.items = min(work.items, sp.slots);
+  }
+  for (int item = first; DIRECT || item < work.items; item += per) {
+  // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
+  const int lane = pa_lane(), tid = 64 * wave + lane, j = lane & 15, g = lane >> 4;
   PaTile t;
-  const int kmax = (int)min((long)sp.n * sp.len, (long)b.max_pages << c.ps_log);
-  if (!pa_find_tile<kKeysRows>(b, c, a.group, blockIdx.x, kmax, &t)) return;
-  const int k0 = z * sp.len, k1 = min(t.kend, k0 + sp.len);
-  if (k0 >= k1 && z > 0) return;
-  const int nsp = max(1, pa_ceil(t.kend, sp.len));
+  PaIds ids;  // lane l: the page of the wave's tile l
+  const int mine = 16 * (wave + 4 * lane);
+  if constexpr (DIRECT) {
+    if (!pa_direct(b, c, a.group, work.len, mine, &t, &ids)) return;
+  } else {
+    if (!pa_item<kKeysRows>(b, c, a.group, work, item, &t)) continue;
+    ids = pa_ids(b, c, t.seq, t.k0 + mine);
+  }
+  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
   const int row = min(t.row0 + j, t.nrows - 1);
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
   const int pos = t.pos0 + tok;
@@ -958,7 +1187,6 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
 
   const int ntile = pa_ceil(max(0, k1 - k0), 16);
   const int nw = ntile > wave ? (ntile - 1 - wave) / 4 + 1 : 0;
-  const PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * (wave + 4 * lane), k1);
   char* const buf = lds + wave * 2 * TILE;
   uint32_t voff[NL];
 #pragma unroll
@@ -1040,12 +1268,21 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
     const char* tile = buf + (i & 1) * TILE;
     const int top = t.kend - 1 - tk;  // the last key any row sees
     bool odd = false;
+    if (!mask) {
+#pragma unroll
+      for (int f = 0; f < NC; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(*(const float*)(tile + (vlane ^ (f * 64)) + r * RB), p[r],
+                                                      o[f], 0, 0, 0);
+      return;
+    }
 #pragma unroll
     for (int f = 0; f < NC; ++f)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v = *(const float*)(tile + (vlane ^ (f * 64)) + r * RB);
-        if (mask) {
+        {
           const bool fin = (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u;
           const bool in = on && 4 * g + r <= top;
           odd |= in && !fin;
@@ -1080,11 +1317,11 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
   }
   __syncthreads();
   const float m = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j]));
-  const float mine = __builtin_amdgcn_exp2f(mrun - m);
+  const float weight = __builtin_amdgcn_exp2f(mrun - m);
   float* const part = (float*)buf;
 #pragma unroll
   for (int f = 0; f < NC; ++f) {
-    const float4_t v = o[f] * mine;
+    const float4_t v = o[f] * weight;
     *(float4_t*)(part + j * DP + 16 * f + 4 * g) = v;
   }
   __syncthreads();
@@ -1101,9 +1338,11 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
     }
     const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
     const long tr = t.first + rt;
-    if (nsp > 1) {
-      const long at = ((long)z * b.rows + tr) * a.nh + h;
-      *(float4_t*)(sp.po + at * c.hd + d) = s;
+    const int at = (kvh * sp.slots + item) * kKeysRows + r;
+    if (k0 == 0 && d == 0)
+      sp.rows[tr * a.nh + h] = (int4_t){at, (DIRECT ? b.n_seqs : t.tiles) * kKeysRows, t.ranges, 0};
+    if (t.ranges > 1) {
+      *(float4_t*)(sp.po + (long)at * c.hd + d) = s;
       if (d == 0) sp.ml[at] = make_float2(mr, l);
       continue;
     }
@@ -1115,6 +1354,9 @@ __global__ __launch_bounds__(256) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, 
     }
     *(float4_t*)((float*)a.out + tr * a.ldo + (long)h * c.hd + d) = s;
   }
+  if constexpr (DIRECT) return;
+  __syncthreads();  // the buffers are free
+  }
 }
 
 // ---- the launch ----------------------------------------------------------------------
@@ -1123,79 +1365,97 @@ enum PaKind { kKeys, kRows1, kRows2, kF32 };
 
 struct PaPlan {
   PaKind kind;
-  int rt, ntiles;  // rows per tile, at most so many tiles
-  int len, n;      // keys per split, splits
-  size_t bytes;    // workspace
+  int rt;             // rows per tile
+  int target, least, most, slots;  // PaSched's
+  bool direct;        // one row tile per sequence, a block for every range there may be
+  int per;            // blocks of a head
+  bool join;          // a tile may have more than one range
+  size_t ml, row, bytes;  // workspace: offsets and size
 };
 
-// Kernel, row tile and key split of a call, from its sizes alone.
+// Kernel, row tile and bounds of the schedule of a call, from its sizes alone.
 int plan(const MxKvCache* c, const MxPagedBatch* b, int nh, PaPlan* p) {
-  const int group = nh / c->n_kv_heads;
+  const int group = nh / c->n_kv_heads, nkv = c->n_kv_heads;
   const long max_q = b->max_q < b->rows ? b->max_q : b->rows;
   const long seqs = b->n_seqs, rows = (long)b->rows * group;
   if (rows >= (1l << 30)) return MX_ERR_UNSUPPORTED;
   p->kind = c->dtype == MX_DT_F32 ? kF32 : max_q * group <= kKeysRows ? kKeys : kRows1;
-  // Two query sets per wave halve the LDS reads per product; int8 heads over 128 dims would spill.
-  if (p->kind == kRows1 && !(c->dtype == MX_DT_I8 && c->head_dim > 128) &&
-      (rows / 128 + seqs) * c->n_kv_heads >= 256)
+  const bool own = p->kind == kKeys || p->kind == kF32;
+  // Two query sets per wave (128 rows) halve the LDS reads per product, but also the tiles: from about
+  // 160 tiles of 64 rows on (4 x 200 rows over 3000 keys: 200 tiles, 112 us with one set, 86 with
+  // two; 1 x 500 rows: 126 tiles, 25 and 30).  Int8 heads over 128 dims would spill.
+  if (p->kind == kRows1 && !(c->dtype == MX_DT_I8 && c->head_dim > 128) && (rows / 64 + seqs) * nkv >= 160)
     p->kind = kRows2;
   p->rt = p->kind == kRows1 ? 64 : p->kind == kRows2 ? 128 : kKeysRows;
-  const long tiles = max_q * group <= p->rt ? seqs : rows / p->rt + seqs;
-  if (tiles * c->n_kv_heads >= (1l << 24)) return MX_ERR_UNSUPPORTED;
-  p->ntiles = (int)tiles;
-  const long blocks = tiles * c->n_kv_heads;
-  const bool own = p->kind == kKeys || p->kind == kF32;
-  const long want = own ? 1024 : 512;     // blocks
-  const long least = own ? 256 : 1024;    // keys of a split
+  const long tiles = rows / p->rt + (seqs < b->rows ? seqs : b->rows);  // at most, of a head
   const long keys = b->max_kv > 0 ? b->max_kv : 1;
-  long n = blocks < want ? (want + blocks - 1) / blocks : 1;
-  long len = (keys + n - 1) / n;
-  if (len < least) len = least;
-  if (own && len > kKeysMax) len = kKeysMax;
-  len = (len + 127) / 128 * 128;
-  n = (keys + len - 1) / len;
-  if (n > 65535) return MX_ERR_UNSUPPORTED;
-  p->len = (int)len;
-  p->n = (int)n;
-  p->bytes = 0;
-  if (n > 1) p->bytes = mx_align_up((size_t)n * b->rows * nh * c->head_dim * 4, 256) + (size_t)n * b->rows * nh * 8;
+  // Items: as many as blocks run at once, by their LDS.  k_pa_keys on rows of 512 bytes: one per CU (64
+  // sequences of 8000 keys, 256 items 184 us, 512 items 191; 32 of 4000 57 and 64); 256 bytes: two
+  // (int8, 48 ragged sequences, 256 items 33 us, 512 27); shorter rows four.
+  const int row_bytes = c->head_dim * pk_esz(c->dtype);
+  p->target = !own ? 512 : row_bytes > (c->dtype == MX_DT_F32 ? 512 : 256) ? 256 : row_bytes > 128 ? 512 : 1024;
+  p->least = own ? 128 : 256;
+  p->most = own ? kKeysMax : 1 << 30;
+  // Items of a head: ranges of len >= least keys, where len >= (sum of keys) / target or is `most`.
+  const long capped = own ? tiles * (keys / kKeysMax) : 0;
+  const long fine = tiles * (keys / p->least);
+  const long extra = 2 * (p->target / nkv + 1);  // (the schedule may count on half the target)
+  long slots = tiles + (extra > capped ? extra : capped);
+  if (slots > tiles + fine) slots = tiles + fine;
+  const long ranges = (keys + p->least - 1) / p->least;
+  p->direct = own && max_q * group <= kKeysRows && seqs * ranges * nkv <= 256;
+  if (p->direct) slots = seqs * ranges;
+  if (slots * nkv * p->rt >= (1l << 31)) return MX_ERR_UNSUPPORTED;
+  p->slots = (int)slots;
+  long per = (p->target + nkv - 1) / nkv;
+  if (per > slots || p->direct) per = slots;
+  if (8 % nkv == 0) per = (per + 8 / nkv - 1) / (8 / nkv) * (8 / nkv);  // whole rounds of the XCDs
+  p->per = (int)per;
+  p->join = keys > p->least;
+  const size_t n = p->join ? (size_t)slots * nkv * p->rt : 0;
+  p->ml = mx_align_up(n * c->head_dim * 4, 256);
+  p->row = p->ml + mx_align_up(n * 8, 256);
+  p->bytes = p->row + (size_t)b->rows * nh * 16;
   return MX_OK;
 }
 
-template <int DT>
-int launch(const PaPlan& p, const PkCache& c, const PkBatch& b, const PaArgs& a, const PaSplit& sp, hipStream_t s) {
-  const dim3 grid(p.ntiles, c.nkv, p.n);
+template <int DT, bool DIRECT>
+int launch(const PaPlan& p, const PkCache& c, const PkBatch& b, const PaArgs& a, const PaSched& sp, hipStream_t s) {
+  const dim3 grid = DIRECT ? dim3(b.n_seqs, c.nkv, p.slots / b.n_seqs) : dim3(p.per * c.nkv);
   mx_clear_error();
   if constexpr (DT == MX_DT_F32) {
-    auto* kern = c.hd <= 32 ? k_pa_f32<32> : c.hd <= 64 ? k_pa_f32<64> : c.hd <= 128 ? k_pa_f32<128> : k_pa_f32<256>;
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp);
+    auto* kern = c.hd <= 32    ? k_pa_f32<32, DIRECT>
+                 : c.hd <= 64  ? k_pa_f32<64, DIRECT>
+                 : c.hd <= 128 ? k_pa_f32<128, DIRECT>
+                               : k_pa_f32<256, DIRECT>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp, p.per);
   } else {
     constexpr int ES = DT == MX_DT_I8 ? 1 : 2;
     const int rb = c.hd * ES;
-    if (p.kind == kKeys) {
-      auto* kern = rb <= 64 ? k_pa_keys<64, DT> : rb <= 128 ? k_pa_keys<128, DT> : k_pa_keys<256, DT>;
-      if constexpr (ES == 2)
-        if (rb > 256) kern = k_pa_keys<512, DT>;
-      hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp);
-    } else {
-      // blocks of a head's XCDs come in whole rounds
-      const int nb = 8 % c.nkv == 0   ? 8 * mx_ceil_div(p.ntiles, 8 / c.nkv)
-                     : c.nkv % 8 == 0 ? p.ntiles * c.nkv
-                                      : p.ntiles * c.nkv;
-      auto* kern = rb <= 64 ? k_pa_rows<64, DT, 1> : rb <= 128 ? k_pa_rows<128, DT, 1> : k_pa_rows<256, DT, 1>;
+    auto* kern = rb <= 64    ? k_pa_keys<64, DT, DIRECT>
+                 : rb <= 128 ? k_pa_keys<128, DT, DIRECT>
+                             : k_pa_keys<256, DT, DIRECT>;
+    if constexpr (ES == 2)
+      if (rb > 256) kern = k_pa_keys<512, DT, DIRECT>;
+    if constexpr (!DIRECT) {
+      if (p.kind == kRows1)
+        kern = rb <= 64 ? k_pa_rows<64, DT, 1> : rb <= 128 ? k_pa_rows<128, DT, 1> : k_pa_rows<256, DT, 1>;
       if (p.kind == kRows2) kern = rb <= 64 ? k_pa_rows<64, DT, 2> : k_pa_rows<128, DT, 2>;
       if constexpr (ES == 2) {
         if (p.kind == kRows2 && rb > 128) kern = k_pa_rows<256, DT, 2>;
-        if (rb > 256) kern = p.kind == kRows1 ? k_pa_rows<512, DT, 1> : k_pa_rows<512, DT, 2>;
+        if (p.kind == kRows1 && rb > 256) kern = k_pa_rows<512, DT, 1>;
+        if (p.kind == kRows2 && rb > 256) kern = k_pa_rows<512, DT, 2>;
       }
-      hipLaunchKernelGGL(kern, dim3(nb, 1, p.n), dim3(256), 0, s, c, b, a, sp, p.ntiles);
     }
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, b, a, sp, p.per);
   }
   MX_TRY(mx_launch_status());
-  if (p.n == 1) return MX_OK;
+  if (!p.join) return MX_OK;
   typedef typename std::conditional<DT == MX_DT_F32, float, half_t>::type OT;
-  auto* join = p.rt == 64 ? k_pa_join<64, OT> : p.rt == 128 ? k_pa_join<128, OT> : k_pa_join<16, OT>;
-  hipLaunchKernelGGL(join, dim3((unsigned)(((long)b.rows * a.nh + 3) / 4)), dim3(256), 0, s, c, b, a, sp);
+  if (p.rt == kKeysRows)
+    hipLaunchKernelGGL((k_pa_join<OT, true>), dim3(b.rows, a.nh), dim3(256), 0, s, c, b, a, sp);
+  else
+    hipLaunchKernelGGL((k_pa_join<OT, false>), dim3(b.rows, mx_ceil_div(a.nh, 4)), dim3(256), 0, s, c, b, a, sp);
   return mx_launch_status();
 }
 
@@ -1234,18 +1494,18 @@ extern "C" int mx_paged_attn(const MxKvCache* cache, const MxPagedBatch* batch,
   if (batch->rows == 0 || batch->n_seqs == 0) return MX_OK;
   PaPlan p;
   MX_TRY(plan(cache, batch, args->n_heads, &p));
-  if (p.bytes) {
-    if (!workspace || workspace_bytes < p.bytes) return MX_ERR_WORKSPACE;
-    if (!mx_aligned16(workspace)) return MX_ERR_ALIGNMENT;
-  }
+  if (!workspace || workspace_bytes < p.bytes) return MX_ERR_WORKSPACE;
+  if (!mx_aligned16(workspace)) return MX_ERR_ALIGNMENT;
   const PkCache c = pk_cache(cache);
   const PkBatch b = pk_batch(batch);
   const PaArgs a{args->q, args->out, args->gate, args->ldq, args->ldo, args->ldg, args->n_heads,
                  args->n_heads / cache->n_kv_heads, args->scale};
-  const size_t ml = mx_align_up((size_t)p.n * b.rows * a.nh * c.hd * 4, 256);
-  const PaSplit sp{p.len, p.n, (float*)workspace, (float2*)((char*)workspace + ml)};
+  char* const ws = (char*)workspace;
+  const PaSched sp{p.target, p.least, p.most, p.slots, (float*)ws, (float2*)(ws + p.ml), (int4_t*)(ws + p.row)};
   const hipStream_t s = (hipStream_t)stream;
-  return cache->dtype == MX_DT_F32   ? launch<MX_DT_F32>(p, c, b, a, sp, s)
-         : cache->dtype == MX_DT_F16 ? launch<MX_DT_F16>(p, c, b, a, sp, s)
-                                     : launch<MX_DT_I8>(p, c, b, a, sp, s);
+  if (cache->dtype == MX_DT_F32)
+    return p.direct ? launch<MX_DT_F32, true>(p, c, b, a, sp, s) : launch<MX_DT_F32, false>(p, c, b, a, sp, s);
+  if (cache->dtype == MX_DT_F16)
+    return p.direct ? launch<MX_DT_F16, true>(p, c, b, a, sp, s) : launch<MX_DT_F16, false>(p, c, b, a, sp, s);
+  return p.direct ? launch<MX_DT_I8, true>(p, c, b, a, sp, s) : launch<MX_DT_I8, false>(p, c, b, a, sp, s);
 }
