@@ -38,7 +38,7 @@ struct GdArgs {
 constexpr int kCols = 32;
 
 template <int NR, typename XT>
-__global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a) {
+__global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
   constexpr int DKP = 32 * NR;
   __shared__ float sk[2][DKP], sq[2][DKP];
   __shared__ float red[2][4][2][kCols];  // [buffer][wave][r, p][column]
@@ -47,6 +47,7 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a) {
   const int hk = h / a.rep, grp = tid >> 3;
   const bool col = c0 < a.dv;
   const int t0 = a.q_start[seq], t1 = min(a.q_start[seq + 1], a.rows);
+  if (t1 - t0 >= below) return;
   const int in = a.slot_in[seq], out = a.slot_out[seq];
   const long head = (long)a.dk * a.dv;
   float4 s[NR];
@@ -143,6 +144,586 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------
+// Chunk by chunk.  For the tokens t = 1 .. 64 of a chunk, with G_t = g_1 + .. + g_t, S the
+// state before it and k, q as they go in (normalised, q scaled):
+//   A_ts = beta_t e^{G_t - G_s} k_t.k_s  (s < t)     T = (I + A)^-1
+//   u = T x,  x_t = beta_t (v_t - e^{G_t} k_t^T S)   P_ts = e^{G_t - G_s} q_t.k_s  (s <= t)
+//   o_t = e^{G_t} q_t^T S + sum_s P_ts u_s           S <- e^{G_64} S + sum_t e^{G_64 - G_t} k_t u_t^T
+// k_gd_prep forms T and P of every chunk at once; k_gd_walk takes a sequence's chunks in order,
+// 16 columns of a head's state per four waves.  The exponents are differences <= 0 of one prefix
+// sum, which is kept in 64 bits: token decays of -256 (e^-256 is 0 in 32 bits) next to
+// decays near 0 leave the differences their digits.  The norms and the scale of q and k are
+// factors of a token, so the products take q and k as they are stored.
+//
+// The products run on the fp16 matrix instructions at fp32's precision: x = 2^e (hi + lo), both fp16,
+// hi = x 2^-e rounded and lo the rest rounded: 22 bits and the sign of lo, an error of 2^-23 |x|, and
+// at least 2^-39 of the largest element that shares the e (of a token's row of k, a row of T, a column
+// of S, 16 tokens of a column of x and u).  hi hi + hi lo + lo hi leave out 2^-22 of a product;
+// fp16 k and q are exact as they are, and take two products.  Sums are in 32 bits.
+// ------------------------------------------------------------------------------------
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t gd_lds_s4;
+
+constexpr int kC = 64;  // tokens of a chunk
+
+// What k_gd_prep leaves of a (chunk, value head): T and P as planes [hi, lo][64][64], and factors
+// of the tokens.
+enum { kFa, kFb, kFc, kFbeta, kFt, kFp, kFkm, kFsk, kFsq, kFend, kFactors };
+constexpr int kPlane = kC * kC * 2, kOffP = 2 * kPlane, kOffF = 4 * kPlane, kRec = kOffF + kFactors * kC * 4;
+
+__device__ __forceinline__ float4_t gd_mfma(half8_t a, half8_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float4_t gd_mfma(half4_t a, half4_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+// Over 16 columns: a holds 4 consecutive columns of the lane's A row, b the same of its B column.
+__device__ __forceinline__ float4_t gd_mfma(const float4_t& a, const float4_t& b, float4_t c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// 2^-e and 2^e with m 2^-e in [2^14, 2^15): fp16 holds twice that.  Under 2^-86 they stay; an
+// infinite or NaN m gives a finite factor.
+__device__ __forceinline__ float gd_scale(float m, float& inv) {
+  const int e = max((int)((__float_as_uint(m) >> 23) & 255), 41);
+  inv = __uint_as_float((uint32_t)(e - 14) << 23);
+  return __uint_as_float((uint32_t)(268 - e) << 23);
+}
+
+template <int N>
+__device__ __forceinline__ void gd_split(const float* x, float s, half_t* hi, half_t* lo) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float y = x[e] * s;
+    hi[e] = (half_t)y;
+    lo[e] = (half_t)(y - (float)hi[e]);
+  }
+}
+
+__device__ __forceinline__ float gd_max4(const float4_t& x) {
+  return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+}
+// Max and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float gd_max16(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float gd_sum16(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// Chunk slots: sequence i's start at q_start[i] / 64 + i, which leaves it ceil(n / 64) of them.
+__device__ __forceinline__ int gd_base(const int* q_start, int i) { return q_start[i] / kC + i; }
+
+// The sequence of chunk slot id: the last i < n with base(i) <= id.  The whole wave looks.
+__device__ __forceinline__ int gd_seq_of(const int* __restrict__ q_start, int n, int id) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n - 1;
+  while (hi > lo) {
+    const int step = (hi - lo + 63) >> 6;
+    const int at = lo + (lane + 1) * step;
+    const bool below = at <= hi && gd_base(q_start, at) <= id;
+    const int nlo = lo + __popcll(__builtin_amdgcn_ballot_w64(below)) * step;
+    hi = min(hi, nlo + step - 1);
+    lo = nlo;
+  }
+  return lo;
+}
+
+// Elements d .. d + 7 of a row of dk elements as fp32 or fp16; zeros past its end and, with !live,
+// throughout (row then points at a row there is).
+template <typename XT>
+struct GdVec;
+template <>
+struct GdVec<half_t> {
+  typedef half8_t T;
+};
+template <>
+struct GdVec<float> {
+  typedef float T __attribute__((ext_vector_type(8)));
+};
+template <typename XT>
+__device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, int dk, bool live, bool wide) {
+  typename GdVec<XT>::T x;
+  if (wide) {  // rows of whole 16-byte pieces
+    constexpr int P = sizeof(XT) / 2;
+    union {
+      int4_t i[P];
+      typename GdVec<XT>::T x;
+    } u;
+#pragma unroll
+    for (int p = 0; p < P; ++p) u.i[p] = live && d < dk ? *(const int4_t*)(row + d + p * 4) : (int4_t)0;
+    x = u.x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = live && d + e < dk ? row[d + e] : (XT)0;
+  }
+  return x;
+}
+
+// T and P of the chunks.  A block: one chunk of one key head, and its value heads in turn; wave w
+// forms the rows 16 w .. of k k^T and q k^T (fp16 rows: exact products; fp32 rows: fp32 matrix
+// instructions), operands straight from memory, as both are rows of k and q.  T: the
+// 16 x 16 blocks on the diagonal by substitution, a column per lane; then pairs, T_10 = -T_11 A_10
+// T_00, twice.  A product's result has the layout of the next one's right operand, so
+// only T's pieces go through LDS.
+template <int DK, typename XT>
+__global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws, int from, int wide) {
+  constexpr int W = kC + 4;
+  __shared__ float sa[kC * W], st[kC * W], sp[kC * W];
+  __shared__ double sg[kC];
+  __shared__ float sk2[kC], sq2[kC], skm[kC], sqm[kC], sbeta[kC], sbad[kC];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
+  const int id = blockIdx.x, hk = blockIdx.y;
+  const int seq = gd_seq_of(a.q_start, a.n_seqs, id);
+  const int t0 = max(a.q_start[seq], 0), n = min(a.q_start[seq + 1], a.rows) - t0;
+  const int c0 = (id - gd_base(a.q_start, seq)) * kC;
+  if (n < from || c0 >= n || c0 < 0) return;
+  const int live = min(n - c0, kC);
+
+  auto row = [&](const void* x, long ld, int t) {
+    return (const XT*)x + (long)(t0 + c0 + min(t, live - 1)) * ld + (long)hk * a.dk;
+  };
+  float4_t kk[4] = {}, qk[4] = {};
+  float k2 = 0.f, q2 = 0.f, km = 0.f, qm = 0.f;
+  {
+    const int t = 16 * w + j;
+    const XT *kr = row(a.k, a.ldk, t), *qr = row(a.q, a.ldq, t);
+    for (int m = 0; m < DK / 32; ++m) {
+      const int d = 32 * m + 8 * q;
+      const auto kf = gd_load8<XT>(kr, d, a.dk, t < live, wide);
+      const auto qf = gd_load8<XT>(qr, d, a.dk, t < live, wide);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)kf[e], y = (float)qf[e];
+        k2 += x * x;
+        q2 += y * y;
+        km = fmaxf(km, fabsf(x));
+        qm = fmaxf(qm, fabsf(y));
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (b > w) continue;
+        const auto bf = gd_load8<XT>(row(a.k, a.ldk, 16 * b + j), d, a.dk, 16 * b + j < live, wide);
+        if constexpr (sizeof(XT) == 2) {
+          kk[b] = gd_mfma(kf, bf, kk[b]);
+          qk[b] = gd_mfma(qf, bf, qk[b]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4_t x = {bf[e], bf[e + 1], bf[e + 2], bf[e + 3]};
+            kk[b] = gd_mfma((float4_t){kf[e], kf[e + 1], kf[e + 2], kf[e + 3]}, x, kk[b]);
+            qk[b] = gd_mfma((float4_t){qf[e], qf[e + 1], qf[e + 2], qf[e + 3]}, x, qk[b]);
+          }
+        }
+      }
+    }
+    k2 = gd_sum16(k2);
+    q2 = gd_sum16(q2);
+    km = gd_max16(km);
+    qm = gd_max16(qm);
+    if (q == 0) {
+      sk2[t] = a.norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.f;
+      sq2[t] = (a.norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.f) * a.scale;
+      skm[t] = km;
+      sqm[t] = qm;
+    }
+  }
+  for (int r = 0; r < a.rep; ++r) {
+    const int h = hk * a.rep + r;
+    char* rec = ws + ((long)id * a.nv + h) * kRec;
+    float* f = (float*)(rec + kOffF);
+    __syncthreads();  // the buffers are free; the norms are there
+    if (w == 0) {
+      const int t = lane;
+      const long at = (long)(t0 + c0 + min(t, live - 1)) * a.nv + h;
+      float g = t < live ? a.g[at] : 0.f;
+      g = g < -256.f ? -256.f : g;
+      sbeta[t] = t < live ? a.beta[at] : 0.f;
+      double G = g;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const double up = __shfl_up(G, o);
+        if (t >= o) G += up;
+      }
+      sg[t] = G;
+      sbad[t] = 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (b > w) continue;
+      const int s = 16 * b + j;
+      const double gs = sg[s];
+      const float ks = sk2[s];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = 16 * w + 4 * q + e;
+        const float decay = expf((float)(sg[t] - gs)) * ks;
+        float x = s < t ? sbeta[t] * sk2[t] * decay * kk[b][e] : 0.f;
+        // A row that is not finite (a NaN key, gate or decay) leaves T to the rows before it.
+        if (!(fabsf(x) <= 3.0e38f)) {
+          sbad[t] = 1.f;
+          x = 0.f;
+        }
+        sa[t * W + s] = x;
+        sp[t * W + s] = s <= t ? sq2[t] * decay * qk[b][e] : 0.f;
+      }
+    }
+    {  // the diagonal block's inverse: column j, of this wave's own rows
+      const float* d = sa + (16 * w) * W + 16 * w;
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float y = i == j ? 1.f : 0.f;
+#pragma unroll
+        for (int m = 0; m < i; m += 4) {
+          const float4_t c = *(const float4_t*)(d + i * W + m);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (m + e < i) y -= c[e] * x[m + e];
+        }
+        x[i] = y;
+      }
+      if (q == 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[(16 * w + i) * W + 16 * w + j] = x[i];
+    }
+    __syncthreads();
+    auto rows = [&](const float* x, int I, int J) { return *(const float4_t*)(x + (16 * I + j) * W + 16 * J + 4 * q); };
+    auto cols = [&](const float* x, int I, int J) {
+      const float* p = x + (16 * I + 4 * q) * W + 16 * J + j;
+      return (float4_t){p[0], p[W], p[2 * W], p[3 * W]};
+    };
+    auto put = [&](int I, int J, const float4_t& z) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[(16 * I + 4 * q + e) * W + 16 * J + j] = -z[e];
+    };
+    if (w < 2) {
+      const int I = 2 * w + 1, J = 2 * w;
+      const float4_t y = gd_mfma(rows(sa, I, J), cols(st, J, J), (float4_t)0.f);
+      put(I, J, gd_mfma(rows(st, I, I), y, (float4_t)0.f));
+    }
+    __syncthreads();
+    {
+      const int I = 2 + (w >> 1), J = w & 1;
+      float4_t z = (float4_t)0.f;
+      for (int K = 2; K <= I; ++K) {
+        float4_t y = (float4_t)0.f;
+        for (int L = J; L < 2; ++L) y = gd_mfma(rows(sa, K, L), cols(st, L, J), y);
+        z = gd_mfma(rows(st, I, K), y, z);
+      }
+      put(I, J, z);
+    }
+    __syncthreads();
+    const int t = tid >> 2, part = tid & 3;  // a row, 16 of its columns
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float* x = (i ? sp : st) + t * W + 16 * part;
+      float y[16], m = 0.f, inv;
+      if (part <= t >> 4) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          y[e] = x[e];
+          m = fmaxf(m, fabsf(y[e]));
+        }
+      }
+      m = fmaxf(m, __shfl_xor(m, 1));
+      m = fmaxf(m, __shfl_xor(m, 2));
+      const float s = gd_scale(m, inv);
+      if (part <= t >> 4) {
+        union {
+          half_t h[2][16];
+          int4_t v[2][2];
+        } u;
+        gd_split<16>(y, s, u.h[0], u.h[1]);
+        char* to = rec + i * kOffP + t * (kC * 2) + part * 32;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          *(int4_t*)(to + p * kPlane) = u.v[p][0];
+          *(int4_t*)(to + p * kPlane + 16) = u.v[p][1];
+        }
+      }
+      if (part == 0) f[(i ? kFp : kFt) * kC + t] = inv;
+    }
+    if (tid < kC) {
+      const double G = sg[tid], end = sg[kC - 1];
+      float ki = 1.f, qi = 1.f, ks = 1.f, qs = 1.f;
+      if constexpr (sizeof(XT) == 4) {
+        ks = gd_scale(skm[tid], ki);
+        qs = gd_scale(sqm[tid], qi);
+      }
+      const float eg = expf((float)G);
+      f[kFa * kC + tid] = sbad[tid] != 0.f ? __builtin_nanf("") : eg * sk2[tid] * ki;
+      f[kFb * kC + tid] = eg * sq2[tid] * qi;
+      f[kFc * kC + tid] = expf((float)(end - G)) * sk2[tid] * ki;
+      f[kFbeta * kC + tid] = sbeta[tid];
+      f[kFkm * kC + tid] = skm[tid] * ks;
+      f[kFsk * kC + tid] = ks;
+      f[kFsq * kC + tid] = qs;
+      f[kFend * kC + tid] = expf((float)end);
+    }
+  }
+}
+
+// A sequence's chunks in order.  Waves come in fours: wave (rt, nt) has the tokens 16 rt .. of
+// the chunk and the 16 columns 16 nt .. of the block's, and the rows 16 SL rt .. of the state, in
+// accumulators.  Per chunk three barriers:
+//   the state's planes to LDS  | k^T S and q^T S; x to LDS, k to LDS  | u = T x to LDS  | o and S
+// A column's factor 2^e of the state's planes has to be known before all waves have the new state: from
+// the bound e^G max|S| + 64 max|k u|, whose maxima went through LDS with x and u before.  It may
+// exceed the maximum by 2^10 before the 2^-39 above reaches fp32's own 2^-24.
+//
+// A NaN or infinity in x (a NaN in v is one of its column, in k of every column) would meet the zeros
+// above T's diagonal: it is taken out, and u, o and S from that row on are NaN, as token by
+// token.
+template <int DK, int NT, typename XT>
+__global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __restrict__ ws, int from, int wide,
+                                                      int groups) {
+  constexpr int SL = DK / 64, NP = sizeof(XT) == 2 ? 1 : 2, NC = 16 * NT;
+  constexpr int M = DK / 32;
+  __shared__ __align__(16) half_t ss[2][NC * DK];        // the state [column][row]
+  __shared__ __align__(16) half_t skey[NP][kC * DK];     // k [token][dim]
+  __shared__ __align__(16) half_t sx[2][NC * kC];        // x, u, c u: [column][token]
+  __shared__ __align__(16) half_t su[2][NC * kC], sd[2][NC * kC];
+  __shared__ float sxi[4][NC], sui[4][NC], sdi[4][NC];   // their 2^e, per 16 tokens
+  __shared__ float smax[2][4][NC], sinc[4][NC];
+  __shared__ int sfirst[NC];
+  __shared__ __align__(16) float sf[2][kFactors * kC];
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rt = wave & 3, nt = wave >> 2, col = 16 * nt + j;
+  const int seq = blockIdx.y;
+  // Slices of a key head's value heads next to each other on one XCD: they read the same k, q, T, P.
+  int hk, r;
+  const int slices = (a.dv + NC - 1) / NC, per = slices * a.rep;
+  if (groups) {
+    hk = (blockIdx.x >> 3) / per * 8 + (blockIdx.x & 7);
+    r = (blockIdx.x >> 3) % per;
+  } else {
+    hk = blockIdx.x / per;
+    r = blockIdx.x % per;
+  }
+  const int h = hk * a.rep + r / slices, v0 = r % slices * NC;
+  const int t0 = max(a.q_start[seq], 0), n = min(a.q_start[seq + 1], a.rows) - t0;
+  if (n < from) return;
+  const int in = a.slot_in[seq], out = a.slot_out[seq];
+  const char* rec = ws + ((long)gd_base(a.q_start, seq) * a.nv + h) * kRec;
+  const bool cl = v0 + col < a.dv;
+  const long head = (long)a.dk * a.dv;
+  const XT* kp = (const XT*)a.k + (long)t0 * a.ldk + (long)hk * a.dk;
+  const XT* qp = (const XT*)a.q + (long)t0 * a.ldq + (long)hk * a.dk;
+  const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + v0 + col;
+  XT* op = (XT*)a.o + (long)t0 * a.ldo + (long)h * a.dv + v0 + col;
+
+  float4_t s[SL];
+#pragma unroll
+  for (int i = 0; i < SL; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 16 * (SL * rt + i) + 4 * q + e;
+      s[i][e] = in >= 0 && in < a.n_slots && cl && d < a.dk
+                    ? a.state[((long)in * a.nv + h) * head + (long)d * a.dv + v0 + col]
+                    : 0.f;
+    }
+
+  // What a chunk reads, a chunk ahead: in registers until the products before it are done.
+  typename GdVec<XT>::T kf[M], qf[M];
+  half4_t tf[2][4], pf[2][4];
+  XT vf[4];
+  float4 ff;
+  const int chunks = (n + kC - 1) / kC;
+  auto load_rows = [&](int c) {
+    const int t = c * kC + 16 * rt + j;
+    const XT *kr = kp + (long)min(t, n - 1) * a.ldk, *qr = qp + (long)min(t, n - 1) * a.ldq;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      kf[m] = gd_load8<XT>(kr, 32 * m + 8 * q, a.dk, t < n, wide);
+      qf[m] = gd_load8<XT>(qr, 32 * m + 8 * q, a.dk, t < n, wide);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int tv = c * kC + 16 * rt + 4 * q + e;
+      vf[e] = tv < n && cl ? vp[(long)tv * a.ldv] : (XT)0;
+    }
+  };
+  auto load_tri = [&](int c, int off, half4_t (&x)[2][4]) {
+    const char* p = rec + (long)c * a.nv * kRec + off + (16 * rt + j) * (kC * 2) + 8 * q;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        x[i][b] = b <= rt ? *(const half4_t*)(p + i * kPlane + 32 * b) : (half4_t)(half_t)0;
+  };
+  auto load_factors = [&](int c) {
+    if (tid < kFactors * kC / 4) ff = *(const float4*)(rec + (long)c * a.nv * kRec + kOffF + 16 * tid);
+  };
+  auto factor = [&](const float* f, int k) { return *(const float4_t*)(f + k * kC + 16 * rt + 4 * q); };
+  // [column][token] tiles: 8-byte pieces, swizzled by the column
+  auto piece = [&](int b) { return col * kC + ((4 * b + q) ^ j) * 4; };
+  auto put = [&](half_t (&to)[2][NC * kC], const float4_t& x, float (&inv)[4][NC]) {
+    float iv;
+    const float sc = gd_scale(gd_max16(gd_max4(x)), iv);
+    half4_t p[2];
+    gd_split<4>((const float*)&x, sc, (half_t*)&p[0], (half_t*)&p[1]);
+    *(half4_t*)&to[0][piece(rt)] = p[0];
+    *(half4_t*)&to[1][piece(rt)] = p[1];
+    if (q == 0) inv[rt][col] = iv;
+  };
+  // sum over the token blocks up to rt of x (row planes) times what put() left
+  auto tri = [&](const half4_t (&x)[2][4], const half_t (&y)[2][NC * kC], const float (&inv)[4][NC]) {
+    float4_t z = (float4_t)0.f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (b > rt) continue;
+      const half4_t hi = *(const half4_t*)&y[0][piece(b)], lo = *(const half4_t*)&y[1][piece(b)];
+      float4_t c = gd_mfma(x[1][b], hi, (float4_t)0.f);
+      c = gd_mfma(x[0][b], lo, c);
+      c = gd_mfma(x[0][b], hi, c);
+      z += c * inv[b][col];
+    }
+    return z;
+  };
+
+  load_rows(0);
+  load_tri(0, 0, tf);
+  load_tri(0, kOffP, pf);
+  load_factors(0);
+  float bound = 0.f;
+#pragma unroll
+  for (int i = 0; i < SL; ++i) bound = fmaxf(bound, gd_max4(s[i]));
+  bound = gd_max16(bound);
+  if (q == 0) smax[1][rt][col] = bound;
+  if (tid < NC) sfirst[tid] = kC;
+  if (tid < kFactors * kC / 4) *(float4*)&sf[0][4 * tid] = ff;
+  __syncthreads();
+  bound = fmaxf(fmaxf(smax[1][0][col], smax[1][1][col]), fmaxf(smax[1][2][col], smax[1][3][col]));
+
+  for (int c = 0; c < chunks; ++c) {
+    const float* f = sf[c & 1];
+    float sinv;
+    {  // the state's planes
+      const float sc = gd_scale(bound, sinv);
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < SL; ++i) {
+        half4_t p[2];
+        gd_split<4>((const float*)&s[i], sc, (half_t*)&p[0], (half_t*)&p[1]);
+        const int pc = 4 * (SL * rt + i) + q;  // 8-byte piece of the column
+        const int at = col * DK + (((pc >> 1) ^ (j & 7)) << 3) + (pc & 1) * 4;
+        *(half4_t*)&ss[0][at] = p[0];
+        *(half4_t*)&ss[1][at] = p[1];
+        m = fmaxf(m, gd_max4(s[i]));
+      }
+      m = gd_max16(m);
+      if (q == 0) smax[c & 1][rt][col] = m;
+    }
+    __syncthreads();
+    float4_t o = (float4_t)0.f;
+    {  // k^T S, q^T S
+      float4_t x = (float4_t)0.f;
+      const float ks = NP == 2 ? f[kFsk * kC + 16 * rt + j] : 1.f, qs = NP == 2 ? f[kFsq * kC + 16 * rt + j] : 1.f;
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int at = col * DK + (((4 * m + q) ^ (j & 7)) << 3);
+        const half8_t hi = *(const half8_t*)&ss[0][at], lo = *(const half8_t*)&ss[1][at];
+        half8_t kh, kl, qh, ql;
+        if constexpr (NP == 1) {
+          kh = kf[m];
+          qh = qf[m];
+        } else {
+          gd_split<8>((const float*)&kf[m], ks, (half_t*)&kh, (half_t*)&kl);
+          gd_split<8>((const float*)&qf[m], qs, (half_t*)&qh, (half_t*)&ql);
+          x = gd_mfma(kl, hi, x);
+          o = gd_mfma(ql, hi, o);
+        }
+        x = gd_mfma(kh, lo, x);
+        o = gd_mfma(qh, lo, o);
+        x = gd_mfma(kh, hi, x);
+        o = gd_mfma(qh, hi, o);
+        if (nt == 0) {
+          const int t = 16 * rt + j, sw = 2 * (t & 3) + ((t >> 2) & 1);
+          *(half8_t*)&skey[0][t * DK + (((4 * m + q) ^ sw) << 3)] = kh;
+          if constexpr (NP == 2) *(half8_t*)&skey[1][t * DK + (((4 * m + q) ^ sw) << 3)] = kl;
+        }
+      }
+      const float4_t fa = factor(f, kFa), fb = factor(f, kFbeta);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = fb[e] * ((float)vf[e] - fa[e] * (x[e] * sinv));
+        if (!(fabsf(x[e]) <= 3.0e38f)) {
+          atomicMin(&sfirst[col], 16 * rt + 4 * q + e);
+          x[e] = 0.f;
+        }
+      }
+      o = o * sinv * factor(f, kFb);
+      put(sx, x, sxi);
+    }
+    const bool more = c + 1 < chunks;
+    if (more) {
+      load_rows(c + 1);
+      load_factors(c + 1);
+    }
+    __syncthreads();
+    const int first = sfirst[col];
+    {  // u
+      const float4_t u = tri(tf, sx, sxi) * factor(f, kFt);
+      const float4_t d = u * factor(f, kFc), km = factor(f, kFkm);
+      put(su, u, sui);
+      put(sd, d, sdi);
+      const float m = gd_max16(gd_max4(d * km));
+      if (q == 0) sinc[rt][col] = m;
+    }
+    if (more) load_tri(c + 1, 0, tf);
+    __syncthreads();
+    o += tri(pf, su, sui) * factor(f, kFp);
+    if (more) load_tri(c + 1, kOffP, pf);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = 16 * rt + 4 * q + e;
+      if (cl && c * kC + t < n) op[(long)(c * kC + t) * a.ldo] = (XT)(t < first ? o[e] : __builtin_nanf(""));
+    }
+    const float end = f[kFend * kC];
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      s[i] *= end;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const half4_t hi = *(const half4_t*)&sd[0][piece(b)], lo = *(const half4_t*)&sd[1][piece(b)];
+        // k's 16 dims of the slab as rows: lane (j, q) dim j of the tokens 4 q ..
+        const int t = 16 * b + 4 * q + (j >> 2), sw = 2 * (t & 3) + ((t >> 2) & 1);
+        const int at = t * DK + (((2 * (SL * rt + i) + ((j & 3) >> 1)) ^ sw) << 3) + (j & 1) * 4;
+        auto key = [&](int p) {
+          return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((gd_lds_s4*)&skey[p][at]));
+        };
+        const half4_t kh = key(0);
+        float4_t z = (float4_t)0.f;
+        if constexpr (NP == 2) z = gd_mfma(key(NP - 1), hi, z);
+        z = gd_mfma(kh, lo, z);
+        z = gd_mfma(kh, hi, z);
+        s[i] += z * sdi[b][col];
+      }
+      if (first < kC) s[i] = (float4_t)__builtin_nanf("");
+    }
+    bound = fmaxf(fmaxf(smax[c & 1][0][col], smax[c & 1][1][col]), fmaxf(smax[c & 1][2][col], smax[c & 1][3][col]));
+    bound = end * bound + 64.f * fmaxf(fmaxf(sinc[0][col], sinc[1][col]), fmaxf(sinc[2][col], sinc[3][col]));
+    if (more && tid < kFactors * kC / 4) *(float4*)&sf[(c + 1) & 1][4 * tid] = ff;
+    if (tid < NC) sfirst[tid] = kC;
+  }
+  if (out < 0 || out >= a.n_slots || !cl) return;
+#pragma unroll
+  for (int i = 0; i < SL; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 16 * (SL * rt + i) + 4 * q + e;
+      if (d < a.dk) a.state[((long)out * a.nv + h) * head + (long)d * a.dv + v0 + col] = s[i][e];
+    }
+}
+
 int check(const MxGatedDelta* d) {
   if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta || !d->o || !d->state || !d->slot_in ||
       !d->slot_out || !d->q_start)
@@ -193,14 +774,41 @@ GdArgs args_of(const MxGatedDelta* d) {
 }
 
 template <typename XT>
-int launch_recurrent(const GdArgs& a, hipStream_t s) {
+int launch_recurrent(const GdArgs& a, int below, hipStream_t s) {
   auto* kern = a.dk <= 32    ? k_gd_recurrent<1, XT>
                : a.dk <= 64  ? k_gd_recurrent<2, XT>
                : a.dk <= 128 ? k_gd_recurrent<4, XT>
                              : k_gd_recurrent<8, XT>;
   mx_clear_error();
-  hipLaunchKernelGGL(kern, dim3(mx_ceil_div(a.dv, kCols), a.nv, a.n_seqs), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(kern, dim3(mx_ceil_div(a.dv, kCols), a.nv, a.n_seqs), dim3(256), 0, s, a, below);
   return mx_launch_status();
+}
+
+constexpr int kFrom = 24;  // rows from which a sequence goes chunk by chunk
+
+bool chunked(const MxGatedDelta* d) {
+  return d->head_dim_k <= 128 && (d->max_q < d->rows ? d->max_q : d->rows) >= kFrom;
+}
+
+template <int DK, typename XT>
+int launch_chunked(const GdArgs& a, char* ws, hipStream_t s) {
+  constexpr int NT = 1;
+  const int esz = sizeof(XT);
+  const int wide = a.dk % 8 == 0 && mx_aligned16(a.q) && mx_aligned16(a.k) && a.ldq * esz % 16 == 0 && a.ldk * esz % 16 == 0;
+  mx_clear_error();
+  hipLaunchKernelGGL((k_gd_prep<DK, XT>), dim3(a.rows / kC + a.n_seqs, a.nk), dim3(256), 0, s, a, ws, kFrom, wide);
+  MX_TRY(mx_launch_status());
+  hipLaunchKernelGGL((k_gd_walk<DK, NT, XT>), dim3(mx_ceil_div(a.dv, 16 * NT) * a.nv, a.n_seqs), dim3(256 * NT), 0, s,
+                     a, ws, kFrom, wide, a.nk % 8 == 0);
+  return mx_launch_status();
+}
+
+template <typename XT>
+int run(const MxGatedDelta* d, const GdArgs& a, char* ws, hipStream_t s) {
+  const bool long_rows = chunked(d);
+  MX_TRY(launch_recurrent<XT>(a, long_rows ? kFrom : 1 << 30, s));
+  if (!long_rows) return MX_OK;
+  return a.dk <= 64 ? launch_chunked<64, XT>(a, ws, s) : launch_chunked<128, XT>(a, ws, s);
 }
 
 }  // namespace
@@ -208,16 +816,19 @@ int launch_recurrent(const GdArgs& a, hipStream_t s) {
 extern "C" int mx_gated_delta_rule_workspace_size(const MxGatedDelta* args, size_t* nbytes) {
   if (!nbytes) return MX_ERR_INVALID;
   MX_TRY(check(args));
-  *nbytes = 0;
+  *nbytes = chunked(args) ? ((size_t)args->rows / kC + args->n_seqs) * args->n_v_heads * kRec : 0;
   return MX_OK;
 }
 
 extern "C" int mx_gated_delta_rule(const MxGatedDelta* args, void* workspace,
                                    size_t workspace_bytes, void* stream) {
-  MX_TRY(check(args));
+  size_t need;
+  MX_TRY(mx_gated_delta_rule_workspace_size(args, &need));
   if (args->n_seqs == 0) return MX_OK;
+  if (need && (!workspace || workspace_bytes < need)) return MX_ERR_WORKSPACE;
+  if (need && !mx_aligned16(workspace)) return MX_ERR_ALIGNMENT;
   const GdArgs a = args_of(args);
   const hipStream_t s = (hipStream_t)stream;
-  return args->x_dtype == MX_DT_F32 ? launch_recurrent<float>(a, s)
-                                    : launch_recurrent<half_t>(a, s);
+  return args->x_dtype == MX_DT_F32 ? run<float>(args, a, (char*)workspace, s)
+                                    : run<half_t>(args, a, (char*)workspace, s);
 }
