@@ -163,21 +163,31 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
 // fp16 k and q are exact as they are, and take two products.  Sums are in 32 bits.
 // ------------------------------------------------------------------------------------
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef __amdgpu_buffer_rsrc_t mx_rsrc_t;
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t gd_lds_s4;
 
 constexpr int kC = 64;  // tokens of a chunk
 
-// What k_gd_prep leaves of a (chunk, value head): T and P as planes [hi, lo][64][64], and factors
-// of the tokens.
-enum { kFa, kFb, kFc, kFbeta, kFt, kFp, kFkm, kFsk, kFsq, kFend, kFactors };
+// What k_gd_prep leaves of a (chunk, value head): T and P as planes hi, lo, and factors of the
+// tokens; of a (chunk, key head): k and q, as they are or as planes.  All of it lane by lane as the
+// walk's matrix instructions take it, in 16-byte pieces: a load of the rows themselves has lanes 64 bytes
+// apart next to each other and keeps the L1 busy for each (walk of 4 prompts of up to
+// 2600 tokens: 278 us, 170 like this).  T and P: [plane][16 rows][2 blocks of 16 columns][lane]; k and q: [plane][16
+// rows][32 dims][lane].
+enum { kFa, kFb, kFc, kFbeta, kFt, kFp, kFkm, kFend, kFactors };
 constexpr int kPlane = kC * kC * 2, kOffP = 2 * kPlane, kOffF = 4 * kPlane, kRec = kOffF + kFactors * kC * 4;
+template <int DK, typename XT>
+constexpr int kRows = kC * DK * (sizeof(XT) == 2 ? 2 : 4);  // bytes of k's planes, and of q's
 
 __device__ __forceinline__ float4_t gd_mfma(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ float4_t gd_mfma(half4_t a, half4_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ half4_t gd_half(half8_t x, int h) {
+  return h ? (half4_t){x[4], x[5], x[6], x[7]} : (half4_t){x[0], x[1], x[2], x[3]};
 }
 // Over 16 columns: a holds 4 consecutive columns of the lane's A row, b the same of its B column.
 __device__ __forceinline__ float4_t gd_mfma(const float4_t& a, const float4_t& b, float4_t c) {
@@ -235,8 +245,8 @@ __device__ __forceinline__ int gd_seq_of(const int* __restrict__ q_start, int n,
   return lo;
 }
 
-// Elements d .. d + 7 of a row of dk elements as fp32 or fp16; zeros past its end and, with !live,
-// throughout (row then points at a row there is).
+// Elements d .. d + 7 of a row of dk elements as fp32 or fp16, zeros past its end.  WIDE: rows
+// of whole 16-byte pieces, d inside.
 template <typename XT>
 struct GdVec;
 template <>
@@ -247,21 +257,21 @@ template <>
 struct GdVec<float> {
   typedef float T __attribute__((ext_vector_type(8)));
 };
-template <typename XT>
-__device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, int dk, bool live, bool wide) {
+template <bool WIDE, typename XT>
+__device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, int dk) {
   typename GdVec<XT>::T x;
-  if (wide) {  // rows of whole 16-byte pieces
+  if constexpr (WIDE) {
     constexpr int P = sizeof(XT) / 2;
     union {
       int4_t i[P];
       typename GdVec<XT>::T x;
     } u;
 #pragma unroll
-    for (int p = 0; p < P; ++p) u.i[p] = live && d < dk ? *(const int4_t*)(row + d + p * 4) : (int4_t)0;
+    for (int p = 0; p < P; ++p) u.i[p] = *(const int4_t*)(row + d + p * 4);
     x = u.x;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = live && d + e < dk ? row[d + e] : (XT)0;
+    for (int e = 0; e < 8; ++e) x[e] = d + e < dk ? row[d + e] : (XT)0;
   }
   return x;
 }
@@ -272,12 +282,12 @@ __device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, 
 // 16 x 16 blocks on the diagonal by substitution, a column per lane; then pairs, T_10 = -T_11 A_10
 // T_00, twice.  A product's result has the layout of the next one's right operand, so
 // only T's pieces go through LDS.
-template <int DK, typename XT>
-__global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws, int from, int wide) {
+template <int DK, bool FULL, typename XT>
+__global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws, char* __restrict__ rows_ws, int from) {
   constexpr int W = kC + 4;
   __shared__ float sa[kC * W], st[kC * W], sp[kC * W];
   __shared__ double sg[kC];
-  __shared__ float sk2[kC], sq2[kC], skm[kC], sqm[kC], sbeta[kC], sbad[kC];
+  __shared__ float sk2[kC], sq2[kC], skm[kC], ski[kC], sqi[kC], sbeta[kC], sbad[kC];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
   const int id = blockIdx.x, hk = blockIdx.y;
   const int seq = gd_seq_of(a.q_start, a.n_seqs, id);
@@ -289,49 +299,78 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
   auto row = [&](const void* x, long ld, int t) {
     return (const XT*)x + (long)(t0 + c0 + min(t, live - 1)) * ld + (long)hk * a.dk;
   };
+  constexpr int M = DK / 32;
   float4_t kk[4] = {}, qk[4] = {};
-  float k2 = 0.f, q2 = 0.f, km = 0.f, qm = 0.f;
   {
     const int t = 16 * w + j;
     const XT *kr = row(a.k, a.ldk, t), *qr = row(a.q, a.ldq, t);
-    for (int m = 0; m < DK / 32; ++m) {
-      const int d = 32 * m + 8 * q;
-      const auto kf = gd_load8<XT>(kr, d, a.dk, t < live, wide);
-      const auto qf = gd_load8<XT>(qr, d, a.dk, t < live, wide);
+    float k2 = 0.f, q2 = 0.f, km = 0.f, qm = 0.f;
+    typename GdVec<XT>::T kf[M], qf[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      kf[m] = gd_load8<FULL, XT>(kr, 32 * m + 8 * q, a.dk);
+      qf[m] = gd_load8<FULL, XT>(qr, 32 * m + 8 * q, a.dk);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (b > w) continue;
+      const XT* br = row(a.k, a.ldk, 16 * b + j);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const auto bf = gd_load8<FULL, XT>(br, 32 * m + 8 * q, a.dk);
+        if constexpr (sizeof(XT) == 2) {
+          kk[b] = gd_mfma(kf[m], bf, kk[b]);
+          qk[b] = gd_mfma(qf[m], bf, qk[b]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4_t x = {bf[e], bf[e + 1], bf[e + 2], bf[e + 3]};
+            kk[b] = gd_mfma((float4_t){kf[m][e], kf[m][e + 1], kf[m][e + 2], kf[m][e + 3]}, x, kk[b]);
+            qk[b] = gd_mfma((float4_t){qf[m][e], qf[m][e + 1], qf[m][e + 2], qf[m][e + 3]}, x, qk[b]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = (float)kf[e], y = (float)qf[e];
+        const float x = (float)kf[m][e], y = (float)qf[m][e];
         k2 += x * x;
         q2 += y * y;
         km = fmaxf(km, fabsf(x));
         qm = fmaxf(qm, fabsf(y));
       }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b > w) continue;
-        const auto bf = gd_load8<XT>(row(a.k, a.ldk, 16 * b + j), d, a.dk, 16 * b + j < live, wide);
-        if constexpr (sizeof(XT) == 2) {
-          kk[b] = gd_mfma(kf, bf, kk[b]);
-          qk[b] = gd_mfma(qf, bf, qk[b]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const float4_t x = {bf[e], bf[e + 1], bf[e + 2], bf[e + 3]};
-            kk[b] = gd_mfma((float4_t){kf[e], kf[e + 1], kf[e + 2], kf[e + 3]}, x, kk[b]);
-            qk[b] = gd_mfma((float4_t){qf[e], qf[e + 1], qf[e + 2], qf[e + 3]}, x, qk[b]);
-          }
-        }
-      }
-    }
     k2 = gd_sum16(k2);
     q2 = gd_sum16(q2);
     km = gd_max16(km);
     qm = gd_max16(qm);
+    float ki = 1.f, qi = 1.f;
+    char* to = rows_ws + ((long)id * a.nk + hk) * (2 * kRows<DK, XT>) + (w * M * 64 + lane) * 16;
+    if constexpr (sizeof(XT) == 2) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        *(half8_t*)(to + m * 1024) = kf[m];
+        *(half8_t*)(to + kRows<DK, XT> + m * 1024) = qf[m];
+      }
+    } else {
+      const float ks = gd_scale(km, ki), qs = gd_scale(qm, qi);
+      km *= ks;
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        half8_t x[4];
+        gd_split<8>((const float*)&kf[m], ks, (half_t*)&x[0], (half_t*)&x[1]);
+        gd_split<8>((const float*)&qf[m], qs, (half_t*)&x[2], (half_t*)&x[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(half8_t*)(to + i * (kRows<DK, XT> / 2) + m * 1024) = x[i];
+      }
+    }
     if (q == 0) {
       sk2[t] = a.norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.f;
       sq2[t] = (a.norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.f) * a.scale;
       skm[t] = km;
-      sqm[t] = qm;
+      ski[t] = ki;
+      sqi[t] = qi;
     }
   }
   for (int r = 0; r < a.rep; ++r) {
@@ -439,33 +478,26 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
       if (part <= t >> 4) {
         union {
           half_t h[2][16];
-          int4_t v[2][2];
+          half4_t v[2][4];
         } u;
         gd_split<16>(y, s, u.h[0], u.h[1]);
-        char* to = rec + i * kOffP + t * (kC * 2) + part * 32;
+        // columns 16 part + 4 c of row t: lane 16 c + t % 16, the half of its piece that part says
+        char* to = rec + i * kOffP + ((t >> 4) * 2 + (part >> 1)) * 1024 + (t & 15) * 16 + (part & 1) * 8;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          *(int4_t*)(to + p * kPlane) = u.v[p][0];
-          *(int4_t*)(to + p * kPlane + 16) = u.v[p][1];
-        }
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) *(half4_t*)(to + p * kPlane + c * 256) = u.v[p][c];
       }
       if (part == 0) f[(i ? kFp : kFt) * kC + t] = inv;
     }
     if (tid < kC) {
       const double G = sg[tid], end = sg[kC - 1];
-      float ki = 1.f, qi = 1.f, ks = 1.f, qs = 1.f;
-      if constexpr (sizeof(XT) == 4) {
-        ks = gd_scale(skm[tid], ki);
-        qs = gd_scale(sqm[tid], qi);
-      }
       const float eg = expf((float)G);
-      f[kFa * kC + tid] = sbad[tid] != 0.f ? __builtin_nanf("") : eg * sk2[tid] * ki;
-      f[kFb * kC + tid] = eg * sq2[tid] * qi;
-      f[kFc * kC + tid] = expf((float)(end - G)) * sk2[tid] * ki;
+      f[kFa * kC + tid] = sbad[tid] != 0.f ? __builtin_nanf("") : eg * sk2[tid] * ski[tid];
+      f[kFb * kC + tid] = eg * sq2[tid] * sqi[tid];
+      f[kFc * kC + tid] = expf((float)(end - G)) * sk2[tid] * ski[tid];
       f[kFbeta * kC + tid] = sbeta[tid];
-      f[kFkm * kC + tid] = skm[tid] * ks;
-      f[kFsk * kC + tid] = ks;
-      f[kFsq * kC + tid] = qs;
+      f[kFkm * kC + tid] = skm[tid];
       f[kFend * kC + tid] = expf((float)end);
     }
   }
@@ -483,8 +515,8 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
 // above T's diagonal: it is taken out, and u, o and S from that row on are NaN, as token by
 // token.
 template <int DK, int NT, typename XT>
-__global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __restrict__ ws, int from, int wide,
-                                                      int groups) {
+__global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __restrict__ ws,
+                                                      const char* __restrict__ rows_ws, int from, int groups) {
   constexpr int SL = DK / 64, NP = sizeof(XT) == 2 ? 1 : 2, NC = 16 * NT;
   constexpr int M = DK / 32;
   __shared__ __align__(16) half_t ss[2][NC * DK];        // the state [column][row]
@@ -515,10 +547,9 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   const char* rec = ws + ((long)gd_base(a.q_start, seq) * a.nv + h) * kRec;
   const bool cl = v0 + col < a.dv;
   const long head = (long)a.dk * a.dv;
-  const XT* kp = (const XT*)a.k + (long)t0 * a.ldk + (long)hk * a.dk;
-  const XT* qp = (const XT*)a.q + (long)t0 * a.ldq + (long)hk * a.dk;
-  const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + v0 + col;
-  XT* op = (XT*)a.o + (long)t0 * a.ldo + (long)h * a.dv + v0 + col;
+  const char* kq = rows_ws + ((long)gd_base(a.q_start, seq) * a.nk + hk) * (2 * kRows<DK, XT>) + (rt * M * 64 + lane) * 16;
+  const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + (cl ? v0 + col : 0);
+  XT* op = (XT*)a.o + (long)t0 * a.ldo + (long)h * a.dv + v0;
 
   float4_t s[SL];
 #pragma unroll
@@ -532,35 +563,33 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
     }
 
   // What a chunk reads, a chunk ahead: in registers until the products before it are done.
-  typename GdVec<XT>::T kf[M], qf[M];
-  half4_t tf[2][4], pf[2][4];
+  half8_t kf[NP][M], qf[NP][M], tf[2][2], pf[2][2];
   XT vf[4];
   float4 ff;
   const int chunks = (n + kC - 1) / kC;
+  // Rows past the end are the last one's again (here and in k_gd_prep): their beta is 0, and where
+  // that row is finite so are x = 0 and all that follows of it.
   auto load_rows = [&](int c) {
-    const int t = c * kC + 16 * rt + j;
-    const XT *kr = kp + (long)min(t, n - 1) * a.ldk, *qr = qp + (long)min(t, n - 1) * a.ldq;
+    const char* p = kq + (long)c * a.nk * (2 * kRows<DK, XT>);
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      kf[m] = gd_load8<XT>(kr, 32 * m + 8 * q, a.dk, t < n, wide);
-      qf[m] = gd_load8<XT>(qr, 32 * m + 8 * q, a.dk, t < n, wide);
-    }
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int tv = c * kC + 16 * rt + 4 * q + e;
-      vf[e] = tv < n && cl ? vp[(long)tv * a.ldv] : (XT)0;
-    }
+      for (int m = 0; m < M; ++m) {
+        kf[i][m] = *(const half8_t*)(p + i * (kC * DK * 2) + m * 1024);
+        qf[i][m] = *(const half8_t*)(p + kRows<DK, XT> + i * (kC * DK * 2) + m * 1024);
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vf[e] = vp[(long)min(c * kC + 16 * rt + 4 * q + e, n - 1) * a.ldv];
   };
-  auto load_tri = [&](int c, int off, half4_t (&x)[2][4]) {
-    const char* p = rec + (long)c * a.nv * kRec + off + (16 * rt + j) * (kC * 2) + 8 * q;
+  auto load_tri = [&](int c, int off, half8_t (&x)[2][2]) {
+    const char* p = rec + (long)c * a.nv * kRec + off + rt * 2048 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        x[i][b] = b <= rt ? *(const half4_t*)(p + i * kPlane + 32 * b) : (half4_t)(half_t)0;
+      for (int b = 0; b < 2; ++b) x[i][b] = *(const half8_t*)(p + i * kPlane + 1024 * min(b, rt >> 1));
   };
   auto load_factors = [&](int c) {
-    if (tid < kFactors * kC / 4) ff = *(const float4*)(rec + (long)c * a.nv * kRec + kOffF + 16 * tid);
+    ff = *(const float4*)(rec + (long)c * a.nv * kRec + kOffF + 16 * min(tid, kFactors * kC / 4 - 1));
   };
   auto factor = [&](const float* f, int k) { return *(const float4_t*)(f + k * kC + 16 * rt + 4 * q); };
   // [column][token] tiles: 8-byte pieces, swizzled by the column
@@ -575,15 +604,15 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
     if (q == 0) inv[rt][col] = iv;
   };
   // sum over the token blocks up to rt of x (row planes) times what put() left
-  auto tri = [&](const half4_t (&x)[2][4], const half_t (&y)[2][NC * kC], const float (&inv)[4][NC]) {
+  auto tri = [&](const half8_t (&x)[2][2], const half_t (&y)[2][NC * kC], const float (&inv)[4][NC]) {
     float4_t z = (float4_t)0.f;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       if (b > rt) continue;
       const half4_t hi = *(const half4_t*)&y[0][piece(b)], lo = *(const half4_t*)&y[1][piece(b)];
-      float4_t c = gd_mfma(x[1][b], hi, (float4_t)0.f);
-      c = gd_mfma(x[0][b], lo, c);
-      c = gd_mfma(x[0][b], hi, c);
+      float4_t c = gd_mfma(gd_half(x[1][b >> 1], b & 1), hi, (float4_t)0.f);
+      c = gd_mfma(gd_half(x[0][b >> 1], b & 1), lo, c);
+      c = gd_mfma(gd_half(x[0][b >> 1], b & 1), hi, c);
       z += c * inv[b][col];
     }
     return z;
@@ -626,29 +655,22 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
     float4_t o = (float4_t)0.f;
     {  // k^T S, q^T S
       float4_t x = (float4_t)0.f;
-      const float ks = NP == 2 ? f[kFsk * kC + 16 * rt + j] : 1.f, qs = NP == 2 ? f[kFsq * kC + 16 * rt + j] : 1.f;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const int at = col * DK + (((4 * m + q) ^ (j & 7)) << 3);
         const half8_t hi = *(const half8_t*)&ss[0][at], lo = *(const half8_t*)&ss[1][at];
-        half8_t kh, kl, qh, ql;
-        if constexpr (NP == 1) {
-          kh = kf[m];
-          qh = qf[m];
-        } else {
-          gd_split<8>((const float*)&kf[m], ks, (half_t*)&kh, (half_t*)&kl);
-          gd_split<8>((const float*)&qf[m], qs, (half_t*)&qh, (half_t*)&ql);
-          x = gd_mfma(kl, hi, x);
-          o = gd_mfma(ql, hi, o);
+        if constexpr (NP == 2) {
+          x = gd_mfma(kf[NP - 1][m], hi, x);
+          o = gd_mfma(qf[NP - 1][m], hi, o);
         }
-        x = gd_mfma(kh, lo, x);
-        o = gd_mfma(qh, lo, o);
-        x = gd_mfma(kh, hi, x);
-        o = gd_mfma(qh, hi, o);
+        x = gd_mfma(kf[0][m], lo, x);
+        o = gd_mfma(qf[0][m], lo, o);
+        x = gd_mfma(kf[0][m], hi, x);
+        o = gd_mfma(qf[0][m], hi, o);
         if (nt == 0) {
           const int t = 16 * rt + j, sw = 2 * (t & 3) + ((t >> 2) & 1);
-          *(half8_t*)&skey[0][t * DK + (((4 * m + q) ^ sw) << 3)] = kh;
-          if constexpr (NP == 2) *(half8_t*)&skey[1][t * DK + (((4 * m + q) ^ sw) << 3)] = kl;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) *(half8_t*)&skey[i][t * DK + (((4 * m + q) ^ sw) << 3)] = kf[i][m];
         }
       }
       const float4_t fa = factor(f, kFa), fb = factor(f, kFbeta);
@@ -663,11 +685,9 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       o = o * sinv * factor(f, kFb);
       put(sx, x, sxi);
     }
-    const bool more = c + 1 < chunks;
-    if (more) {
-      load_rows(c + 1);
-      load_factors(c + 1);
-    }
+    const int next = min(c + 1, chunks - 1);  // (loads without a branch can be waited for one by one)
+    load_rows(next);
+    load_factors(next);
     __syncthreads();
     const int first = sfirst[col];
     {  // u
@@ -678,14 +698,23 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       const float m = gd_max16(gd_max4(d * km));
       if (q == 0) sinc[rt][col] = m;
     }
-    if (more) load_tri(c + 1, 0, tf);
+    load_tri(next, 0, tf);
     __syncthreads();
     o += tri(pf, su, sui) * factor(f, kFp);
-    if (more) load_tri(c + 1, kOffP, pf);
+    load_tri(next, kOffP, pf);
+    // A store past the descriptor's end (a row or column there is not) is dropped: no branch.
+    const mx_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+        op + (long)c * kC * a.ldo, (short)0,
+        (int)(((min(n - c * kC, kC) - 1) * a.ldo + min(NC, a.dv - v0)) * (long)sizeof(XT)), 0x00020000);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int t = 16 * rt + 4 * q + e;
-      if (cl && c * kC + t < n) op[(long)(c * kC + t) * a.ldo] = (XT)(t < first ? o[e] : __builtin_nanf(""));
+      const XT y = (XT)(t < first ? o[e] : __builtin_nanf(""));
+      const int at = cl ? (t * (int)a.ldo + col) * (int)sizeof(XT) : -(1 << 31);
+      if constexpr (sizeof(XT) == 2)
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), to, at, 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), to, at, 0, 0);
     }
     const float end = f[kFend * kC];
 #pragma unroll
@@ -711,7 +740,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
     }
     bound = fmaxf(fmaxf(smax[c & 1][0][col], smax[c & 1][1][col]), fmaxf(smax[c & 1][2][col], smax[c & 1][3][col]));
     bound = end * bound + 64.f * fmaxf(fmaxf(sinc[0][col], sinc[1][col]), fmaxf(sinc[2][col], sinc[3][col]));
-    if (more && tid < kFactors * kC / 4) *(float4*)&sf[(c + 1) & 1][4 * tid] = ff;
+    if (tid < kFactors * kC / 4) *(float4*)&sf[(c + 1) & 1][4 * tid] = ff;
     if (tid < NC) sfirst[tid] = kC;
   }
   if (out < 0 || out >= a.n_slots || !cl) return;
@@ -787,20 +816,29 @@ int launch_recurrent(const GdArgs& a, int below, hipStream_t s) {
 constexpr int kFrom = 24;  // rows from which a sequence goes chunk by chunk
 
 bool chunked(const MxGatedDelta* d) {
-  return d->head_dim_k <= 128 && (d->max_q < d->rows ? d->max_q : d->rows) >= kFrom;
+  // (o's chunks are written through a descriptor of 2^31 bytes)
+  return d->head_dim_k <= 128 && d->ldo < (1 << 23) && (d->max_q < d->rows ? d->max_q : d->rows) >= kFrom;
 }
 
-template <int DK, typename XT>
+template <int DK, bool FULL, typename XT>
 int launch_chunked(const GdArgs& a, char* ws, hipStream_t s) {
   constexpr int NT = 1;
-  const int esz = sizeof(XT);
-  const int wide = a.dk % 8 == 0 && mx_aligned16(a.q) && mx_aligned16(a.k) && a.ldq * esz % 16 == 0 && a.ldk * esz % 16 == 0;
+  const int slots = a.rows / kC + a.n_seqs;
+  char* rows_ws = ws + (size_t)slots * a.nv * kRec;
   mx_clear_error();
-  hipLaunchKernelGGL((k_gd_prep<DK, XT>), dim3(a.rows / kC + a.n_seqs, a.nk), dim3(256), 0, s, a, ws, kFrom, wide);
+  hipLaunchKernelGGL((k_gd_prep<DK, FULL, XT>), dim3(slots, a.nk), dim3(256), 0, s, a, ws, rows_ws, kFrom);
   MX_TRY(mx_launch_status());
-  hipLaunchKernelGGL((k_gd_walk<DK, NT, XT>), dim3(mx_ceil_div(a.dv, 16 * NT) * a.nv, a.n_seqs), dim3(256 * NT), 0, s,
-                     a, ws, kFrom, wide, a.nk % 8 == 0);
+  hipLaunchKernelGGL((k_gd_walk<DK, NT, XT>), dim3(mx_ceil_div(a.dv, 16 * NT) * a.nv, a.n_seqs), dim3(256 * NT), 0, s, a,
+                     ws, rows_ws, kFrom, a.nk % 8 == 0);
   return mx_launch_status();
+}
+
+// Rows of q and k in whole 16-byte pieces.
+template <typename XT>
+bool full(const GdArgs& a) {
+  const int esz = sizeof(XT);
+  return (a.dk == 64 || a.dk == 128) && mx_aligned16(a.q) && mx_aligned16(a.k) && a.ldq * esz % 16 == 0 &&
+         a.ldk * esz % 16 == 0;
 }
 
 template <typename XT>
@@ -808,7 +846,8 @@ int run(const MxGatedDelta* d, const GdArgs& a, char* ws, hipStream_t s) {
   const bool long_rows = chunked(d);
   MX_TRY(launch_recurrent<XT>(a, long_rows ? kFrom : 1 << 30, s));
   if (!long_rows) return MX_OK;
-  return a.dk <= 64 ? launch_chunked<64, XT>(a, ws, s) : launch_chunked<128, XT>(a, ws, s);
+  if (full<XT>(a)) return a.dk == 64 ? launch_chunked<64, true, XT>(a, ws, s) : launch_chunked<128, true, XT>(a, ws, s);
+  return a.dk <= 64 ? launch_chunked<64, false, XT>(a, ws, s) : launch_chunked<128, false, XT>(a, ws, s);
 }
 
 }  // namespace
@@ -816,7 +855,10 @@ int run(const MxGatedDelta* d, const GdArgs& a, char* ws, hipStream_t s) {
 extern "C" int mx_gated_delta_rule_workspace_size(const MxGatedDelta* args, size_t* nbytes) {
   if (!nbytes) return MX_ERR_INVALID;
   MX_TRY(check(args));
-  *nbytes = chunked(args) ? ((size_t)args->rows / kC + args->n_seqs) * args->n_v_heads * kRec : 0;
+  *nbytes = 0;
+  if (!chunked(args)) return MX_OK;
+  const size_t row = kC * (args->head_dim_k <= 64 ? 64 : 128) * (args->x_dtype == MX_DT_F16 ? 2 : 4);
+  *nbytes = ((size_t)args->rows / kC + args->n_seqs) * (args->n_v_heads * (size_t)kRec + args->n_k_heads * 2 * row);
   return MX_OK;
 }
 
