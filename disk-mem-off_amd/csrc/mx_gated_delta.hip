@@ -30,20 +30,21 @@ struct GdArgs {
 // lanes of 4 columns, 32 row groups of NR rows (row = group + 32 i).  With S' = e^g S the two
 // products that reduce over the rows are taken together, r = k^T S' and p = q^T S', and o =
 // scale (p + (q . k) u) follows without a second pass; q . k, |q|^2 and |k|^2 come out of the
-// same rows in LDS, so a token costs one exchange between the waves.
+// same rows in LDS, so a token costs one exchange between the waves.  Eight tokens' rows are
+// loaded at once (16 tokens of one sequence: 28 us one by one, 18 so).
 //
 // For decode steps bound by the state's bytes, read and written once (128 x 32 columns are 16 KiB
 // per block, 128-byte pieces of a row).
 // ------------------------------------------------------------------------------------
-constexpr int kCols = 32;
+constexpr int kCols = 32, kAhead = 8;
 
 template <int NR, typename XT>
 __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
   constexpr int DKP = 32 * NR;
-  __shared__ float sk[2][DKP], sq[2][DKP];
-  __shared__ float red[2][4][2][kCols];  // [buffer][wave][r, p][column]
+  __shared__ __align__(16) float sk[kAhead][DKP], sq[kAhead][DKP], sv[kAhead][kCols], sg[kAhead], sb[kAhead];
+  __shared__ __align__(16) float red[2][4][2][kCols];  // [buffer][wave][r, p][column]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int seq = blockIdx.z, h = blockIdx.y, c0 = blockIdx.x * kCols + 4 * (tid & 7);
+  const int seq = blockIdx.z, h = blockIdx.y, cl = 4 * (tid & 7), c0 = blockIdx.x * kCols + cl;
   const int hk = h / a.rep, grp = tid >> 3;
   const bool col = c0 < a.dv;
   const int t0 = a.q_start[seq], t1 = min(a.q_start[seq + 1], a.rows);
@@ -58,81 +59,94 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
     if (in >= 0 && in < a.n_slots && col && r < a.dk)
       s[i] = *(const float4*)(a.state + ((long)in * a.nv + h) * head + (long)r * a.dv + c0);
   }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    for (int i = tid; i < DKP; i += 256) {
-      sk[buf][i] = i < a.dk ? (float)((const XT*)a.k)[(long)t * a.ldk + (long)hk * a.dk + i] : 0.f;
-      sq[buf][i] = i < a.dk ? (float)((const XT*)a.q)[(long)t * a.ldq + (long)hk * a.dk + i] : 0.f;
+  for (int first = t0; first < t1; first += kAhead) {
+    const int some = min(kAhead, t1 - first);
+    if (first > t0) __syncthreads();  // the rows before are read
+    for (int i = tid; i < some * DKP; i += 256) {
+      const int d = i % DKP;
+      const long t = first + i / DKP;
+      sk[i / DKP][d] = d < a.dk ? (float)((const XT*)a.k)[t * a.ldk + (long)hk * a.dk + d] : 0.f;
+      sq[i / DKP][d] = d < a.dk ? (float)((const XT*)a.q)[t * a.ldq + (long)hk * a.dk + d] : 0.f;
     }
-    const float eg = expf(a.g[(long)t * a.nv + h]), beta = a.beta[(long)t * a.nv + h];
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[e] = col ? (float)((const XT*)a.v)[(long)t * a.ldv + (long)h * a.dv + c0 + e] : 0.f;
-    __syncthreads();
-    float kk = 0.f, qq = 0.f, qk = 0.f;
-#pragma unroll
-    for (int i = 0; i < (DKP + 63) / 64; ++i) {
-      const int r = lane + 64 * i;
-      const float kv = r < DKP ? sk[buf][r] : 0.f, qv = r < DKP ? sq[buf][r] : 0.f;
-      kk += kv * kv;
-      qq += qv * qv;
-      qk += qv * kv;
-    }
-    kk = mx_wave_sum(kk);
-    qq = mx_wave_sum(qq);
-    qk = mx_wave_sum(qk);
-    const float rk = a.norm ? 1.0f / sqrtf(kk + 1e-6f) : 1.f;
-    const float rq = (a.norm ? 1.0f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f), p = r;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const float kv = sk[buf][grp + 32 * i], qv = sq[buf][grp + 32 * i];
-      s[i] = make_float4(s[i].x * eg, s[i].y * eg, s[i].z * eg, s[i].w * eg);
-      r.x += kv * s[i].x;
-      r.y += kv * s[i].y;
-      r.z += kv * s[i].z;
-      r.w += kv * s[i].w;
-      p.x += qv * s[i].x;
-      p.y += qv * s[i].y;
-      p.z += qv * s[i].z;
-      p.w += qv * s[i].w;
-    }
-    float rp[8] = {r.x, r.y, r.z, r.w, p.x, p.y, p.z, p.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int o = 8; o < 64; o *= 2) rp[e] += __shfl_xor(rp[e], o);
-    if (lane < 8) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        red[buf][wave][0][4 * lane + e] = rp[e];
-        red[buf][wave][1][4 * lane + e] = rp[4 + e];
+    {
+      const int i = tid / kCols, c = blockIdx.x * kCols + tid % kCols;  // 8 x 32 threads
+      if (i < some) sv[i][tid % kCols] = c < a.dv ? (float)((const XT*)a.v)[(long)(first + i) * a.ldv + (long)h * a.dv + c] : 0.f;
+      if (tid < some) {
+        sg[tid] = expf(a.g[(long)(first + tid) * a.nv + h]);
+        sb[tid] = a.beta[(long)(first + tid) * a.nv + h];
       }
     }
     __syncthreads();
-    float u[4];
-    const int cl = 4 * (tid & 7);
+    for (int i = 0; i < some; ++i) {
+      const int buf = i & 1;
+      const float eg = sg[i], beta = sb[i];
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f), p = r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float rs = (red[buf][0][0][cl + e] + red[buf][1][0][cl + e]) +
-                       (red[buf][2][0][cl + e] + red[buf][3][0][cl + e]);
-      u[e] = beta * (v[e] - rk * rs);
-    }
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const float kv = sk[buf][grp + 32 * i] * rk;
-      s[i].x += kv * u[0];
-      s[i].y += kv * u[1];
-      s[i].z += kv * u[2];
-      s[i].w += kv * u[3];
-    }
-    if (tid < 8 && col) {
+      for (int n = 0; n < NR; ++n) {
+        const float kv = sk[i][grp + 32 * n], qv = sq[i][grp + 32 * n];
+        s[n] = make_float4(s[n].x * eg, s[n].y * eg, s[n].z * eg, s[n].w * eg);
+        r.x += kv * s[n].x;
+        r.y += kv * s[n].y;
+        r.z += kv * s[n].z;
+        r.w += kv * s[n].w;
+        p.x += qv * s[n].x;
+        p.y += qv * s[n].y;
+        p.z += qv * s[n].z;
+        p.w += qv * s[n].w;
+      }
+      // The wave's 8 row groups: halves of the lanes, then quarters, each keep half of the 8 sums.
+      float x[4] = {r.x, r.y, r.z, r.w}, y[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float ps = (red[buf][0][1][cl + e] + red[buf][1][1][cl + e]) +
-                         (red[buf][2][1][cl + e] + red[buf][3][1][cl + e]);
-        ((XT*)a.o)[(long)t * a.ldo + (long)h * a.dv + c0 + e] = (XT)(rq * (ps + qk * rk * u[e]));
+        pk_swap32(x[e], y[e]);
+        x[e] += y[e];  // r in the lower half of the lanes, p in the upper
+      }
+      pk_swap16(x[0], x[2]);
+      pk_swap16(x[1], x[3]);
+      float2 z = make_float2(x[0] + x[2], x[1] + x[3]);  // columns 0, 1 in the even rows, 2, 3 in the odd
+      z.x += mx_dpp<0x128>(z.x);  // row_ror:8
+      z.y += mx_dpp<0x128>(z.y);
+      if ((lane & 8) == 0) *(float2*)&red[buf][wave][lane >> 5][cl + 2 * ((lane >> 4) & 1)] = z;
+      float kk = 0.f, qq = 0.f, qk = 0.f;
+#pragma unroll
+      for (int n = 0; n < (DKP + 63) / 64; ++n) {
+        const int d = lane + 64 * n;
+        const float kv = d < DKP ? sk[i][d] : 0.f, qv = d < DKP ? sq[i][d] : 0.f;
+        kk += kv * kv;
+        qq += qv * qv;
+        qk += qv * kv;
+      }
+      kk = mx_wave_sum(kk);
+      qq = mx_wave_sum(qq);
+      qk = mx_wave_sum(qk);
+      const float rk = a.norm ? 1.0f / sqrtf(kk + 1e-6f) : 1.f;
+      const float rq = (a.norm ? 1.0f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
+      __syncthreads();
+      auto sum = [&](int w) {
+        const float4 x0 = *(const float4*)&red[buf][0][w][cl], x1 = *(const float4*)&red[buf][1][w][cl];
+        const float4 x2 = *(const float4*)&red[buf][2][w][cl], x3 = *(const float4*)&red[buf][3][w][cl];
+        return make_float4((x0.x + x1.x) + (x2.x + x3.x), (x0.y + x1.y) + (x2.y + x3.y), (x0.z + x1.z) + (x2.z + x3.z),
+                           (x0.w + x1.w) + (x2.w + x3.w));
+      };
+      const float4 rs = sum(0), v = *(const float4*)&sv[i][cl];
+      const float4 u = make_float4(beta * (v.x - rk * rs.x), beta * (v.y - rk * rs.y), beta * (v.z - rk * rs.z),
+                                   beta * (v.w - rk * rs.w));
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float kv = sk[i][grp + 32 * n] * rk;
+        s[n].x += kv * u.x;
+        s[n].y += kv * u.y;
+        s[n].z += kv * u.z;
+        s[n].w += kv * u.w;
+      }
+      if (tid < 8 && col) {
+        const float4 ps = sum(1);
+        const float f = qk * rk;
+        XT* o = (XT*)a.o + (long)(first + i) * a.ldo + (long)h * a.dv + c0;
+        o[0] = (XT)(rq * (ps.x + f * u.x));
+        o[1] = (XT)(rq * (ps.y + f * u.y));
+        o[2] = (XT)(rq * (ps.z + f * u.z));
+        o[3] = (XT)(rq * (ps.w + f * u.w));
       }
     }
   }
@@ -217,11 +231,7 @@ __device__ __forceinline__ void gd_split(const float* x, float s, half_t* hi, ha
 __device__ __forceinline__ float gd_max4(const float4_t& x) {
   return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 }
-// Max and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float gd_max16(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
+// Sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float gd_sum16(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
@@ -343,8 +353,8 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
       }
     k2 = gd_sum16(k2);
     q2 = gd_sum16(q2);
-    km = gd_max16(km);
-    qm = gd_max16(qm);
+    km = pk_rowmax(km);
+    qm = pk_rowmax(qm);
     float ki = 1.f, qi = 1.f;
     char* to = rows_ws + ((long)id * a.nk + hk) * (2 * kRows<DK, XT>) + (w * M * 64 + lane) * 16;
     if constexpr (sizeof(XT) == 2) {
@@ -596,7 +606,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   auto piece = [&](int b) { return col * kC + ((4 * b + q) ^ j) * 4; };
   auto put = [&](half_t (&to)[2][NC * kC], const float4_t& x, float (&inv)[4][NC]) {
     float iv;
-    const float sc = gd_scale(gd_max16(gd_max4(x)), iv);
+    const float sc = gd_scale(pk_rowmax(gd_max4(x)), iv);
     half4_t p[2];
     gd_split<4>((const float*)&x, sc, (half_t*)&p[0], (half_t*)&p[1]);
     *(half4_t*)&to[0][piece(rt)] = p[0];
@@ -625,7 +635,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   float bound = 0.f;
 #pragma unroll
   for (int i = 0; i < SL; ++i) bound = fmaxf(bound, gd_max4(s[i]));
-  bound = gd_max16(bound);
+  bound = pk_rowmax(bound);
   if (q == 0) smax[1][rt][col] = bound;
   if (tid < NC) sfirst[tid] = kC;
   if (tid < kFactors * kC / 4) *(float4*)&sf[0][4 * tid] = ff;
@@ -648,7 +658,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
         *(half4_t*)&ss[1][at] = p[1];
         m = fmaxf(m, gd_max4(s[i]));
       }
-      m = gd_max16(m);
+      m = pk_rowmax(m);
       if (q == 0) smax[c & 1][rt][col] = m;
     }
     __syncthreads();
@@ -695,7 +705,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       const float4_t d = u * factor(f, kFc), km = factor(f, kFkm);
       put(su, u, sui);
       put(sd, d, sdi);
-      const float m = gd_max16(gd_max4(d * km));
+      const float m = pk_rowmax(gd_max4(d * km));
       if (q == 0) sinc[rt][col] = m;
     }
     load_tri(next, 0, tf);

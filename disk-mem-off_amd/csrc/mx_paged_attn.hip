@@ -275,25 +275,7 @@ __device__ __forceinline__ pa_rsrc_t pa_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
 }
 
-// Both operands of a lane swap: v_permlane16_swap exchanges the odd 16-lane rows of x with
-// the even ones of y, v_permlane32_swap the upper half of x with the lower half of y.  With x = y
-// = v the two hold v of the lane and of its partner.  (The compiler's builtins return x alone:
-// a maximum over both results of one is folded away.)  s_nop: the swap's operands were just
-// written.
-__device__ __forceinline__ void pa_swap16(float& x, float& y) {
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-}
-__device__ __forceinline__ void pa_swap32(float& x, float& y) {
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-}
-// Max and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float pa_rowmax(float v) {
-  float x = v, y = v;
-  pa_swap16(x, y);
-  x = y = fmaxf(x, y);
-  pa_swap32(x, y);
-  return fmaxf(x, y);
-}
+// Sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float pa_rowsum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
@@ -486,7 +468,7 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
   }
   float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                    fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-  mt = pa_rowmax(mt);
+  mt = pk_rowmax(mt);
   const bool up = mt > mrun + kTau;
   if (__builtin_amdgcn_ballot_w64(up)) {
     const float mnew = up ? mt : mrun;
@@ -1249,7 +1231,7 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
       for (int r = 0; r < 4; ++r)
         if (4 * g + r > lim || !on) s[r] = -INFINITY;
     }
-    const float mt = pa_rowmax(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float mt = pk_rowmax(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
     const bool up = mt > mrun + kTau;
     if (__builtin_amdgcn_ballot_w64(up)) {
       const float mnew = up ? mt : mrun;
