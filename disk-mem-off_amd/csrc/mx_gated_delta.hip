@@ -38,13 +38,22 @@ struct GdArgs {
 // ------------------------------------------------------------------------------------
 constexpr int kCols = 32, kAhead = 8;
 
+template <int NR>
+struct GdRecLds {
+  static constexpr int DKP = 32 * NR;
+  float k[kAhead][DKP], q[kAhead][DKP], v[kAhead][kCols], g[kAhead], beta[kAhead];
+  float red[2][4][2][kCols];  // [buffer][wave][r, p][column]
+};
+
 template <int NR, typename XT>
-__global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
+__device__ void gd_recurrent(const GdArgs& a, GdRecLds<NR>& lds, int piece, int h, int seq, int below) {
   constexpr int DKP = 32 * NR;
-  __shared__ __align__(16) float sk[kAhead][DKP], sq[kAhead][DKP], sv[kAhead][kCols], sg[kAhead], sb[kAhead];
-  __shared__ __align__(16) float red[2][4][2][kCols];  // [buffer][wave][r, p][column]
+  auto &sk = lds.k, &sq = lds.q;
+  auto& sv = lds.v;
+  auto &sg = lds.g, &sb = lds.beta;
+  auto& red = lds.red;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int seq = blockIdx.z, h = blockIdx.y, cl = 4 * (tid & 7), c0 = blockIdx.x * kCols + cl;
+  const int cl = 4 * (tid & 7), c0 = piece * kCols + cl;
   const int hk = h / a.rep, grp = tid >> 3;
   const bool col = c0 < a.dv;
   const int t0 = a.q_start[seq], t1 = min(a.q_start[seq + 1], a.rows);
@@ -69,7 +78,7 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
       sq[i / DKP][d] = d < a.dk ? (float)((const XT*)a.q)[t * a.ldq + (long)hk * a.dk + d] : 0.f;
     }
     {
-      const int i = tid / kCols, c = blockIdx.x * kCols + tid % kCols;  // 8 x 32 threads
+      const int i = tid / kCols, c = piece * kCols + tid % kCols;  // 8 x 32 threads
       if (i < some) sv[i][tid % kCols] = c < a.dv ? (float)((const XT*)a.v)[(long)(first + i) * a.ldv + (long)h * a.dv + c] : 0.f;
       if (tid < some) {
         sg[tid] = expf(a.g[(long)(first + tid) * a.nv + h]);
@@ -156,6 +165,12 @@ __global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a, int below) {
     const int r = grp + 32 * i;
     if (r < a.dk) *(float4*)(a.state + ((long)out * a.nv + h) * head + (long)r * a.dv + c0) = s[i];
   }
+}
+
+template <int NR, typename XT>
+__global__ __launch_bounds__(256) void k_gd_recurrent(GdArgs a) {
+  __shared__ __align__(16) GdRecLds<NR> lds;
+  gd_recurrent<NR, XT>(a, lds, blockIdx.x, blockIdx.y, blockIdx.z, 1 << 30);
 }
 
 // ------------------------------------------------------------------------------------
@@ -286,20 +301,39 @@ __device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, 
   return x;
 }
 
-// T and P of the chunks.  A block: one chunk of one key head, and its value heads in turn; wave w
-// forms the rows 16 w .. of k k^T and q k^T (fp16 rows: exact products; fp32 rows: fp32 matrix
-// instructions), operands straight from memory, as both are rows of k and q.  T: the
-// 16 x 16 blocks on the diagonal by substitution, a column per lane; then pairs, T_10 = -T_11 A_10
-// T_00, twice.  A product's result has the layout of the next one's right operand, so
-// only T's pieces go through LDS.
+// T and P of the chunks, and the sequences that are too short for chunks (token by token, by the
+// first blocks: a launch of their own would take its time next to the others').  A block: one chunk of one value
+// head; wave w forms the rows 16 w .. of k k^T and q k^T (fp16 rows: exact products; fp32 rows: fp32
+// matrix instructions), operands straight from memory, as both are rows of k and q.  T: the 16 x 16
+// blocks on the diagonal by substitution, a column per lane; then pairs, T_10 = -T_11 A_10 T_00,
+// twice.  A product's result has the layout of the next one's right operand, so only T's
+// pieces go through LDS.  A chain of short steps, each waiting for the one before: bound by how many
+// blocks a CU holds.
+struct GdPrepLds {
+  static constexpr int W = kC + 4;
+  float a[kC * W], t[kC * W];
+  double g[kC];
+  float k2[kC], q2[kC], km[kC], ki[kC], qi[kC], beta[kC], bad[kC];
+};
+
 template <int DK, bool FULL, typename XT>
-__global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws, char* __restrict__ rows_ws, int from) {
-  constexpr int W = kC + 4;
-  __shared__ float sa[kC * W], st[kC * W], sp[kC * W];
-  __shared__ double sg[kC];
-  __shared__ float sk2[kC], sq2[kC], skm[kC], ski[kC], sqi[kC], sbeta[kC], sbad[kC];
+__global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_prep(GdArgs a, char* __restrict__ ws,
+                                                                         char* __restrict__ rows_ws, int from, int pieces,
+                                                                         int slots) {
+  constexpr int W = GdPrepLds::W, M = DK / 32;
+  __shared__ __align__(16) union Lds {
+    GdPrepLds p;
+    GdRecLds<DK / 32> r;
+  } lds;
+  const long block = (long)blockIdx.y * gridDim.x + blockIdx.x, short_blocks = (long)pieces * a.nv * a.n_seqs;
+  if (block < short_blocks) {
+    const int hs = (int)(block / pieces);
+    gd_recurrent<DK / 32, XT>(a, lds.r, (int)(block % pieces), hs % a.nv, hs / a.nv, from);
+    return;
+  }
+  const int h = (int)((block - short_blocks) / slots), hk = h / a.rep, id = (int)((block - short_blocks) % slots);
+  float *sa = lds.p.a, *st = lds.p.t;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-  const int id = blockIdx.x, hk = blockIdx.y;
   const int seq = gd_seq_of(a.q_start, a.n_seqs, id);
   const int t0 = max(a.q_start[seq], 0), n = min(a.q_start[seq + 1], a.rows) - t0;
   const int c0 = (id - gd_base(a.q_start, seq)) * kC;
@@ -309,17 +343,32 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
   auto row = [&](const void* x, long ld, int t) {
     return (const XT*)x + (long)(t0 + c0 + min(t, live - 1)) * ld + (long)hk * a.dk;
   };
-  constexpr int M = DK / 32;
   float4_t kk[4] = {}, qk[4] = {};
   {
+    float g = 0.f, beta = 0.f;
+    if (w == 0 && lane < live) {
+      const long at = (long)(t0 + c0 + lane) * a.nv + h;
+      g = a.g[at];
+      beta = a.beta[at];
+    }
     const int t = 16 * w + j;
     const XT *kr = row(a.k, a.ldk, t), *qr = row(a.q, a.ldq, t);
-    float k2 = 0.f, q2 = 0.f, km = 0.f, qm = 0.f;
     typename GdVec<XT>::T kf[M], qf[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       kf[m] = gd_load8<FULL, XT>(kr, 32 * m + 8 * q, a.dk);
       qf[m] = gd_load8<FULL, XT>(qr, 32 * m + 8 * q, a.dk);
+    }
+    if (w == 0) {
+      double G = g < -256.f ? -256.f : g;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const double up = __shfl_up(G, o);
+        if (lane >= o) G += up;
+      }
+      lds.p.g[lane] = G;
+      lds.p.beta[lane] = beta;
+      lds.p.bad[lane] = 0.f;
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -341,6 +390,7 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
         }
       }
     }
+    float k2 = 0.f, q2 = 0.f, km = 0.f, qm = 0.f;
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -355,161 +405,169 @@ __global__ __launch_bounds__(256) void k_gd_prep(GdArgs a, char* __restrict__ ws
     q2 = gd_sum16(q2);
     km = pk_rowmax(km);
     qm = pk_rowmax(qm);
-    float ki = 1.f, qi = 1.f;
-    char* to = rows_ws + ((long)id * a.nk + hk) * (2 * kRows<DK, XT>) + (w * M * 64 + lane) * 16;
-    if constexpr (sizeof(XT) == 2) {
-#pragma unroll
-      for (int m = 0; m < M; ++m) {
-        *(half8_t*)(to + m * 1024) = kf[m];
-        *(half8_t*)(to + kRows<DK, XT> + m * 1024) = qf[m];
-      }
-    } else {
-      const float ks = gd_scale(km, ki), qs = gd_scale(qm, qi);
+    float ki = 1.f, qi = 1.f, ks = 1.f, qs = 1.f;
+    if constexpr (sizeof(XT) == 4) {
+      ks = gd_scale(km, ki);
+      qs = gd_scale(qm, qi);
       km *= ks;
+    }
+    if (h == hk * a.rep) {  // k and q for all value heads of theirs
+      char* to = rows_ws + ((long)id * a.nk + hk) * (2 * kRows<DK, XT>) + (w * M * 64 + lane) * 16;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        half8_t x[4];
-        gd_split<8>((const float*)&kf[m], ks, (half_t*)&x[0], (half_t*)&x[1]);
-        gd_split<8>((const float*)&qf[m], qs, (half_t*)&x[2], (half_t*)&x[3]);
+        if constexpr (sizeof(XT) == 2) {
+          *(half8_t*)(to + m * 1024) = kf[m];
+          *(half8_t*)(to + kRows<DK, XT> + m * 1024) = qf[m];
+        } else {
+          half8_t x[4];
+          gd_split<8>((const float*)&kf[m], ks, (half_t*)&x[0], (half_t*)&x[1]);
+          gd_split<8>((const float*)&qf[m], qs, (half_t*)&x[2], (half_t*)&x[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *(half8_t*)(to + i * (kRows<DK, XT> / 2) + m * 1024) = x[i];
+          for (int i = 0; i < 4; ++i) *(half8_t*)(to + i * (kRows<DK, XT> / 2) + m * 1024) = x[i];
+        }
       }
     }
     if (q == 0) {
-      sk2[t] = a.norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.f;
-      sq2[t] = (a.norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.f) * a.scale;
-      skm[t] = km;
-      ski[t] = ki;
-      sqi[t] = qi;
+      lds.p.k2[t] = a.norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.f;
+      lds.p.q2[t] = (a.norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.f) * a.scale;
+      lds.p.km[t] = km;
+      lds.p.ki[t] = ki;
+      lds.p.qi[t] = qi;
     }
   }
-  for (int r = 0; r < a.rep; ++r) {
-    const int h = hk * a.rep + r;
-    char* rec = ws + ((long)id * a.nv + h) * kRec;
-    float* f = (float*)(rec + kOffF);
-    __syncthreads();  // the buffers are free; the norms are there
-    if (w == 0) {
-      const int t = lane;
-      const long at = (long)(t0 + c0 + min(t, live - 1)) * a.nv + h;
-      float g = t < live ? a.g[at] : 0.f;
-      g = g < -256.f ? -256.f : g;
-      sbeta[t] = t < live ? a.beta[at] : 0.f;
-      double G = g;
+  __syncthreads();
+  {
+    float4_t ft, fq;  // beta |k|^-1 and scale |q|^-1 of the rows
+    double gt[4];
+    bool bad[4] = {};
 #pragma unroll
-      for (int o = 1; o < 64; o *= 2) {
-        const double up = __shfl_up(G, o);
-        if (t >= o) G += up;
-      }
-      sg[t] = G;
-      sbad[t] = 0.f;
+    for (int e = 0; e < 4; ++e) {
+      const int t = 16 * w + 4 * q + e;
+      gt[e] = lds.p.g[t];
+      ft[e] = lds.p.beta[t] * lds.p.k2[t];
+      fq[e] = lds.p.q2[t];
     }
-    __syncthreads();
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       if (b > w) continue;
       const int s = 16 * b + j;
-      const double gs = sg[s];
-      const float ks = sk2[s];
+      const double gs = lds.p.g[s];
+      const float ks = lds.p.k2[s];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int t = 16 * w + 4 * q + e;
-        const float decay = expf((float)(sg[t] - gs)) * ks;
-        float x = s < t ? sbeta[t] * sk2[t] * decay * kk[b][e] : 0.f;
+        const float decay = expf((float)(gt[e] - gs)) * ks;
+        float x = s < t ? ft[e] * decay * kk[b][e] : 0.f;
         // A row that is not finite (a NaN key, gate or decay) leaves T to the rows before it.
-        if (!(fabsf(x) <= 3.0e38f)) {
-          sbad[t] = 1.f;
-          x = 0.f;
-        }
-        sa[t * W + s] = x;
-        sp[t * W + s] = s <= t ? sq2[t] * decay * qk[b][e] : 0.f;
+        const bool inf = !(fabsf(x) <= 3.0e38f);
+        bad[e] |= inf;
+        sa[t * W + s] = inf ? 0.f : x;
+        qk[b][e] = s <= t ? fq[e] * decay * qk[b][e] : 0.f;  // P
       }
     }
-    {  // the diagonal block's inverse: column j, of this wave's own rows
-      const float* d = sa + (16 * w) * W + 16 * w;
-      float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float y = i == j ? 1.f : 0.f;
+    for (int e = 0; e < 4; ++e)
+      if (bad[e]) lds.p.bad[16 * w + 4 * q + e] = 1.f;
+  }
+  {  // the diagonal block's inverse: column j, of this wave's own rows
+    const float* d = sa + (16 * w) * W + 16 * w;
+    float x[16];
 #pragma unroll
-        for (int m = 0; m < i; m += 4) {
-          const float4_t c = *(const float4_t*)(d + i * W + m);
+    for (int i = 0; i < 16; ++i) {
+      float y[4] = {i == j ? 1.f : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (m + e < i) y -= c[e] * x[m + e];
-        }
-        x[i] = y;
+      for (int m = 0; m < i; m += 4) {
+        const float4_t c = *(const float4_t*)(d + i * W + m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (m + e < i) y[e] -= c[e] * x[m + e];
       }
-      if (q == 0)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[(16 * w + i) * W + 16 * w + j] = x[i];
+      x[i] = (y[0] + y[1]) + (y[2] + y[3]);
     }
-    __syncthreads();
-    auto rows = [&](const float* x, int I, int J) { return *(const float4_t*)(x + (16 * I + j) * W + 16 * J + 4 * q); };
-    auto cols = [&](const float* x, int I, int J) {
-      const float* p = x + (16 * I + 4 * q) * W + 16 * J + j;
-      return (float4_t){p[0], p[W], p[2 * W], p[3 * W]};
-    };
-    auto put = [&](int I, int J, const float4_t& z) {
+    if (q == 0)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st[(16 * I + 4 * q + e) * W + 16 * J + j] = -z[e];
-    };
-    if (w < 2) {
-      const int I = 2 * w + 1, J = 2 * w;
-      const float4_t y = gd_mfma(rows(sa, I, J), cols(st, J, J), (float4_t)0.f);
-      put(I, J, gd_mfma(rows(st, I, I), y, (float4_t)0.f));
+      for (int i = 0; i < 16; ++i) st[(16 * w + i) * W + 16 * w + j] = x[i];
+  }
+  __syncthreads();
+  auto rows = [&](const float* x, int I, int J) { return *(const float4_t*)(x + (16 * I + j) * W + 16 * J + 4 * q); };
+  auto cols = [&](const float* x, int I, int J) {
+    const float* p = x + (16 * I + 4 * q) * W + 16 * J + j;
+    return (float4_t){p[0], p[W], p[2 * W], p[3 * W]};
+  };
+  auto put = [&](int I, int J, const float4_t& z) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st[(16 * I + 4 * q + e) * W + 16 * J + j] = -z[e];
+  };
+  if (w < 2) {
+    const int I = 2 * w + 1, J = 2 * w;
+    const float4_t y = gd_mfma(rows(sa, I, J), cols(st, J, J), (float4_t)0.f);
+    put(I, J, gd_mfma(rows(st, I, I), y, (float4_t)0.f));
+  }
+  __syncthreads();
+  {
+    const int I = 2 + (w >> 1), J = w & 1;
+    const float4_t c1 = cols(st, 1, J);
+    float4_t y = gd_mfma(rows(sa, 2, 1), c1, (float4_t)0.f), y3 = (float4_t)0.f;
+    if (I == 3) y3 = gd_mfma(rows(sa, 3, 1), c1, y3);
+    if (J == 0) {
+      const float4_t c0 = cols(st, 0, 0);
+      y = gd_mfma(rows(sa, 2, 0), c0, y);
+      if (I == 3) y3 = gd_mfma(rows(sa, 3, 0), c0, y3);
     }
-    __syncthreads();
-    {
-      const int I = 2 + (w >> 1), J = w & 1;
-      float4_t z = (float4_t)0.f;
-      for (int K = 2; K <= I; ++K) {
-        float4_t y = (float4_t)0.f;
-        for (int L = J; L < 2; ++L) y = gd_mfma(rows(sa, K, L), cols(st, L, J), y);
-        z = gd_mfma(rows(st, I, K), y, z);
+    float4_t z = gd_mfma(rows(st, I, 2), y, (float4_t)0.f);
+    if (I == 3) z = gd_mfma(rows(st, 3, 3), y3, z);
+    put(I, J, z);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {  // A is done with
+    if (b > w) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sa[(16 * w + 4 * q + e) * W + 16 * b + j] = qk[b][e];
+  }
+  char* rec = ws + ((long)id * a.nv + h) * kRec;
+  float* f = (float*)(rec + kOffF);
+  const int t = tid >> 2, part = tid & 3;  // a row, 16 of its columns: both of this wave's own for P
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float* x = (i ? sa : st) + t * W + 16 * part;
+    float y[16], m = 0.f, inv;
+    if (part <= t >> 4) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4_t c = *(const float4_t*)(x + e);
+        m = fmaxf(m, gd_max4(c));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) y[e + d] = c[d];
       }
-      put(I, J, z);
     }
-    __syncthreads();
-    const int t = tid >> 2, part = tid & 3;  // a row, 16 of its columns
+    m = fmaxf(m, mx_dpp<MX_DPP_XOR1>(m));
+    m = fmaxf(m, mx_dpp<MX_DPP_XOR2>(m));
+    const float s = gd_scale(m, inv);
+    if (part <= t >> 4) {
+      union {
+        half_t h[2][16];
+        half4_t v[2][4];
+      } u;
+      gd_split<16>(y, s, u.h[0], u.h[1]);
+      // columns 16 part + 4 c of row t: lane 16 c + t % 16, the half of its piece that part says
+      char* to = rec + i * kOffP + ((t >> 4) * 2 + (part >> 1)) * 1024 + (t & 15) * 16 + (part & 1) * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float* x = (i ? sp : st) + t * W + 16 * part;
-      float y[16], m = 0.f, inv;
-      if (part <= t >> 4) {
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          y[e] = x[e];
-          m = fmaxf(m, fabsf(y[e]));
-        }
-      }
-      m = fmaxf(m, __shfl_xor(m, 1));
-      m = fmaxf(m, __shfl_xor(m, 2));
-      const float s = gd_scale(m, inv);
-      if (part <= t >> 4) {
-        union {
-          half_t h[2][16];
-          half4_t v[2][4];
-        } u;
-        gd_split<16>(y, s, u.h[0], u.h[1]);
-        // columns 16 part + 4 c of row t: lane 16 c + t % 16, the half of its piece that part says
-        char* to = rec + i * kOffP + ((t >> 4) * 2 + (part >> 1)) * 1024 + (t & 15) * 16 + (part & 1) * 8;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) *(half4_t*)(to + p * kPlane + c * 256) = u.v[p][c];
-      }
-      if (part == 0) f[(i ? kFp : kFt) * kC + t] = inv;
+        for (int c = 0; c < 4; ++c) *(half4_t*)(to + p * kPlane + c * 256) = u.v[p][c];
     }
-    if (tid < kC) {
-      const double G = sg[tid], end = sg[kC - 1];
-      const float eg = expf((float)G);
-      f[kFa * kC + tid] = sbad[tid] != 0.f ? __builtin_nanf("") : eg * sk2[tid] * ski[tid];
-      f[kFb * kC + tid] = eg * sq2[tid] * sqi[tid];
-      f[kFc * kC + tid] = expf((float)(end - G)) * sk2[tid] * ski[tid];
-      f[kFbeta * kC + tid] = sbeta[tid];
-      f[kFkm * kC + tid] = skm[tid];
-      f[kFend * kC + tid] = expf((float)end);
-    }
+    if (part == 0) f[(i ? kFp : kFt) * kC + t] = inv;
+  }
+  if (tid < kC) {
+    const double G = lds.p.g[tid], end = lds.p.g[kC - 1];
+    const float eg = expf((float)G), k2 = lds.p.k2[tid], ki = lds.p.ki[tid];
+    f[kFa * kC + tid] = lds.p.bad[tid] != 0.f ? __builtin_nanf("") : eg * k2 * ki;
+    f[kFb * kC + tid] = eg * lds.p.q2[tid] * lds.p.qi[tid];
+    f[kFc * kC + tid] = expf((float)(end - G)) * k2 * ki;
+    f[kFbeta * kC + tid] = lds.p.beta[tid];
+    f[kFkm * kC + tid] = lds.p.km[tid];
+    f[kFend * kC + tid] = expf((float)end);
   }
 }
 
@@ -813,13 +871,13 @@ GdArgs args_of(const MxGatedDelta* d) {
 }
 
 template <typename XT>
-int launch_recurrent(const GdArgs& a, int below, hipStream_t s) {
+int launch_recurrent(const GdArgs& a, hipStream_t s) {
   auto* kern = a.dk <= 32    ? k_gd_recurrent<1, XT>
                : a.dk <= 64  ? k_gd_recurrent<2, XT>
                : a.dk <= 128 ? k_gd_recurrent<4, XT>
                              : k_gd_recurrent<8, XT>;
   mx_clear_error();
-  hipLaunchKernelGGL(kern, dim3(mx_ceil_div(a.dv, kCols), a.nv, a.n_seqs), dim3(256), 0, s, a, below);
+  hipLaunchKernelGGL(kern, dim3(mx_ceil_div(a.dv, kCols), a.nv, a.n_seqs), dim3(256), 0, s, a);
   return mx_launch_status();
 }
 
@@ -836,7 +894,9 @@ int launch_chunked(const GdArgs& a, char* ws, hipStream_t s) {
   const int slots = a.rows / kC + a.n_seqs;
   char* rows_ws = ws + (size_t)slots * a.nv * kRec;
   mx_clear_error();
-  hipLaunchKernelGGL((k_gd_prep<DK, FULL, XT>), dim3(slots, a.nk), dim3(256), 0, s, a, ws, rows_ws, kFrom);
+  const int pieces = mx_ceil_div(a.dv, kCols);
+  hipLaunchKernelGGL((k_gd_prep<DK, FULL, XT>), dim3(pieces * a.n_seqs + slots, a.nv), dim3(256), 0, s, a, ws, rows_ws,
+                     kFrom, pieces, slots);
   MX_TRY(mx_launch_status());
   hipLaunchKernelGGL((k_gd_walk<DK, NT, XT>), dim3(mx_ceil_div(a.dv, 16 * NT) * a.nv, a.n_seqs), dim3(256 * NT), 0, s, a,
                      ws, rows_ws, kFrom, a.nk % 8 == 0);
@@ -853,9 +913,7 @@ bool full(const GdArgs& a) {
 
 template <typename XT>
 int run(const MxGatedDelta* d, const GdArgs& a, char* ws, hipStream_t s) {
-  const bool long_rows = chunked(d);
-  MX_TRY(launch_recurrent<XT>(a, long_rows ? kFrom : 1 << 30, s));
-  if (!long_rows) return MX_OK;
+  if (!chunked(d)) return launch_recurrent<XT>(a, s);
   if (full<XT>(a)) return a.dk == 64 ? launch_chunked<64, true, XT>(a, ws, s) : launch_chunked<128, true, XT>(a, ws, s);
   return a.dk <= 64 ? launch_chunked<64, false, XT>(a, ws, s) : launch_chunked<128, false, XT>(a, ws, s);
 }
