@@ -204,7 +204,7 @@ constexpr int kC = 64;  // tokens of a chunk
 // apart next to each other and keeps the L1 busy for each (walk of 4 prompts of up to
 // 2600 tokens: 278 us, 170 like this).  T and P: [plane][16 rows][2 blocks of 16 columns][lane]; k and q: [plane][16
 // rows][32 dims][lane].
-enum { kFa, kFb, kFc, kFbeta, kFt, kFp, kFkm, kFend, kFactors };
+enum { kFa, kFb, kFc, kFbeta, kFt, kFp, kFend, kFactors };
 constexpr int kPlane = kC * kC * 2, kOffP = 2 * kPlane, kOffF = 4 * kPlane, kRec = kOffF + kFactors * kC * 4;
 template <int DK, typename XT>
 constexpr int kRows = kC * DK * (sizeof(XT) == 2 ? 2 : 4);  // bytes of k's planes, and of q's
@@ -313,7 +313,7 @@ struct GdPrepLds {
   static constexpr int W = kC + 4;
   float a[kC * W], t[kC * W];
   double g[kC];
-  float k2[kC], q2[kC], km[kC], ki[kC], qi[kC], beta[kC], bad[kC];
+  float k2[kC], q2[kC], ki[kC], qi[kC], beta[kC], bad[kC];
 };
 
 template <int DK, bool FULL, typename XT>
@@ -405,19 +405,21 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
     q2 = gd_sum16(q2);
     km = pk_rowmax(km);
     qm = pk_rowmax(qm);
-    float ki = 1.f, qi = 1.f, ks = 1.f, qs = 1.f;
-    if constexpr (sizeof(XT) == 4) {
-      ks = gd_scale(km, ki);
-      qs = gd_scale(qm, qi);
-      km *= ks;
-    }
+    float ki, qi;
+    const float ks = gd_scale(km, ki), qs = gd_scale(qm, qi);
     if (h == hk * a.rep) {  // k and q for all value heads of theirs
       char* to = rows_ws + ((long)id * a.nk + hk) * (2 * kRows<DK, XT>) + (w * M * 64 + lane) * 16;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         if constexpr (sizeof(XT) == 2) {
-          *(half8_t*)(to + m * 1024) = kf[m];
-          *(half8_t*)(to + kRows<DK, XT> + m * 1024) = qf[m];
+          half8_t x, y;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = (half_t)((float)kf[m][e] * ks);
+            y[e] = (half_t)((float)qf[m][e] * qs);
+          }
+          *(half8_t*)(to + m * 1024) = x;
+          *(half8_t*)(to + kRows<DK, XT> + m * 1024) = y;
         } else {
           half8_t x[4];
           gd_split<8>((const float*)&kf[m], ks, (half_t*)&x[0], (half_t*)&x[1]);
@@ -430,7 +432,6 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
     if (q == 0) {
       lds.p.k2[t] = a.norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.f;
       lds.p.q2[t] = (a.norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.f) * a.scale;
-      lds.p.km[t] = km;
       lds.p.ki[t] = ki;
       lds.p.qi[t] = qi;
     }
@@ -566,7 +567,6 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
     f[kFb * kC + tid] = eg * lds.p.q2[tid] * lds.p.qi[tid];
     f[kFc * kC + tid] = expf((float)(end - G)) * k2 * ki;
     f[kFbeta * kC + tid] = lds.p.beta[tid];
-    f[kFkm * kC + tid] = lds.p.km[tid];
     f[kFend * kC + tid] = expf((float)end);
   }
 }
@@ -575,15 +575,26 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
 // the chunk and the 16 columns 16 nt .. of the block's, and the rows 16 SL rt .. of the state, in
 // accumulators.  Per chunk three barriers:
 //   the state's planes to LDS  | k^T S and q^T S; x to LDS, k to LDS  | u = T x to LDS  | o and S
+// The next chunk's loads go out a few at a time (GD_HERE): four waves' 16-byte loads take the L1 about 64
+// cycles, and a wave that issues nine in a row waits for most of them.
+//
 // A column's factor 2^e of the state's planes has to be known before all waves have the new state: from
-// the bound e^G max|S| + 64 max|k u|, whose maxima went through LDS with x and u before.  It may
-// exceed the maximum by 2^10 before the 2^-39 above reaches fp32's own 2^-24.
+// the bound e^G max|S| + 64 max|k| max|c u|, whose maxima went through LDS before (k's rows are
+// scaled to 2^15, c u's are below 2^15 of their factor).  It may exceed the maximum by 2^10 before
+// the 2^-39 above reaches fp32's own 2^-24.
 //
 // A NaN or infinity in x (a NaN in v is one of its column, in k of every column) would meet the zeros
-// above T's diagonal: it is taken out, and u, o and S from that row on are NaN, as token by
-// token.
+// above T's diagonal: it is taken out, as it is out of u, and u, o and S from that row on are NaN, as
+// token by token.
+#define GD_HERE(x)                     \
+  do {                                 \
+    __builtin_amdgcn_sched_barrier(0); \
+    x;                                 \
+    __builtin_amdgcn_sched_barrier(0); \
+  } while (0)
+
 template <int DK, int NT, typename XT>
-__global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __restrict__ ws,
+__global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* __restrict__ ws,
                                                       const char* __restrict__ rows_ws, int from, int groups) {
   constexpr int SL = DK / 64, NP = sizeof(XT) == 2 ? 1 : 2, NC = 16 * NT;
   constexpr int M = DK / 32;
@@ -592,8 +603,8 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   __shared__ __align__(16) half_t sx[2][NC * kC];        // x, u, c u: [column][token]
   __shared__ __align__(16) half_t su[2][NC * kC], sd[2][NC * kC];
   __shared__ float sxi[4][NC], sui[4][NC], sdi[4][NC];   // their 2^e, per 16 tokens
-  __shared__ float smax[2][4][NC], sinc[4][NC];
-  __shared__ int sfirst[NC];
+  __shared__ float smax[2][4][NC];
+  __shared__ int sfirst[2][NC];
   __shared__ __align__(16) float sf[2][kFactors * kC];
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rt = wave & 3, nt = wave >> 2, col = 16 * nt + j;
@@ -615,8 +626,8 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   const char* rec = ws + ((long)gd_base(a.q_start, seq) * a.nv + h) * kRec;
   const bool cl = v0 + col < a.dv;
   const long head = (long)a.dk * a.dv;
-  const char* kq = rows_ws + ((long)gd_base(a.q_start, seq) * a.nk + hk) * (2 * kRows<DK, XT>) + (rt * M * 64 + lane) * 16;
-  const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + (cl ? v0 + col : 0);
+  const char* kq = rows_ws + ((long)gd_base(a.q_start, seq) * a.nk + hk) * (2 * kRows<DK, XT>) + rt * M * 1024;
+  const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + v0;
   XT* op = (XT*)a.o + (long)t0 * a.ldo + (long)h * a.dv + v0;
 
   float4_t s[SL];
@@ -635,58 +646,105 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   XT vf[4];
   float4 ff;
   const int chunks = (n + kC - 1) / kC;
-  // Rows past the end are the last one's again (here and in k_gd_prep): their beta is 0, and where
-  // that row is finite so are x = 0 and all that follows of it.
-  auto load_rows = [&](int c) {
+  // Rows past the end: k and q are the last one's again (k_gd_prep), v is 0 and so is beta; where that
+  // row is finite so are x = 0 and all that follows of it.  All addresses are a base of the wave's and
+  // an offset of the lane's that stays; what lies past a descriptor's end reads as 0 and
+  // is not written, so nothing branches and each load is waited for by itself.
+  const uint32_t lane16 = lane * 16, tid16 = 16 * min(tid, kFactors * kC / 4 - 1);
+  int v_at[4], o_at[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int t = 16 * rt + 4 * q + e;
+    v_at[e] = cl ? (t * (int)a.ldv + col) * (int)sizeof(XT) : -(1 << 31);
+    o_at[e] = cl ? (t * (int)a.ldo + col) * (int)sizeof(XT) : -(1 << 31);
+  }
+  auto rows_of = [&](const XT* x, long ld, int c) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(x + (long)c * kC * ld), (short)0,
+        (int)(((min(n - c * kC, kC) - 1) * ld + min(NC, a.dv - v0)) * (long)sizeof(XT)), 0x00020000);
+  };
+  auto load_rows = [&](int c, int m) {
     const char* p = kq + (long)c * a.nk * (2 * kRows<DK, XT>);
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
+    for (int i = 0; i < NP; ++i) {
+      kf[i][m] = *(const half8_t*)(p + i * (kC * DK * 2) + m * 1024 + lane16);
+      qf[i][m] = *(const half8_t*)(p + kRows<DK, XT> + i * (kC * DK * 2) + m * 1024 + lane16);
+    }
+  };
+  auto load_v = [&](int c) {
+    const mx_rsrc_t vr = rows_of(vp, a.ldv, c);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        kf[i][m] = *(const half8_t*)(p + i * (kC * DK * 2) + m * 1024);
-        qf[i][m] = *(const half8_t*)(p + kRows<DK, XT> + i * (kC * DK * 2) + m * 1024);
-      }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) vf[e] = vp[(long)min(c * kC + 16 * rt + 4 * q + e, n - 1) * a.ldv];
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(XT) == 2)
+        vf[e] = __builtin_bit_cast(XT, __builtin_amdgcn_raw_buffer_load_b16(vr, v_at[e], 0, 0));
+      else
+        vf[e] = __builtin_bit_cast(XT, __builtin_amdgcn_raw_buffer_load_b32(vr, v_at[e], 0, 0));
+    }
   };
   auto load_tri = [&](int c, int off, half8_t (&x)[2][2]) {
-    const char* p = rec + (long)c * a.nv * kRec + off + rt * 2048 + lane * 16;
+    const char* p = rec + (long)c * a.nv * kRec + off + rt * 2048;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) x[i][b] = *(const half8_t*)(p + i * kPlane + 1024 * min(b, rt >> 1));
+      for (int b = 0; b < 2; ++b) x[i][b] = *(const half8_t*)(p + i * kPlane + 1024 * min(b, rt >> 1) + lane16);
   };
-  auto load_factors = [&](int c) {
-    ff = *(const float4*)(rec + (long)c * a.nv * kRec + kOffF + 16 * min(tid, kFactors * kC / 4 - 1));
-  };
+  auto load_factors = [&](int c) { ff = *(const float4*)(rec + (long)c * a.nv * kRec + kOffF + tid16); };
   auto factor = [&](const float* f, int k) { return *(const float4_t*)(f + k * kC + 16 * rt + 4 * q); };
-  // [column][token] tiles: 8-byte pieces, swizzled by the column
-  auto piece = [&](int b) { return col * kC + ((4 * b + q) ^ j) * 4; };
+  // Places in LDS, in halves; the swizzles are xors, so that places differ by xors of constants too.
+  // [column][token]: 8-byte piece 4 b + q of the tokens 16 b .., at piece ^ column
+  int pieces[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) pieces[b] = col * kC + ((4 * b + q) ^ j) * 4;
+  const int pieces_rt = col * kC + ((4 * rt + q) ^ j) * 4;
+  // the state [column][row]: 16-byte pieces at piece ^ (column & 7); written by 8 bytes, read by 16
+  const int s_put = col * DK + (((2 * SL * rt + (q >> 1)) ^ (j & 7)) << 3) + (q & 1) * 4;
+  const int s_get = col * DK + ((q ^ (j & 7)) << 3);
+  // k [token][dim]: 16-byte pieces at piece ^ (2 (token & 3) + (token >> 2 & 1)); written by token 16 rt + j,
+  // read transposed, 16 dims of the tokens 4 q .. by 16 lanes
+  const int k_put = (16 * rt + j) * DK + ((q ^ (2 * (j & 3) + ((j >> 2) & 1))) << 3);
+  const int k_get = (4 * q + (j >> 2)) * DK + (((2 * SL * rt + ((j & 3) >> 1)) ^ (2 * (j >> 2) + (q & 1))) << 3) + (j & 1) * 4;
   auto put = [&](half_t (&to)[2][NC * kC], const float4_t& x, float (&inv)[4][NC]) {
     float iv;
     const float sc = gd_scale(pk_rowmax(gd_max4(x)), iv);
     half4_t p[2];
     gd_split<4>((const float*)&x, sc, (half_t*)&p[0], (half_t*)&p[1]);
-    *(half4_t*)&to[0][piece(rt)] = p[0];
-    *(half4_t*)&to[1][piece(rt)] = p[1];
+    *(half4_t*)&to[0][pieces_rt] = p[0];
+    *(half4_t*)&to[1][pieces_rt] = p[1];
     if (q == 0) inv[rt][col] = iv;
   };
-  // sum over the token blocks up to rt of x (row planes) times what put() left
+  // sum over the token blocks up to rt of x (row planes) times what put() left; the other blocks' x is
+  // not there: as zeros they keep the sum free of branches
   auto tri = [&](const half8_t (&x)[2][2], const half_t (&y)[2][NC * kC], const float (&inv)[4][NC]) {
-    float4_t z = (float4_t)0.f;
+    float4_t hh[4], mix[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      if (b > rt) continue;
-      const half4_t hi = *(const half4_t*)&y[0][piece(b)], lo = *(const half4_t*)&y[1][piece(b)];
-      float4_t c = gd_mfma(gd_half(x[1][b >> 1], b & 1), hi, (float4_t)0.f);
-      c = gd_mfma(gd_half(x[0][b >> 1], b & 1), lo, c);
-      c = gd_mfma(gd_half(x[0][b >> 1], b & 1), hi, c);
-      z += c * inv[b][col];
+      const half4_t hi = *(const half4_t*)&y[0][pieces[b]], lo = *(const half4_t*)&y[1][pieces[b]];
+      const half4_t zero = (half4_t)(half_t)0;
+      const half4_t xh = b <= rt ? gd_half(x[0][b >> 1], b & 1) : zero, xl = b <= rt ? gd_half(x[1][b >> 1], b & 1) : zero;
+      mix[b] = gd_mfma(xl, hi, (float4_t)0.f);
+      hh[b] = gd_mfma(xh, hi, (float4_t)0.f);
+      mix[b] = gd_mfma(xh, lo, mix[b]);
     }
+    float4_t z = (float4_t)0.f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) z += (hh[b] + mix[b]) * inv[b][col];
     return z;
   };
+  // Takes what is not finite out of x, and notes the first such token of the column.
+  auto clean = [&](float4_t& x, int (&first)[NC]) {
+    const float sum = (fabsf(x[0]) + fabsf(x[1])) + (fabsf(x[2]) + fabsf(x[3]));
+    if (__builtin_amdgcn_ballot_w64(!(sum <= 3.0e38f)) == 0) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(fabsf(x[e]) <= 3.0e38f)) {
+        atomicMin(&first[col], 16 * rt + 4 * q + e);
+        x[e] = 0.f;
+      }
+  };
 
-  load_rows(0);
+#pragma unroll
+  for (int m = 0; m < M; ++m) load_rows(0, m);
+  load_v(0);
   load_tri(0, 0, tf);
   load_tri(0, kOffP, pf);
   load_factors(0);
@@ -695,13 +753,14 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
   for (int i = 0; i < SL; ++i) bound = fmaxf(bound, gd_max4(s[i]));
   bound = pk_rowmax(bound);
   if (q == 0) smax[1][rt][col] = bound;
-  if (tid < NC) sfirst[tid] = kC;
+  if (tid < NC) sfirst[0][tid] = kC;
   if (tid < kFactors * kC / 4) *(float4*)&sf[0][4 * tid] = ff;
   __syncthreads();
   bound = fmaxf(fmaxf(smax[1][0][col], smax[1][1][col]), fmaxf(smax[1][2][col], smax[1][3][col]));
 
   for (int c = 0; c < chunks; ++c) {
     const float* f = sf[c & 1];
+    const int next = min(c + 1, chunks - 1);
     float sinv;
     {  // the state's planes
       const float sc = gd_scale(bound, sinv);
@@ -710,8 +769,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       for (int i = 0; i < SL; ++i) {
         half4_t p[2];
         gd_split<4>((const float*)&s[i], sc, (half_t*)&p[0], (half_t*)&p[1]);
-        const int pc = 4 * (SL * rt + i) + q;  // 8-byte piece of the column
-        const int at = col * DK + (((pc >> 1) ^ (j & 7)) << 3) + (pc & 1) * 4;
+        const int at = s_put ^ (16 * i);
         *(half4_t*)&ss[0][at] = p[0];
         *(half4_t*)&ss[1][at] = p[1];
         m = fmaxf(m, gd_max4(s[i]));
@@ -725,7 +783,7 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       float4_t x = (float4_t)0.f;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const int at = col * DK + (((4 * m + q) ^ (j & 7)) << 3);
+        const int at = (s_get ^ (32 * (m & 1))) + 64 * (m >> 1);
         const half8_t hi = *(const half8_t*)&ss[0][at], lo = *(const half8_t*)&ss[1][at];
         if constexpr (NP == 2) {
           x = gd_mfma(kf[NP - 1][m], hi, x);
@@ -735,54 +793,46 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
         o = gd_mfma(qf[0][m], lo, o);
         x = gd_mfma(kf[0][m], hi, x);
         o = gd_mfma(qf[0][m], hi, o);
-        if (nt == 0) {
-          const int t = 16 * rt + j, sw = 2 * (t & 3) + ((t >> 2) & 1);
-#pragma unroll
-          for (int i = 0; i < NP; ++i) *(half8_t*)&skey[i][t * DK + (((4 * m + q) ^ sw) << 3)] = kf[i][m];
-        }
       }
+      if (nt == 0) {
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < NP; ++i) *(half8_t*)&skey[i][(k_put ^ (32 * (m & 1))) + 64 * (m >> 1)] = kf[i][m];
+      }
+      GD_HERE(load_rows(next, 0));
       const float4_t fa = factor(f, kFa), fb = factor(f, kFbeta);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = fb[e] * ((float)vf[e] - fa[e] * (x[e] * sinv));
-        if (!(fabsf(x[e]) <= 3.0e38f)) {
-          atomicMin(&sfirst[col], 16 * rt + 4 * q + e);
-          x[e] = 0.f;
-        }
-      }
+      for (int e = 0; e < 4; ++e) x[e] = fb[e] * ((float)vf[e] - fa[e] * (x[e] * sinv));
+      clean(x, sfirst[c & 1]);
       o = o * sinv * factor(f, kFb);
       put(sx, x, sxi);
+      GD_HERE(load_rows(next, 1));
     }
-    const int next = min(c + 1, chunks - 1);  // (loads without a branch can be waited for one by one)
-    load_rows(next);
-    load_factors(next);
     __syncthreads();
-    const int first = sfirst[col];
     {  // u
-      const float4_t u = tri(tf, sx, sxi) * factor(f, kFt);
-      const float4_t d = u * factor(f, kFc), km = factor(f, kFkm);
+      if constexpr (M > 2) GD_HERE(load_rows(next, 2));
+      float4_t u = tri(tf, sx, sxi) * factor(f, kFt);
+      if constexpr (M > 2) GD_HERE(load_rows(next, 3));
+      clean(u, sfirst[c & 1]);
       put(su, u, sui);
-      put(sd, d, sdi);
-      const float m = pk_rowmax(gd_max4(d * km));
-      if (q == 0) sinc[rt][col] = m;
+      put(sd, u * factor(f, kFc), sdi);
     }
-    load_tri(next, 0, tf);
+    GD_HERE(load_tri(next, 0, tf));
     __syncthreads();
+    const int first = sfirst[c & 1][col];
     o += tri(pf, su, sui) * factor(f, kFp);
-    load_tri(next, kOffP, pf);
-    // A store past the descriptor's end (a row or column there is not) is dropped: no branch.
-    const mx_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
-        op + (long)c * kC * a.ldo, (short)0,
-        (int)(((min(n - c * kC, kC) - 1) * a.ldo + min(NC, a.dv - v0)) * (long)sizeof(XT)), 0x00020000);
+    GD_HERE(load_tri(next, kOffP, pf));
+    load_v(next);
+    load_factors(next);
+    const mx_rsrc_t to = rows_of(op, a.ldo, c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int t = 16 * rt + 4 * q + e;
-      const XT y = (XT)(t < first ? o[e] : __builtin_nanf(""));
-      const int at = cl ? (t * (int)a.ldo + col) * (int)sizeof(XT) : -(1 << 31);
+      const XT y = (XT)(16 * rt + 4 * q + e < first ? o[e] : __builtin_nanf(""));
       if constexpr (sizeof(XT) == 2)
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), to, at, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), to, o_at[e], 0, 0);
       else
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), to, at, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), to, o_at[e], 0, 0);
     }
     const float end = f[kFend * kC];
 #pragma unroll
@@ -790,10 +840,8 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       s[i] *= end;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const half4_t hi = *(const half4_t*)&sd[0][piece(b)], lo = *(const half4_t*)&sd[1][piece(b)];
-        // k's 16 dims of the slab as rows: lane (j, q) dim j of the tokens 4 q ..
-        const int t = 16 * b + 4 * q + (j >> 2), sw = 2 * (t & 3) + ((t >> 2) & 1);
-        const int at = t * DK + (((2 * (SL * rt + i) + ((j & 3) >> 1)) ^ sw) << 3) + (j & 1) * 4;
+        const half4_t hi = *(const half4_t*)&sd[0][pieces[b]], lo = *(const half4_t*)&sd[1][pieces[b]];
+        const int at = (k_get ^ (16 * i)) + 16 * b * DK;
         auto key = [&](int p) {
           return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((gd_lds_s4*)&skey[p][at]));
         };
@@ -807,9 +855,9 @@ __global__ __launch_bounds__(256 * NT) void k_gd_walk(GdArgs a, const char* __re
       if (first < kC) s[i] = (float4_t)__builtin_nanf("");
     }
     bound = fmaxf(fmaxf(smax[c & 1][0][col], smax[c & 1][1][col]), fmaxf(smax[c & 1][2][col], smax[c & 1][3][col]));
-    bound = end * bound + 64.f * fmaxf(fmaxf(sinc[0][col], sinc[1][col]), fmaxf(sinc[2][col], sinc[3][col]));
+    bound = end * bound + 0x1p36f * fmaxf(fmaxf(sdi[0][col], sdi[1][col]), fmaxf(sdi[2][col], sdi[3][col]));
     if (tid < kFactors * kC / 4) *(float4*)&sf[(c + 1) & 1][4 * tid] = ff;
-    if (tid < NC) sfirst[tid] = kC;
+    if (tid < NC) sfirst[(c + 1) & 1][tid] = kC;
   }
   if (out < 0 || out >= a.n_slots || !cl) return;
 #pragma unroll
@@ -884,8 +932,8 @@ int launch_recurrent(const GdArgs& a, hipStream_t s) {
 constexpr int kFrom = 24;  // rows from which a sequence goes chunk by chunk
 
 bool chunked(const MxGatedDelta* d) {
-  // (o's chunks are written through a descriptor of 2^31 bytes)
-  return d->head_dim_k <= 128 && d->ldo < (1 << 23) && (d->max_q < d->rows ? d->max_q : d->rows) >= kFrom;
+  // (a chunk's rows of v and o go through a descriptor of 2^31 bytes)
+  return d->head_dim_k <= 128 && d->ldv < (1 << 23) && d->ldo < (1 << 23) && (d->max_q < d->rows ? d->max_q : d->rows) >= kFrom;
 }
 
 template <int DK, bool FULL, typename XT>
