@@ -780,6 +780,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     __syncthreads();
     float4_t o = (float4_t)0.f;
     {  // k^T S, q^T S
+      GD_HERE(load_factors(next));
       float4_t x = (float4_t)0.f;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
@@ -824,7 +825,6 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     o += tri(pf, su, sui) * factor(f, kFp);
     GD_HERE(load_tri(next, kOffP, pf));
     load_v(next);
-    load_factors(next);
     const mx_rsrc_t to = rows_of(op, a.ldo, c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
