@@ -304,7 +304,7 @@ __device__ __forceinline__ typename GdVec<XT>::T gd_load8(const XT* row, int d, 
 // T and P of the chunks, and the sequences that are too short for chunks (token by token, by the
 // first blocks: a launch of their own would take its time next to the others').  A block: one chunk of one value
 // head; wave w forms the rows 16 w .. of k k^T and q k^T (fp16 rows: exact products; fp32 rows: fp32
-// matrix instructions), operands straight from memory, as both are rows of k and q.  T: the 16 x 16
+// matrix instructions), whose operands are both rows of k and q.  T: the 16 x 16
 // blocks on the diagonal by substitution, a column per lane; then pairs, T_10 = -T_11 A_10 T_00,
 // twice.  A product's result has the layout of the next one's right operand, so only T's
 // pieces go through LDS.  A chain of short steps, each waiting for the one before: bound by how many
@@ -352,12 +352,36 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
       beta = a.beta[at];
     }
     const int t = 16 * w + j;
-    const XT *kr = row(a.k, a.ldk, t), *qr = row(a.q, a.ldq, t);
     typename GdVec<XT>::T kf[M], qf[M];
+    // Fp16 rows through LDS (where T and A come later), a row's 16-byte pieces at piece ^ (row & 7): a
+    // fragment's lanes next to each other are in 16 rows, 64 accesses of the L1 for each load.
+    half_t *lk = (half_t*)sa, *lq = (half_t*)st;
+    auto place = [&](int r, int p) { return r * DK + ((p ^ (r & 7)) << 3); };
+    if constexpr (sizeof(XT) == 2) {
+      constexpr int PR = DK / 8;
+#pragma unroll
+      for (int i = 0; i < kC * PR / 256; ++i) {
+        const int r = (i * 256 + tid) / PR, p = tid % PR;
+        kf[i] = gd_load8<FULL, XT>(row(a.k, a.ldk, r), 8 * p, a.dk);
+        qf[i] = gd_load8<FULL, XT>(row(a.q, a.ldq, r), 8 * p, a.dk);
+      }
+#pragma unroll
+      for (int i = 0; i < kC * PR / 256; ++i) {
+        const int r = (i * 256 + tid) / PR, p = tid % PR;
+        *(half8_t*)&lk[place(r, p)] = kf[i];
+        *(half8_t*)&lq[place(r, p)] = qf[i];
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      kf[m] = gd_load8<FULL, XT>(kr, 32 * m + 8 * q, a.dk);
-      qf[m] = gd_load8<FULL, XT>(qr, 32 * m + 8 * q, a.dk);
+      if constexpr (sizeof(XT) == 2) {
+        kf[m] = *(const half8_t*)&lk[place(t, 4 * m + q)];
+        qf[m] = *(const half8_t*)&lq[place(t, 4 * m + q)];
+      } else {
+        kf[m] = gd_load8<FULL, XT>(row(a.k, a.ldk, t), 32 * m + 8 * q, a.dk);
+        qf[m] = gd_load8<FULL, XT>(row(a.q, a.ldq, t), 32 * m + 8 * q, a.dk);
+      }
     }
     if (w == 0) {
       double G = g < -256.f ? -256.f : g;
@@ -373,10 +397,13 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       if (b > w) continue;
-      const XT* br = row(a.k, a.ldk, 16 * b + j);
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const auto bf = gd_load8<FULL, XT>(br, 32 * m + 8 * q, a.dk);
+        typename GdVec<XT>::T bf;
+        if constexpr (sizeof(XT) == 2)
+          bf = *(const half8_t*)&lk[place(16 * b + j, 4 * m + q)];
+        else
+          bf = gd_load8<FULL, XT>(row(a.k, a.ldk, 16 * b + j), 32 * m + 8 * q, a.dk);
         if constexpr (sizeof(XT) == 2) {
           kk[b] = gd_mfma(kf[m], bf, kk[b]);
           qk[b] = gd_mfma(qf[m], bf, qk[b]);
