@@ -202,3 +202,82 @@ def test_a_prompt_in_pieces_is_the_prompt_at_once(mi355x, stream):
         at += n
     tol = 2 * (2 * dk + 64) * 2.0 ** -24
     assert at == T and off(np.concatenate(parts), o) <= tol and off(st, s) <= tol
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_many_sequences_of_all_lengths(mi355x, stream, dtype):
+    """More sequences than a wave looks at in one go, empty ones and single tokens among prompts: some
+    go token by token and some chunk by chunk in the same call."""
+    say(f"delta rule, 150 sequences, {dtype}")
+    nk, nv, dk, dv = 1, 2, 64, 64
+    rng = np.random.default_rng(17)
+    news = [0, 1, 23, 24, 25, 63, 64, 65, 128, 0, 2, 129, 1, 0]
+    news = news + [int(n) for n in rng.choice([0, 1, 1, 3, 26, 40], 150 - len(news))]
+    x = make(rng, news, nk, nv, dk, dv, dtype, pad=70)
+    n = len(news)
+    state = (rng.standard_normal((n, nv, dk, dv)) * 0.3).astype(np.float32)
+    slot_in = rng.permutation(n)
+    slot_out = slot_in.copy()
+    slot_in[5::7] = n + 3  # afresh
+    slot_out[3::11] = -1   # left nowhere
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, slot_in, slot_out)
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, slot_in, slot_out, dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    assert off(s, ws) <= tol and off(o[:sum(news)], wo) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("news", [[12], [90, 150]])
+def test_magnitudes_far_apart(mi355x, stream, news, dtype):
+    """Keys and queries of lengths from 2^-8 to 2^8 (they are normalised), columns of v and of the state
+    from 2^-40 to 2^40 (fp16 rows: v 2^-6 to 2^6): every column to its own scale."""
+    say(f"delta rule, magnitudes far apart, rows={news} {dtype}")
+    nk, nv, dk, dv = 2, 2, 128, 64
+    rng = np.random.default_rng(21)
+    q, k, v, g, beta = make(rng, news, nk, nv, dk, dv, "float32")
+    T = sum(news)
+    q *= 2.0 ** rng.integers(-8, 9, (T, nk, 1))
+    k *= 2.0 ** rng.integers(-8, 9, (T, nk, 1))
+    wide = 40 if dtype == "float32" else 6
+    col = 2.0 ** rng.integers(-wide, wide + 1, dv)
+    x = tuple(a.astype(sv.DT[dtype]) for a in (q, k, v * col)) + (g, beta)
+    state = (rng.standard_normal((2, nv, dk, dv)) * col).astype(np.float32)
+    io = list(range(len(news)))
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, io, io)
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, io, io, dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    half = 0.0 if dtype == "float32" else 2.0 ** -11
+    for c in range(dv):
+        assert off(s[..., c], ws[..., c]) <= tol
+        # an output under fp16's normal range is off by half its smallest step
+        small = 0.0 if dtype == "float32" else 2.0 ** -25 * np.sqrt(wo[..., c].size)
+        assert np.linalg.norm(o[..., c] - wo[..., c]) <= (tol + half) * np.linalg.norm(wo[..., c]) + small
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("n,at", [(10, 4), (150, 70), (150, 63), (150, 0), (130, 129)])
+def test_a_token_that_is_not_finite_leaves_those_before_it(mi355x, stream, n, at, dtype):
+    """NaN or an infinity in one token of v (one column), k, g, beta or q: what comes before it is as it
+    was, what follows is not finite, and q's is its own row alone."""
+    say(f"delta rule, poisoned token {at} of {n}, {dtype}")
+    nk, nv, dk, dv = 1, 1, 64, 32
+    rng = np.random.default_rng(n + at)
+    news = [n] * 7
+    q, k, v, g, beta = x = make(rng, news, nk, nv, dk, dv, dtype)
+    v[at, 0, 5] = np.nan
+    v[n + at, 0, 7] = np.inf
+    k[2 * n + at, 0, 9] = np.nan
+    g[3 * n + at] = np.nan
+    beta[4 * n + at] = np.nan
+    q[5 * n + at, 0, 3] = np.nan
+    k[6 * n + at, 0, 3] = -np.inf
+    state = rng.standard_normal((7, nv, dk, dv)).astype(np.float32)
+    io = list(range(7))
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, io, io)
+    with np.errstate(invalid="ignore", over="ignore"):
+        wo, ws = want_of(x, news, nk, nv, dk, dv, state, io, io, dk ** -0.5)
+    assert np.array_equal(np.isfinite(o), np.isfinite(wo)) and np.array_equal(np.isfinite(s), np.isfinite(ws))
+    tol = (2 * dk + 64) * 2.0 ** -24
+    ok, good = np.isfinite(wo), np.isfinite(ws)
+    assert off(s[good], ws[good]) <= tol
+    assert off(o[ok], wo[ok]) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)

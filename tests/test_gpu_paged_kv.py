@@ -370,3 +370,52 @@ def test_a_server_of_forking_sequences(mi355x, stream, dtype):
         assert cache.tables.free_pages > 0
     finally:
         cache.close()
+
+
+# ---- many sequences --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float16", "int8", "float32"])
+@pytest.mark.parametrize("n,longest", [(100, 900), (4200, 20)])
+def test_more_sequences_than_a_wave_looks_at(mi355x, stream, n, longest, dtype):
+    """The sequence of a row and the ranges of keys are found 64 sequences at a time."""
+    say(f"attention over {n} sequences, {dtype}")
+    rng = np.random.default_rng(n)
+    news = [int(v) for v in rng.choice([0, 1, 1, 1, 2], n)]
+    lens = [int(m + v) for m, v in zip(news, rng.integers(0, longest, n))]
+    lens[n // 2] = 3 * longest
+    b = sv.Batch(rng, news, lens, 16, pad=5)
+    got, want, tol = check_attention(mi355x, stream, b, 2, 1, 32, dtype, 3)
+    assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_append_of_more_sequences_than_a_wave_looks_at(mi355x, stream, dtype):
+    n, nkv, hd, page = 4200, 1, 16, 16
+    say(f"append to {n} sequences, {dtype}")
+    rng = np.random.default_rng(3)
+    news = [int(v) for v in rng.choice([0, 1, 1, 2], n)]
+    lens = [int(m + v) for m, v in zip(news, rng.integers(0, 20, n))]
+    b = sv.Batch(rng, news, lens, page, pad=3)
+    k0 = np.zeros((b.n_pages, nkv, page, hd), sv.DT[dtype])
+    x = rng.standard_normal((b.rows, nkv * hd)).astype(sv.DT[dtype])
+    with sv.Arrays(mi355x, stream) as ar:
+        cache, buf = cache_of(mi355x, ar, b, nkv, hd, dtype, k0, None, k0, None)
+        px = ar.put(x)
+        cache.append(0, b.device(ar), append_args(k=px, v=px, n_kv_heads=nkv, head_dim=hd, dtype=dtype),
+                     stream)
+        k = ar.get(buf[0], k0)
+    want = k0.copy()
+    for i, m in enumerate(news):
+        pos = b.positions(i)
+        want[b.table[i, pos // page], 0, pos % page] = x[b.q_start[i]:b.q_start[i] + m]
+    assert np.array_equal(k, want)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "int8", "float32"])
+@pytest.mark.parametrize("news,lens", [([1], [30000]), ([1, 1], [9000, 20000]), ([2, 1, 70], [4097, 8193, 4200])])
+def test_long_caches(mi355x, stream, news, lens, dtype):
+    """More ranges of keys per row than a wave has lanes, and ranges of the largest size."""
+    say(f"attention over long caches {lens}, {dtype}")
+    b = sv.Batch(np.random.default_rng(1), news, lens, 64)
+    got, want, tol = check_attention(mi355x, stream, b, 4, 1, 64, dtype, 2)
+    assert np.all(np.abs(got - want) <= tol)

@@ -265,3 +265,22 @@ def test_python_arguments_are_checked():
         PagedKvCache(None, 2, 2, 64, 4, buffers=[(A, A, None, None)])
     with pytest.raises(ValueError):
         PageTables(0, 16)
+
+
+def test_delta_workspaces():
+    """Token by token there is none; chunk by chunk it has to be there, large enough and aligned."""
+    lib, n = _lib.load(), ctypes.c_size_t()
+
+    def size(**kw):
+        assert lib.mx_gated_delta_rule_workspace_size(ctypes.byref(delta(**kw)), ctypes.byref(n)) == 0
+        return n.value
+
+    long_rows = dict(rows=100, max_q=64)
+    assert size() == 0 and size(rows=4, max_q=1000) == 0 and size(rows=1000, max_q=1) == 0
+    assert size(head_dim_k=256, ldq=1024, ldk=1024, **long_rows) == 0
+    need = size(**long_rows)
+    assert need > 0 and size(rows=200, max_q=64) > need
+    d = delta(**long_rows)
+    assert lib.mx_gated_delta_rule(ctypes.byref(d), None, need, None) == _lib.MX_ERR_WORKSPACE
+    assert lib.mx_gated_delta_rule(ctypes.byref(d), A, need - 1, None) == _lib.MX_ERR_WORKSPACE
+    assert lib.mx_gated_delta_rule(ctypes.byref(d), A + 8, need, None) == ALI
