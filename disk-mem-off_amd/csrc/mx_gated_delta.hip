@@ -327,8 +327,8 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
   } lds;
   const long block = (long)blockIdx.y * gridDim.x + blockIdx.x, short_blocks = (long)pieces * a.nv * a.n_seqs;
   if (block < short_blocks) {
-    const int hs = (int)(block / pieces);
-    gd_recurrent<DK / 32, XT>(a, lds.r, (int)(block % pieces), hs % a.nv, hs / a.nv, from);
+    const long hs = block / pieces;
+    gd_recurrent<DK / 32, XT>(a, lds.r, (int)(block % pieces), (int)(hs % a.nv), (int)(hs / a.nv), from);
     return;
   }
   const int h = (int)((block - short_blocks) / slots), hk = h / a.rep, id = (int)((block - short_blocks) % slots);
@@ -598,10 +598,13 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
   }
 }
 
-// A sequence's chunks in order.  Waves come in fours: wave (rt, nt) has the tokens 16 rt .. of
-// the chunk and the 16 columns 16 nt .. of the block's, and the rows 16 SL rt .. of the state, in
-// accumulators.  Per chunk three barriers:
+// A sequence's chunks in order, 16 columns of a head's state per block.  Wave rt has the tokens 16 rt ..
+// of the chunk and the rows 16 SL rt .. of the state, in accumulators.  Per chunk three barriers:
 //   the state's planes to LDS  | k^T S and q^T S; x to LDS, k to LDS  | u = T x to LDS  | o and S
+// Bound by these steps one after the other: a chunk takes 2.3 us where a CU has one block and 3.5 with
+// two (heads of 128 x 128, fp16).  Tried and slower: 32 columns per block of 8 waves (442 us
+// against 380 for 4 prompts of up to 2600 tokens, early on), and 8 waves for 16 columns, four
+// of them for k and T and four for q and P (180 us against 147).
 // The next chunk's loads go out a few at a time (GD_HERE): four waves' 16-byte loads take the L1 about 64
 // cycles, and a wave that issues nine in a row waits for most of them.
 //
@@ -620,11 +623,10 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
     __builtin_amdgcn_sched_barrier(0); \
   } while (0)
 
-template <int DK, int NT, typename XT>
-__global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* __restrict__ ws,
-                                                      const char* __restrict__ rows_ws, int from, int groups) {
-  constexpr int SL = DK / 64, NP = sizeof(XT) == 2 ? 1 : 2, NC = 16 * NT;
-  constexpr int M = DK / 32;
+template <int DK, typename XT>
+__global__ __launch_bounds__(256, 2) void k_gd_walk(GdArgs a, const char* __restrict__ ws,
+                                                   const char* __restrict__ rows_ws, int from, int groups) {
+  constexpr int SL = DK / 64, NP = sizeof(XT) == 2 ? 1 : 2, NC = 16, M = DK / 32;
   __shared__ __align__(16) half_t ss[2][NC * DK];        // the state [column][row]
   __shared__ __align__(16) half_t skey[NP][kC * DK];     // k [token][dim]
   __shared__ __align__(16) half_t sx[2][NC * kC];        // x, u, c u: [column][token]
@@ -634,7 +636,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
   __shared__ int sfirst[2][NC];
   __shared__ __align__(16) float sf[2][kFactors * kC];
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rt = wave & 3, nt = wave >> 2, col = 16 * nt + j;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rt = wave;
   const int seq = blockIdx.y;
   // Slices of a key head's value heads next to each other on one XCD: they read the same k, q, T, P.
   int hk, r;
@@ -651,7 +653,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
   if (n < from) return;
   const int in = a.slot_in[seq], out = a.slot_out[seq];
   const char* rec = ws + ((long)gd_base(a.q_start, seq) * a.nv + h) * kRec;
-  const bool cl = v0 + col < a.dv;
+  const bool cl = v0 + j < a.dv;
   const long head = (long)a.dk * a.dv;
   const char* kq = rows_ws + ((long)gd_base(a.q_start, seq) * a.nk + hk) * (2 * kRows<DK, XT>) + rt * M * 1024;
   const XT* vp = (const XT*)a.v + (long)t0 * a.ldv + (long)h * a.dv + v0;
@@ -664,7 +666,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     for (int e = 0; e < 4; ++e) {
       const int d = 16 * (SL * rt + i) + 4 * q + e;
       s[i][e] = in >= 0 && in < a.n_slots && cl && d < a.dk
-                    ? a.state[((long)in * a.nv + h) * head + (long)d * a.dv + v0 + col]
+                    ? a.state[((long)in * a.nv + h) * head + (long)d * a.dv + v0 + j]
                     : 0.f;
     }
 
@@ -682,8 +684,8 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int t = 16 * rt + 4 * q + e;
-    v_at[e] = cl ? (t * (int)a.ldv + col) * (int)sizeof(XT) : -(1 << 31);
-    o_at[e] = cl ? (t * (int)a.ldo + col) * (int)sizeof(XT) : -(1 << 31);
+    v_at[e] = cl ? (t * (int)a.ldv + j) * (int)sizeof(XT) : -(1 << 31);
+    o_at[e] = cl ? (t * (int)a.ldo + j) * (int)sizeof(XT) : -(1 << 31);
   }
   auto rows_of = [&](const XT* x, long ld, int c) {
     return __builtin_amdgcn_make_buffer_rsrc(
@@ -721,11 +723,11 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
   // [column][token]: 8-byte piece 4 b + q of the tokens 16 b .., at piece ^ column
   int pieces[4];
 #pragma unroll
-  for (int b = 0; b < 4; ++b) pieces[b] = col * kC + ((4 * b + q) ^ j) * 4;
-  const int pieces_rt = col * kC + ((4 * rt + q) ^ j) * 4;
+  for (int b = 0; b < 4; ++b) pieces[b] = j * kC + ((4 * b + q) ^ j) * 4;
+  const int pieces_rt = j * kC + ((4 * rt + q) ^ j) * 4;
   // the state [column][row]: 16-byte pieces at piece ^ (column & 7); written by 8 bytes, read by 16
-  const int s_put = col * DK + (((2 * SL * rt + (q >> 1)) ^ (j & 7)) << 3) + (q & 1) * 4;
-  const int s_get = col * DK + ((q ^ (j & 7)) << 3);
+  const int s_put = j * DK + (((2 * SL * rt + (q >> 1)) ^ (j & 7)) << 3) + (q & 1) * 4;
+  const int s_get = j * DK + ((q ^ (j & 7)) << 3);
   // k [token][dim]: 16-byte pieces at piece ^ (2 (token & 3) + (token >> 2 & 1)); written by token 16 rt + j,
   // read transposed, 16 dims of the tokens 4 q .. by 16 lanes
   const int k_put = (16 * rt + j) * DK + ((q ^ (2 * (j & 3) + ((j >> 2) & 1))) << 3);
@@ -737,7 +739,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     gd_split<4>((const float*)&x, sc, (half_t*)&p[0], (half_t*)&p[1]);
     *(half4_t*)&to[0][pieces_rt] = p[0];
     *(half4_t*)&to[1][pieces_rt] = p[1];
-    if (q == 0) inv[rt][col] = iv;
+    if (q == 0) inv[rt][j] = iv;
   };
   // sum over the token blocks up to rt of x (row planes) times what put() left; the other blocks' x is
   // not there: as zeros they keep the sum free of branches
@@ -754,7 +756,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     }
     float4_t z = (float4_t)0.f;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) z += (hh[b] + mix[b]) * inv[b][col];
+    for (int b = 0; b < 4; ++b) z += (hh[b] + mix[b]) * inv[b][j];
     return z;
   };
   // Takes what is not finite out of x, and notes the first such token of the column.
@@ -764,7 +766,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (!(fabsf(x[e]) <= 3.0e38f)) {
-        atomicMin(&first[col], 16 * rt + 4 * q + e);
+        atomicMin(&first[j], 16 * rt + 4 * q + e);
         x[e] = 0.f;
       }
   };
@@ -779,11 +781,11 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
 #pragma unroll
   for (int i = 0; i < SL; ++i) bound = fmaxf(bound, gd_max4(s[i]));
   bound = pk_rowmax(bound);
-  if (q == 0) smax[1][rt][col] = bound;
+  if (q == 0) smax[1][rt][j] = bound;
   if (tid < NC) sfirst[0][tid] = kC;
   if (tid < kFactors * kC / 4) *(float4*)&sf[0][4 * tid] = ff;
   __syncthreads();
-  bound = fmaxf(fmaxf(smax[1][0][col], smax[1][1][col]), fmaxf(smax[1][2][col], smax[1][3][col]));
+  bound = fmaxf(fmaxf(smax[1][0][j], smax[1][1][j]), fmaxf(smax[1][2][j], smax[1][3][j]));
 
   for (int c = 0; c < chunks; ++c) {
     const float* f = sf[c & 1];
@@ -802,7 +804,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
         m = fmaxf(m, gd_max4(s[i]));
       }
       m = pk_rowmax(m);
-      if (q == 0) smax[c & 1][rt][col] = m;
+      if (q == 0) smax[c & 1][rt][j] = m;
     }
     __syncthreads();
     float4_t o = (float4_t)0.f;
@@ -822,12 +824,10 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
         x = gd_mfma(kf[0][m], hi, x);
         o = gd_mfma(qf[0][m], hi, o);
       }
-      if (nt == 0) {
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < NP; ++i) *(half8_t*)&skey[i][(k_put ^ (32 * (m & 1))) + 64 * (m >> 1)] = kf[i][m];
-      }
+        for (int i = 0; i < NP; ++i) *(half8_t*)&skey[i][(k_put ^ (32 * (m & 1))) + 64 * (m >> 1)] = kf[i][m];
       GD_HERE(load_rows(next, 0));
       const float4_t fa = factor(f, kFa), fb = factor(f, kFbeta);
 #pragma unroll
@@ -848,7 +848,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
     }
     GD_HERE(load_tri(next, 0, tf));
     __syncthreads();
-    const int first = sfirst[c & 1][col];
+    const int first = sfirst[c & 1][j];
     o += tri(pf, su, sui) * factor(f, kFp);
     GD_HERE(load_tri(next, kOffP, pf));
     load_v(next);
@@ -877,12 +877,12 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
         if constexpr (NP == 2) z = gd_mfma(key(NP - 1), hi, z);
         z = gd_mfma(kh, lo, z);
         z = gd_mfma(kh, hi, z);
-        s[i] += z * sdi[b][col];
+        s[i] += z * sdi[b][j];
       }
       if (first < kC) s[i] = (float4_t)__builtin_nanf("");
     }
-    bound = fmaxf(fmaxf(smax[c & 1][0][col], smax[c & 1][1][col]), fmaxf(smax[c & 1][2][col], smax[c & 1][3][col]));
-    bound = end * bound + 0x1p36f * fmaxf(fmaxf(sdi[0][col], sdi[1][col]), fmaxf(sdi[2][col], sdi[3][col]));
+    bound = fmaxf(fmaxf(smax[c & 1][0][j], smax[c & 1][1][j]), fmaxf(smax[c & 1][2][j], smax[c & 1][3][j]));
+    bound = end * bound + 0x1p36f * fmaxf(fmaxf(sdi[0][j], sdi[1][j]), fmaxf(sdi[2][j], sdi[3][j]));
     if (tid < kFactors * kC / 4) *(float4*)&sf[(c + 1) & 1][4 * tid] = ff;
     if (tid < NC) sfirst[(c + 1) & 1][tid] = kC;
   }
@@ -892,7 +892,7 @@ __global__ __launch_bounds__(256 * NT, 2) void k_gd_walk(GdArgs a, const char* _
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = 16 * (SL * rt + i) + 4 * q + e;
-      if (d < a.dk) a.state[((long)out * a.nv + h) * head + (long)d * a.dv + v0 + col] = s[i][e];
+      if (d < a.dk) a.state[((long)out * a.nv + h) * head + (long)d * a.dv + v0 + j] = s[i][e];
     }
 }
 
@@ -965,7 +965,6 @@ bool chunked(const MxGatedDelta* d) {
 
 template <int DK, bool FULL, typename XT>
 int launch_chunked(const GdArgs& a, char* ws, hipStream_t s) {
-  constexpr int NT = 1;
   const int slots = a.rows / kC + a.n_seqs;
   char* rows_ws = ws + (size_t)slots * a.nv * kRec;
   mx_clear_error();
@@ -973,7 +972,7 @@ int launch_chunked(const GdArgs& a, char* ws, hipStream_t s) {
   hipLaunchKernelGGL((k_gd_prep<DK, FULL, XT>), dim3(pieces * a.n_seqs + slots, a.nv), dim3(256), 0, s, a, ws, rows_ws,
                      kFrom, pieces, slots);
   MX_TRY(mx_launch_status());
-  hipLaunchKernelGGL((k_gd_walk<DK, NT, XT>), dim3(mx_ceil_div(a.dv, 16 * NT) * a.nv, a.n_seqs), dim3(256 * NT), 0, s, a,
+  hipLaunchKernelGGL((k_gd_walk<DK, XT>), dim3(mx_ceil_div(a.dv, 16) * a.nv, a.n_seqs), dim3(256), 0, s, a,
                      ws, rows_ws, kFrom, a.nk % 8 == 0);
   return mx_launch_status();
 }
