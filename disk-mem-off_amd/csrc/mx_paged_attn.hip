@@ -77,9 +77,12 @@ __device__ __forceinline__ int pa_lane() {
 // a tile's keys into ranges of `len` keys; an item is one range of one tile.  Every block works
 // the same schedule out of the batch's lengths: len such that about `target` items of equal
 // size come out (sum over the tiles of their keys / target, within [least, most]), the items in
-// order of sequence, range, tile (last tile first).  The blocks of a head take its items in turn.
+// order of sequence, range, tile.  A tile's ranges are as long as each other, in 128 keys (12 ragged
+// chunks over up to 7000 keys: 132 us, 138 with a short last range), and the tiles of every other range come
+// in the other order, so that a CU's two blocks get a long and a short one of a causal chunk (2048
+// rows over 8192 keys: 260 us, 269).  The blocks of a head take its items in turn.
 // An item whose tile fits one range writes its rows; the others leave sums, relative to their
-// reference, in the slot of their number for k_pa_join.
+// reference, in a slot for k_pa_join.
 struct PaSched {
   int target, least, most;
   int slots;     // at most so many items of a head
@@ -108,8 +111,8 @@ struct PaTile {
   int pos0;              // position of the sequence's row 0
   int kend;              // keys the tile's last row sees
   int k0;                // first key of the range
-  int ranges;            // ranges of the tile
-  int tiles;             // tiles of the sequence
+  int len, ranges;       // keys of its ranges, how many
+  int slot, tiles;       // the range's slot for sums; the tile's next range's is `tiles` further
 };
 
 template <int RT>
@@ -162,6 +165,7 @@ __device__ __forceinline__ PaWork pa_schedule(const PkBatch& b, const PkCache& c
   w.items = __builtin_amdgcn_readlane(w.incl, 63);
   for (int s = 64 + lane; s - lane < b.n_seqs; s += 64)
     w.items += __builtin_amdgcn_readlane(pa_scan(pa_items(pa_seq<RT>(b, c, group, s), w.len)), 63);
+  w.items = min(w.items, sp.slots);
   return w;
 }
 
@@ -206,16 +210,19 @@ __device__ __forceinline__ bool pa_item(const PkBatch& b, const PkCache& c, int 
                                         PaTile* t) {
   int before;
   const PaSeq q = pa_locate<RT>(b, c, group, w, item, &t->seq, &before);
-  const int z = (item - before) / q.tiles, tile = q.tiles - 1 - (item - before - z * q.tiles);
+  const int z = (item - before) / q.tiles, i = item - before - z * q.tiles, tile = z & 1 ? i : q.tiles - 1 - i;
+  t->slot = before + (z + 1) * q.tiles - 1 - tile;
   t->first = q.q0;
   t->row0 = tile * RT;
   t->nrows = q.m * group;
   t->pos0 = q.len - q.m;
   t->kend = pa_kend<RT>(q, t->row0, group);
-  t->k0 = z * w.len;
-  t->ranges = max(1, pa_ceil(t->kend, w.len));
+  const int n = max(1, pa_ceil(t->kend, w.len));  // at most; rounded up, fewer may do
+  t->len = (pa_ceil(t->kend, n) + 127) & ~127;
+  t->k0 = z * t->len;
+  t->ranges = min(n, max(1, pa_ceil(t->kend, t->len)));
   t->tiles = q.tiles;
-  return z < t->ranges;
+  return z < t->ranges && t->slot < w.items;
 }
 
 // The page ids of 64 sub-tiles, one per lane (the one that holds key `key`), and which of them
@@ -249,7 +256,10 @@ __device__ __forceinline__ bool pa_direct(const PkBatch& b, const PkCache& c, in
   t->pos0 = n - m;
   t->kend = (int)max(0l, min((long)min(n, b.max_kv), (long)b.max_pages << c.ps_log));
   t->k0 = z * len;
+  t->len = len;
   t->ranges = max(1, pa_ceil(t->kend, len));
+  t->tiles = b.n_seqs;
+  t->slot = z * b.n_seqs + s;
   return m > 0 && z < t->ranges;
 }
 
@@ -521,7 +531,6 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
   } else {
     pa_head_of(c.nkv, &kvh, &first);
     work = pa_schedule<kKeysRows>(b, c, sp, a.group);
-    work.items = min(work.items, sp.slots);
   }
   for (int item = first; DIRECT || item < work.items; item += per) {
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
     if (!pa_item<kKeysRows>(b, c, a.group, work, item, &t)) continue;
     ids = pa_ids(b, c, t.seq, t.k0 + mine);
   }
-  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
+  const int k0 = t.k0, k1 = min(t.kend, k0 + t.len);
 
   const int row = min(t.row0 + j, t.nrows - 1);
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
@@ -724,9 +733,9 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
     }
     const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
     const long tr = t.first + rt;
-    const int at = (kvh * sp.slots + item) * kKeysRows + r;
+    const int at = (kvh * sp.slots + t.slot) * kKeysRows + r;
     if (k0 == 0 && d == 0)
-      sp.rows[tr * a.nh + h] = (int4_t){at, (DIRECT ? b.n_seqs : t.tiles) * kKeysRows, t.ranges, 0};
+      sp.rows[tr * a.nh + h] = (int4_t){at, t.tiles * kKeysRows, t.ranges, 0};
     if (t.ranges > 1) {
       *(float4_t*)(sp.po + (long)at * c.hd + d) = s;
       if (d == 0) sp.ml[at] = make_float2(mr, l);
@@ -867,12 +876,12 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
   now.target = pa_opaque_s(sp.target);
   const int group = pa_opaque_s(a.group);
   const PaWork work = pa_schedule<RT>(b, c, now, group);
-  if (item >= min(work.items, sp.slots)) return;
+  if (item >= work.items) return;
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
   const int lane = pa_lane(), j = lane & 15, g = lane >> 4;
   PaTile t;
   if (!pa_item<RT>(b, c, group, work, item, &t)) continue;
-  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
+  const int k0 = t.k0, k1 = min(t.kend, k0 + t.len);
   PaIds ids = pa_ids(b, c, t.seq, k0 + 16 * lane);
   const int ntile = pa_ceil(max(0, k1 - k0), 32);
 
@@ -1088,7 +1097,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
     int tok, hq;
     where(u, tok, hq);
     const long tr = t.first + tok;
-    const int at = (kvh * sp.slots + item) * RT + (w0 - t.row0) + 16 * u + j1;
+    const int at = (kvh * sp.slots + t.slot) * RT + (w0 - t.row0) + 16 * u + j1;
     if (k0 == 0 && g1 == 0) sp.rows[tr * a.nh + hq] = (int4_t){at, t.tiles * RT, t.ranges, 0};
     if (t.ranges > 1) {
 #pragma unroll
@@ -1139,7 +1148,6 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
   } else {
     pa_head_of(c.nkv, &kvh, &first);
     work = pa_schedule<kKeysRows>(b, c, sp, a.group);
-    work.items = min(work.items, sp.slots);
   }
   for (int item = first; DIRECT || item < work.items; item += per) {
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
@@ -1153,7 +1161,7 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
     if (!pa_item<kKeysRows>(b, c, a.group, work, item, &t)) continue;
     ids = pa_ids(b, c, t.seq, t.k0 + mine);
   }
-  const int k0 = t.k0, k1 = min(t.kend, k0 + work.len);
+  const int k0 = t.k0, k1 = min(t.kend, k0 + t.len);
   const int row = min(t.row0 + j, t.nrows - 1);
   const int tok = row / a.group, hq = kvh * a.group + row - tok * a.group;
   const int pos = t.pos0 + tok;
@@ -1320,9 +1328,9 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
     }
     const int rt = (t.row0 + r) / a.group, h = kvh * a.group + (t.row0 + r) - rt * a.group;
     const long tr = t.first + rt;
-    const int at = (kvh * sp.slots + item) * kKeysRows + r;
+    const int at = (kvh * sp.slots + t.slot) * kKeysRows + r;
     if (k0 == 0 && d == 0)
-      sp.rows[tr * a.nh + h] = (int4_t){at, (DIRECT ? b.n_seqs : t.tiles) * kKeysRows, t.ranges, 0};
+      sp.rows[tr * a.nh + h] = (int4_t){at, t.tiles * kKeysRows, t.ranges, 0};
     if (t.ranges > 1) {
       *(float4_t*)(sp.po + (long)at * c.hd + d) = s;
       if (d == 0) sp.ml[at] = make_float2(mr, l);
