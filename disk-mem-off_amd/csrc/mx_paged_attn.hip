@@ -73,11 +73,13 @@ __device__ __forceinline__ int pa_lane() {
   return pa_opaque(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)));
 }
 
+constexpr int kKeysRows = 16;
+
 // Work items.  A call's rows are cut into row tiles (RT rows of one sequence and key/value head) and
 // a tile's keys into ranges of `len` keys; an item is one range of one tile.  Every block works
 // the same schedule out of the batch's lengths: len such that about `target` items of equal
 // size come out (sum over the tiles of their keys / target, within [least, most]), the items in
-// order of sequence, range, tile.  A tile's ranges are as long as each other, in 128 keys (12 ragged
+// order of sequence, range, tile.  A tile's ranges are as long as each other, in whole steps (12 ragged
 // chunks over up to 7000 keys: 132 us, 138 with a short last range), and the tiles of every other range come
 // in the other order, so that a CU's two blocks get a long and a short one of a causal chunk (2048
 // rows over 8192 keys: 260 us, 269).  The blocks of a head take its items in turn.
@@ -86,6 +88,7 @@ __device__ __forceinline__ int pa_lane() {
 struct PaSched {
   int target, least, most;
   int slots;     // at most so many items of a head
+  int end;       // rows of sums in all
   float* po;     // [nkv][slots][RT][hd]
   float2* ml;    // [nkv][slots][RT]: reference, sum
   int4_t* rows;  // [rows][nh]: where a row's first partial sum lies in them, the step to the next, how many
@@ -144,7 +147,8 @@ __device__ __forceinline__ int pa_items(const PaSeq& q, int len) {
 
 // The schedule (wave-uniform but for `own`; callers converged).
 template <int RT>
-__device__ __forceinline__ PaWork pa_schedule(const PkBatch& b, const PkCache& c, const PaSched& sp, int group) {
+__device__ __forceinline__ PaWork pa_schedule(const PkBatch& b, const PkCache& c, const PaSched& sp, int group,
+                                              int per) {
   const int lane = pa_lane();
   PaWork w;
   w.own = pa_seq<RT>(b, c, group, lane);
@@ -156,15 +160,25 @@ __device__ __forceinline__ PaWork pa_schedule(const PkBatch& b, const PkCache& c
   }
   total = mx_wave_sum(total) * (float)c.nkv;
   tiles = mx_wave_sum(tiles);
-  // Every tile rounds its last range up: half an item each is set aside for that.
-  const float room = max((float)sp.target - 0.5f * tiles * (float)c.nkv, 0.5f * (float)sp.target);
-  const float each = min(total / room, 1.0e9f);
-  w.len = max(sp.least, min(sp.most, ((int)each + 128) & ~127));
-  w.own.items = pa_items(w.own, w.len);
-  w.incl = pa_scan(w.own.items);
-  w.items = __builtin_amdgcn_readlane(w.incl, 63);
-  for (int s = 64 + lane; s - lane < b.n_seqs; s += 64)
-    w.items += __builtin_amdgcn_readlane(pa_scan(pa_items(pa_seq<RT>(b, c, group, s), w.len)), 63);
+  // Every tile rounds its last range up: half an item each is set aside for that.  k_pa_keys and k_pa_f32,
+  // bound by the copies that a block has in flight, let the ranges grow instead until one item per block is
+  // enough, where there are no more tiles than blocks (48 ragged sequences of up to 12000 keys in fp16:
+  // 32 us, 44 with a second item for some).
+  const int most = min(per, sp.slots);
+  const bool fits = RT == kKeysRows && tiles <= (float)most;
+  const int unit = fits ? 64 : 128;
+  const float room = fits ? (float)sp.target : max((float)sp.target - 0.5f * tiles * (float)c.nkv, 0.5f * (float)sp.target);
+  const int each = (int)min(total / room, 1.0e9f);
+  w.len = max(sp.least, min(sp.most, (each + unit) / unit * unit));
+  for (;;) {
+    w.own.items = pa_items(w.own, w.len);
+    w.incl = pa_scan(w.own.items);
+    w.items = __builtin_amdgcn_readlane(w.incl, 63);
+    for (int s = 64 + lane; s - lane < b.n_seqs; s += 64)
+      w.items += __builtin_amdgcn_readlane(pa_scan(pa_items(pa_seq<RT>(b, c, group, s), w.len)), 63);
+    if (!fits || w.items <= most || w.len >= sp.most) break;
+    w.len = min(sp.most, w.len + max(unit, w.len / 16 / unit * unit));
+  }
   w.items = min(w.items, sp.slots);
   return w;
 }
@@ -218,7 +232,8 @@ __device__ __forceinline__ bool pa_item(const PkBatch& b, const PkCache& c, int 
   t->pos0 = q.len - q.m;
   t->kend = pa_kend<RT>(q, t->row0, group);
   const int n = max(1, pa_ceil(t->kend, w.len));  // at most; rounded up, fewer may do
-  t->len = (pa_ceil(t->kend, n) + 127) & ~127;
+  constexpr int unit = RT == kKeysRows ? 64 : 128;
+  t->len = (pa_ceil(t->kend, n) + unit - 1) / unit * unit;
   t->k0 = z * t->len;
   t->ranges = min(n, max(1, pa_ceil(t->kend, t->len)));
   t->tiles = q.tiles;
@@ -509,7 +524,6 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
 // their way from the moment this tile's scores are formed, its values from the moment this
 // tile's are used.  No barrier until the waves' sums are put together at the end.
 // ------------------------------------------------------------------------------------
-constexpr int kKeysRows = 16;
 constexpr int kKeysMax = 4096;  // keys of a split: 64 sub-tile page ids per wave
 
 template <int RB, int DT, bool DIRECT>
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
     work.len = sp.least;
   } else {
     pa_head_of(c.nkv, &kvh, &first);
-    work = pa_schedule<kKeysRows>(b, c, sp, a.group);
+    work = pa_schedule<kKeysRows>(b, c, sp, a.group, per);
   }
   for (int item = first; DIRECT || item < work.items; item += per) {
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
@@ -773,7 +787,8 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
   const int4_t where = sp.rows[(long)t * a.nh + h];
   if (t >= b.q_start[b.n_seqs]) return;  // behind the last sequence
   const int ranges = __builtin_amdgcn_readfirstlane(where[2]);
-  if (ranges <= 1) return;
+  // (a row that no sequence has, or two have, left no place for its sums)
+  if (ranges <= 1 || where[0] < 0 || where[1] < 0 || where[0] + (ranges - 1l) * where[1] >= sp.end) return;
   // This wave's: every 4th range, or all of them.
   constexpr int HOP = WIDE ? 4 : 1;
   const int n = WIDE ? (ranges - wave + 3) / 4 : ranges;
@@ -875,7 +890,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
   PaSched now = sp;
   now.target = pa_opaque_s(sp.target);
   const int group = pa_opaque_s(a.group);
-  const PaWork work = pa_schedule<RT>(b, c, now, group);
+  const PaWork work = pa_schedule<RT>(b, c, now, group, per);
   if (item >= work.items) return;
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
   const int lane = pa_lane(), j = lane & 15, g = lane >> 4;
@@ -1147,7 +1162,7 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
     work.len = sp.least;
   } else {
     pa_head_of(c.nkv, &kvh, &first);
-    work = pa_schedule<kKeysRows>(b, c, sp, a.group);
+    work = pa_schedule<kKeysRows>(b, c, sp, a.group, per);
   }
   for (int item = first; DIRECT || item < work.items; item += per) {
   // Opaque: what follows from the lane is worked out per item and holds nothing across the loop.
@@ -1494,7 +1509,7 @@ extern "C" int mx_paged_attn(const MxKvCache* cache, const MxPagedBatch* batch,
   const PaArgs a{args->q, args->out, args->gate, args->ldq, args->ldo, args->ldg, args->n_heads,
                  args->n_heads / cache->n_kv_heads, args->scale};
   char* const ws = (char*)workspace;
-  const PaSched sp{p.target, p.least, p.most, p.slots, (float*)ws, (float2*)(ws + p.ml), (int4_t*)(ws + p.row)};
+  const PaSched sp{p.target, p.least, p.most, p.slots, p.slots * c.nkv * p.rt, (float*)ws, (float2*)(ws + p.ml), (int4_t*)(ws + p.row)};
   const hipStream_t s = (hipStream_t)stream;
   if (cache->dtype == MX_DT_F32)
     return p.direct ? launch<MX_DT_F32, true>(p, c, b, a, sp, s) : launch<MX_DT_F32, false>(p, c, b, a, sp, s);
