@@ -572,8 +572,8 @@ typedef struct MxPagedAttn {
   int32_t n_heads;
   float scale;
 } MxPagedAttn;
-/* Bytes of workspace of such a call (16-byte aligned; partial results of split key ranges).
- * Calls that may overlap need a workspace each.                                        */
+/* Bytes of workspace of such a call (16-byte aligned; sums of split key ranges and where each row's
+ * lie).  What is in it before does not matter.  Calls that may overlap need a workspace each. */
 int mx_paged_attn_workspace_size(const MxKvCache* cache, const MxPagedBatch* batch,
                                  int32_t n_heads, size_t* nbytes);
 int mx_paged_attn(const MxKvCache* cache, const MxPagedBatch* batch, const MxPagedAttn* args,
@@ -633,8 +633,11 @@ typedef struct MxGatedDelta {
   int32_t qk_norm;
   float scale;
 } MxGatedDelta;
-/* Workspace (16-byte aligned) of such a call: 0 where the recurrence runs token by token.
- * Calls that may overlap need a workspace each.                                        */
+/* Sequences of 24 rows and more go chunk by chunk (64 tokens, products at fp32 precision) where max_q
+ * and rows allow such sequences, head_dim_k <= 128 and ldv, ldo < 2^23; all others token by token.
+ * Workspace (16-byte aligned) of such a call: 0 where all go token by token; else it grows with
+ * rows + 64 n_seqs.  What is in it before does not matter.  Calls that may overlap need a
+ * workspace each.                                                                      */
 int mx_gated_delta_rule_workspace_size(const MxGatedDelta* args, size_t* nbytes);
 int mx_gated_delta_rule(const MxGatedDelta* args, void* workspace, size_t workspace_bytes,
                         void* stream);
