@@ -798,6 +798,8 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
   const long step = (long)HOP * __builtin_amdgcn_readfirstlane(where[1]);
   const int d = min(4 * lane, c.hd - 4);
   const float* po = sp.po + at * c.hd + d;
+  float4 gv = make_float4(0.f, 0.f, 0.f, 0.f);  // on its way with the sums
+  if (a.gate) gv = *(const float4*)(a.gate + (long)t * a.ldg + (long)h * c.hd + d);
   float mr = kLow, l = 0.f;
   float4_t s = {0.f, 0.f, 0.f, 0.f};
   // 64 ranges at a time: lane z holds range z's reference and sum, whose weights all lanes
@@ -846,7 +848,6 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
   if (4 * lane >= c.hd) return;
   s *= l == 0.f ? 0.f : 1.f / l;
   if (a.gate) {
-    const float4 gv = *(const float4*)(a.gate + (long)t * a.ldg + (long)h * c.hd + d);
     s = (float4_t){s[0] * mx_sigmoid(gv.x), s[1] * mx_sigmoid(gv.y), s[2] * mx_sigmoid(gv.z),
                    s[3] * mx_sigmoid(gv.w)};
   }
@@ -1150,7 +1151,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
 // rows, keys dealt to the waves 16 at a time, keys in registers, values through the wave's LDS
 // buffers.  The MFMA k-slot of lane group g at step r is key 4 g + r on both operands.  Bound by those
 // instructions (a sixteenth of fp16's rate) and, in small calls, by their latency: 3 x 130 rows over 1500 tokens,
-// 16 heads over 2 of 128: 134 us, 69 TFLOP/s.
+// 32 heads over 8 of 128: 134 us, 68 TFLOP/s.
 // ------------------------------------------------------------------------------------
 template <int DP, bool DIRECT>
 __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
