@@ -281,3 +281,57 @@ def test_a_token_that_is_not_finite_leaves_those_before_it(mi355x, stream, n, at
     ok, good = np.isfinite(wo), np.isfinite(ws)
     assert off(s[good], ws[good]) <= tol
     assert off(o[ok], wo[ok]) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("nk,nv,dk,dv,news", [
+    (1, 2, 32, 40, [70]), (1, 1, 4, 4, [65]), (3, 3, 100, 12, [30, 90]), (2, 6, 64, 24, [64, 25]),
+    (8, 8, 128, 256, [40]), (1, 4, 124, 132, [129])])
+def test_chunks_of_odd_heads(mi355x, stream, nk, nv, dk, dv, news, dtype):
+    """Head sizes that fill no tile, in sequences that go chunk by chunk."""
+    say(f"delta rule heads={nk}/{nv} dk={dk} dv={dv} rows={news} {dtype}")
+    rng = np.random.default_rng(dk * dv)
+    x = make(rng, news, nk, nv, dk, dv, dtype, pad=1)
+    state = (rng.standard_normal((3, nv, dk, dv)) * 0.3).astype(np.float32)
+    io = list(range(len(news)))
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, dtype, state, io, io, pads=(0, 0, 0, 4))
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, io, io, dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    assert off(s, ws) <= tol and off(o[:sum(news)], wo) <= tol + (2.0 ** -11 if dtype == "float16" else 0.0)
+    assert np.array_equal(s[len(news):], state[len(news):])
+
+
+@pytest.mark.parametrize("news", [[3], [70]])
+def test_state_slots_behind_four_gigabytes(mi355x, stream, news):
+    """The last slots of more than 2^32 bytes of states, out of one call and into the next."""
+    say(f"delta rule, far slots, rows={news}")
+    nk, nv, dk, dv = 2, 4, 128, 128
+    slots = (5 << 30) // (nv * dk * dv * 4)
+    rng = np.random.default_rng(3)
+    x = make(rng, [2 * news[0]], nk, nv, dk, dv, "float32")
+    n = news[0]
+    buf = mi355x.alloc_device(slots * nv * dk * dv * 4)
+    runner = GatedDeltaRunner(mi355x)
+    try:
+        with sv.Arrays(mi355x, stream) as ar:
+            o0 = np.zeros((n, nv, dv), np.float32)
+            got = []
+            for i, (a, b) in enumerate([(-1, slots - 1), (slots - 1, slots - 2)]):
+                q, k, v, g, beta = (ar.put(t[i * n:(i + 1) * n]) for t in x)
+                po = ar.put(o0)
+                ids = np.array([a], np.int32), np.array([b], np.int32)
+                args = delta_args(q=q, k=k, v=v, g=g, beta=beta, o=po, state=int(buf.handle),
+                                  slot_in=ar.put(ids[0]), slot_out=ar.put(ids[1]),
+                                  q_start=ar.put(np.array([0, n], np.int32)), n_slots=slots, n_seqs=1, rows=n,
+                                  max_q=n, n_k_heads=nk, n_v_heads=nv, head_dim_k=dk, head_dim_v=dv,
+                                  dtype="float32")
+                runner.reserve(args)
+                runner.forward_device(args, stream)
+                got.append(ar.get(po, o0))
+    finally:
+        mi355x.synchronize_stream(stream)
+        runner.close()
+        mi355x.free_device(buf)
+    zero = np.zeros((1, nv, dk, dv), np.float32)
+    wo, _ = want_of(x, [2 * n], nk, nv, dk, dv, zero, [0], [0], dk ** -0.5)
+    assert off(np.concatenate(got), wo) <= 2 * (2 * dk + 64) * 2.0 ** -24

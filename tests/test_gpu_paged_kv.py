@@ -419,3 +419,50 @@ def test_long_caches(mi355x, stream, news, lens, dtype):
     b = sv.Batch(np.random.default_rng(1), news, lens, 64)
     got, want, tol = check_attention(mi355x, stream, b, 4, 1, 64, dtype, 2)
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("news", [[100], [1]])
+def test_pages_behind_four_gigabytes(mi355x, stream, dtype, news):
+    """Pages at the end of a pool of more than 2^32 bytes: written by append, copied, attended to."""
+    nh, nkv, hd, page = 4, 2, 128, 64
+    esz = np.dtype(sv.DT[dtype]).itemsize
+    n_pages = (5 << 30) // (nkv * page * hd * esz)
+    say(f"attention over the last of {n_pages} pages, {dtype} {news}")
+    rng = np.random.default_rng(6)
+    b = sv.Batch(rng, news, [100], page, spare=0)
+    x = rng.standard_normal((100, nkv * hd)).astype(sv.DT[dtype])
+    q = rng.standard_normal((news[0], nh, hd)).astype(sv.DT[dtype])
+    pool = np.zeros((b.n_pages, nkv, page, hd), sv.DT[dtype])
+    at = np.arange(100)
+    pool[b.table[0, at // page], :, at % page] = x.reshape(100, nkv, hd)
+    want, mag, big = sv.attention(b, q, pool.astype(np.float64), pool.astype(np.float64), nkv, hd ** -0.5)
+    far = n_pages - 2 * b.n_pages  # append there, copy behind, attend to the copies
+    bufs = [mi355x.alloc_device(n_pages * nkv * page * hd * esz) for _ in range(2)]
+    try:
+        with sv.Arrays(mi355x, stream) as ar:
+            cache = PagedKvCache(mi355x, 1, nkv, hd, n_pages, page_size=page, dtype=dtype,
+                                 buffers=[(int(bufs[0].handle), int(bufs[1].handle), None, None)])
+            fill = sv.Batch(rng, [100], [100], page, spare=0)
+            fill.table = b.table + far
+            px, pq, o = ar.put(x), ar.put(q), np.zeros_like(q)
+            po = ar.put(o)
+            cache.append(0, fill.device(ar), append_args(k=px, v=px, n_kv_heads=nkv, head_dim=hd, dtype=dtype),
+                         stream)
+            src = np.arange(far, far + b.n_pages, dtype=np.int32)
+            copy_pages(cache.pools, ar.put(src), ar.put(src + b.n_pages), len(src), stream)
+            b.table = b.table + far + b.n_pages
+            db = b.device(ar)
+            cache.reserve_attn(db, nh)
+            cache.attend(0, db, attn_args(pq, po, n_heads=nh, head_dim=hd), stream)
+            got = ar.get(po, o).astype(np.float64)
+            cache.close()
+    finally:
+        mi355x.synchronize_stream(stream)
+        for buf in bufs:
+            mi355x.free_device(buf)
+    if dtype == "float32":
+        tol = mag * 2.0 ** -24 * (2 * 10 + 8 * hd) + 1e-30
+    else:
+        tol = mag * (2.0 ** -11 + 2.0 ** -13) + 2.0 ** -11 * np.abs(want) + 100 * 2.0 ** -25 * big + 1e-7
+    assert np.all(np.abs(got - want) <= tol)
