@@ -225,10 +225,10 @@ __device__ __forceinline__ float4_t gd_mfma(const float4_t& a, const float4_t& b
   return c;
 }
 
-// 2^-e and 2^e with m 2^-e in [2^14, 2^15): fp16 holds twice that.  Under 2^-86 they stay; an
+// 2^-e and 2^e with m 2^-e in [2^14, 2^15): fp16 holds twice that.  Under 2^-112 they stay; an
 // infinite or NaN m gives a finite factor.
 __device__ __forceinline__ float gd_scale(float m, float& inv) {
-  const int e = max((int)((__float_as_uint(m) >> 23) & 255), 41);
+  const int e = max((int)((__float_as_uint(m) >> 23) & 255), 15);
   inv = __uint_as_float((uint32_t)(e - 14) << 23);
   return __uint_as_float((uint32_t)(268 - e) << 23);
 }

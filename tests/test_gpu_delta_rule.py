@@ -335,3 +335,22 @@ def test_state_slots_behind_four_gigabytes(mi355x, stream, news):
     zero = np.zeros((1, nv, dk, dv), np.float32)
     wo, _ = want_of(x, [2 * n], nk, nv, dk, dv, zero, [0], [0], dk ** -0.5)
     assert off(np.concatenate(got), wo) <= 2 * (2 * dk + 64) * 2.0 ** -24
+
+
+def test_a_state_that_faded_keeps_its_digits(mi355x, stream):
+    """States of 2^-70, chunks that add nothing to them (beta 0) and chunks that do."""
+    say("delta rule, faded states")
+    nk, nv, dk, dv, news = 1, 2, 64, 32, [200, 20]
+    rng = np.random.default_rng(30)
+    q, k, v, g, beta = x = make(rng, news, nk, nv, dk, dv, "float32")
+    v *= np.float32(2.0 ** -70)
+    beta[:130] = 0.0
+    beta[200:210] = 0.0
+    g *= np.float32(0.01)
+    state = (rng.standard_normal((2, nv, dk, dv)) * 2.0 ** -70).astype(np.float32)
+    o, s = run(mi355x, stream, x, news, nk, nv, dk, dv, "float32", state, [0, 1], [0, 1])
+    wo, ws = want_of(x, news, nk, nv, dk, dv, state, [0, 1], [0, 1], dk ** -0.5)
+    tol = (2 * dk + 64) * 2.0 ** -24
+    assert off(s, ws) <= tol and off(o, wo) <= tol
+    for r in range(0, 220, 20):  # every stretch to its own size
+        assert off(o[r:r + 20], wo[r:r + 20]) <= tol
