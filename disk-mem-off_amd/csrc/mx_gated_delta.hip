@@ -637,7 +637,18 @@ __global__ __launch_bounds__(256, 2) void k_gd_walk(GdArgs a, const char* __rest
   __shared__ __align__(16) float sf[2][kFactors * kC];
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rt = wave;
-  const int seq = blockIdx.y;
+  int seq = blockIdx.y;
+  // The longest first: the last to end sets the time (8 ragged prompts of up to 600 rows: 81 us, 92 as they
+  // come).  More than a wave looks at in one go come as they are.
+  if (a.n_seqs > 1 && a.n_seqs <= 64) {
+    const int at = min(lane, a.n_seqs - 1), size = min(a.q_start[at + 1], a.rows) - a.q_start[at];
+    int before = 0;
+    for (int i = 0; i < a.n_seqs; ++i) {
+      const int other = __builtin_amdgcn_readlane(size, i);
+      before += other > size || (other == size && i < lane);
+    }
+    seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.n_seqs && before == (int)blockIdx.y));
+  }
   // Slices of a key head's value heads next to each other on one XCD: they read the same k, q, T, P.
   int hk, r;
   const int slices = (a.dv + NC - 1) / NC, per = slices * a.rep;
