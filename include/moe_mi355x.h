@@ -491,7 +491,7 @@ int mx_gated_delta_scan_ws(const float* q, const float* kb, const float* v,
 
 /* The keys and values of one layer, in pages of page_size tokens:
  * k, v [n_pages, n_kv_heads, page_size, head_dim] of dtype F32, F16 or I8 (16-byte aligned);
- * int8 rows stand for int8 * scale with one fp32 scale per row in k_scale, v_scale
+ * int8 rows stand for int8 * scale with one fp32 scale (finite, >= 0) per row in k_scale, v_scale
  * [n_pages, n_kv_heads, page_size] (16-byte aligned; NULL for the other types).
  * page_size: 16, 32, 64, 128 or 256.  head_dim: a multiple of 8 (I8: 16), <= 256.      */
 typedef struct MxKvCache {
