@@ -233,7 +233,7 @@ __device__ __forceinline__ bool pa_item(const PkBatch& b, const PkCache& c, int 
   t->kend = pa_kend<RT>(q, t->row0, group);
   const int n = max(1, pa_ceil(t->kend, w.len));  // at most; rounded up, fewer may do
   constexpr int unit = RT == kKeysRows ? 64 : 128;
-  t->len = (pa_ceil(t->kend, n) + unit - 1) / unit * unit;
+  t->len = max(unit, (pa_ceil(t->kend, n) + unit - 1) / unit * unit);
   t->k0 = z * t->len;
   t->ranges = min(n, max(1, pa_ceil(t->kend, t->len)));
   t->tiles = q.tiles;
