@@ -78,6 +78,25 @@ __device__ __forceinline__ float mx_wave_max(float v) {
                fmaxf(mx_readlane(v, 32), mx_readlane(v, 48)));
 }
 
+// Both operands of a lane swap: v_permlane16_swap exchanges the odd 16-lane rows of x with
+// the even ones of y, v_permlane32_swap the upper half of x with the lower half of y.  With x = y
+// = v the two hold v of the lane and of its partner.  (A bit cast of the second result of the
+// compiler's builtins is folded into the first: a maximum over both is the first alone.)  s_nop: the swap's operands were just written.
+__device__ __forceinline__ void mx_swap16(float& x, float& y) {
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
+__device__ __forceinline__ void mx_swap32(float& x, float& y) {
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
+// Max over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float mx_rowmax4(float v) {
+  float x = v, y = v;
+  mx_swap16(x, y);
+  x = y = fmaxf(x, y);
+  mx_swap32(x, y);
+  return fmaxf(x, y);
+}
+
 // Reference silu: x / (1 + exp(-x))  (_common.py:83-84).
 __device__ __forceinline__ float mx_silu(float x) { return x / (1.0f + expf(-x)); }
 

@@ -806,19 +806,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(FA_H_WP
 #endif
 #define FA_D_RESIDENT 512  // blocks that run at once: two on each of 256 CUs
 
-// Max over the lanes l, l ^ 16, l ^ 32 and l ^ 48 (one query's four lane groups) without
-// going through LDS: permlane16_swap exchanges 16-lane rows 2k and 2k + 1 between its two
-// operands and permlane32_swap the wave's halves, so with both operands v the two results
-// hold v of the lane and of its partner row (half).
-__device__ __forceinline__ float fa_rowmax4(float v) {
-  const unsigned b = __builtin_bit_cast(unsigned, v);
-  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-  v = fmaxf(__builtin_bit_cast(float, r[0]), __builtin_bit_cast(float, r[1]));
-  const unsigned c = __builtin_bit_cast(unsigned, v);
-  const auto h = __builtin_amdgcn_permlane32_swap(c, c, false, false);
-  return fmaxf(__builtin_bit_cast(float, h[0]), __builtin_bit_cast(float, h[1]));
-}
-
 template <int NC, int NW, int QS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(FA_D_WPE, FA_D_WPE)))
 void k_fa_attn_d(const float* __restrict__ qg, const half_t* __restrict__ k16,
@@ -1023,7 +1010,7 @@ void k_fa_attn_d(const float* __restrict__ qg, const half_t* __restrict__ k16,
                              fmaxf(sc[u][0][0][2], sc[u][0][0][3])),
                        fmaxf(fmaxf(sc[u][1][0][0], sc[u][1][0][1]),
                              fmaxf(sc[u][1][0][2], sc[u][1][0][3])));
-      mt = fa_rowmax4(mt);
+      mt = mx_rowmax4(mt);  // the query's four lane groups
       // Lazy rescale: a query's reference max moves only when the tile's max passes it by
       // more than FA_D_TAU (base-2 units), so the probabilities stay below 2^FA_D_TAU (fp16
       // holds them) and the accumulators are rescaled on few tiles.  Tile 0 holds key 0,

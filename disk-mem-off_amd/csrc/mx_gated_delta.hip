@@ -107,11 +107,11 @@ __device__ void gd_recurrent(const GdArgs& a, GdRecLds<NR>& lds, int piece, int 
       float x[4] = {r.x, r.y, r.z, r.w}, y[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        pk_swap32(x[e], y[e]);
+        mx_swap32(x[e], y[e]);
         x[e] += y[e];  // r in the lower half of the lanes, p in the upper
       }
-      pk_swap16(x[0], x[2]);
-      pk_swap16(x[1], x[3]);
+      mx_swap16(x[0], x[2]);
+      mx_swap16(x[1], x[3]);
       float2 z = make_float2(x[0] + x[2], x[1] + x[3]);  // columns 0, 1 in the even rows, 2, 3 in the odd
       z.x += mx_dpp<0x128>(z.x);  // row_ror:8
       z.y += mx_dpp<0x128>(z.y);
@@ -430,8 +430,8 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
       }
     k2 = gd_sum16(k2);
     q2 = gd_sum16(q2);
-    km = pk_rowmax(km);
-    qm = pk_rowmax(qm);
+    km = mx_rowmax4(km);
+    qm = mx_rowmax4(qm);
     float ki, qi;
     const float ks = gd_scale(km, ki), qs = gd_scale(qm, qi);
     if (h == hk * a.rep) {  // k and q for all value heads of theirs
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void k_gd_walk(GdArgs a, const char* __rest
   const int k_get = (4 * q + (j >> 2)) * DK + (((2 * SL * rt + ((j & 3) >> 1)) ^ (2 * (j >> 2) + (q & 1))) << 3) + (j & 1) * 4;
   auto put = [&](half_t (&to)[2][NC * kC], const float4_t& x, float (&inv)[4][NC]) {
     float iv;
-    const float sc = gd_scale(pk_rowmax(gd_max4(x)), iv);
+    const float sc = gd_scale(mx_rowmax4(gd_max4(x)), iv);
     half4_t p[2];
     gd_split<4>((const float*)&x, sc, (half_t*)&p[0], (half_t*)&p[1]);
     *(half4_t*)&to[0][pieces_rt] = p[0];
@@ -791,7 +791,7 @@ __global__ __launch_bounds__(256, 2) void k_gd_walk(GdArgs a, const char* __rest
   float bound = 0.f;
 #pragma unroll
   for (int i = 0; i < SL; ++i) bound = fmaxf(bound, gd_max4(s[i]));
-  bound = pk_rowmax(bound);
+  bound = mx_rowmax4(bound);
   if (q == 0) smax[1][rt][j] = bound;
   if (tid < NC) sfirst[0][tid] = kC;
   if (tid < kFactors * kC / 4) *(float4*)&sf[0][4 * tid] = ff;
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256, 2) void k_gd_walk(GdArgs a, const char* __rest
         *(half4_t*)&ss[1][at] = p[1];
         m = fmaxf(m, gd_max4(s[i]));
       }
-      m = pk_rowmax(m);
+      m = mx_rowmax4(m);
       if (q == 0) smax[c & 1][rt][j] = m;
     }
     __syncthreads();

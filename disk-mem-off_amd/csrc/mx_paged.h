@@ -64,26 +64,6 @@ static inline PkBatch pk_batch(const MxPagedBatch* b) {
                  b->max_kv};
 }
 
-// Both operands of a lane swap: v_permlane16_swap exchanges the odd 16-lane rows of x with
-// the even ones of y, v_permlane32_swap the upper half of x with the lower half of y.  With x = y
-// = v the two hold v of the lane and of its partner.  (The compiler's builtins return x alone:
-// a maximum over both results of one is folded away.)  s_nop: the swap's operands were just
-// written.
-__device__ __forceinline__ void pk_swap16(float& x, float& y) {
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-}
-__device__ __forceinline__ void pk_swap32(float& x, float& y) {
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-}
-// Max over the lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float pk_rowmax(float v) {
-  float x = v, y = v;
-  pk_swap16(x, y);
-  x = y = fmaxf(x, y);
-  pk_swap32(x, y);
-  return fmaxf(x, y);
-}
-
 // The sequence that row t belongs to: the last b with q_start[b] <= t, or n where t is past
 // q_start[n].  The whole wave looks: 64 boundaries at once, so up to 64 sequences take one
 // load and up to 4096 two.  Callers must be converged.

@@ -493,7 +493,7 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
   }
   float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                    fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-  mt = pk_rowmax(mt);
+  mt = mx_rowmax4(mt);
   const bool up = mt > mrun + kTau;
   if (__builtin_amdgcn_ballot_w64(up)) {
     const float mnew = up ? mt : mrun;
@@ -1259,7 +1259,7 @@ __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkB
       for (int r = 0; r < 4; ++r)
         if (4 * g + r > lim || !on) s[r] = -INFINITY;
     }
-    const float mt = pk_rowmax(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float mt = mx_rowmax4(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
     const bool up = mt > mrun + kTau;
     if (__builtin_amdgcn_ballot_w64(up)) {
       const float mnew = up ? mt : mrun;

@@ -96,3 +96,51 @@ def test_norm_weights_at_any_address(mi355x, stream):
         mi355x.free_device(buf)
         layer.close()
     assert np.linalg.norm(got - want) <= 4 * 2.0 ** -11 * np.linalg.norm(want - x)
+
+
+@pytest.mark.parametrize("hd,nh,nkv,T", [(128, 4, 2, 100), (256, 8, 2, 400), (72, 4, 1, 65),
+                                         (128, 32, 4, 2200)])
+def test_sharp_heads_match_float64(mi355x, stream, hd, nh, nkv, T):
+    """Scores tens of units apart, the largest of a key tile in any of its rows: the softmax takes
+    its reference over all of them.  Tolerance: q and k are rounded to fp16, so a score is off by up
+    to d = (2 x 2^-11 + hd 2^-24) sum |q_i k_i| / sqrt(hd) and a normalised probability by a factor
+    e^(2 d); then one rounding each of probability, value and output, 2^-25 of the largest value
+    for a subnormal probability, and 2^-13 for the sums."""
+    s = syn.FullAttnShape(128, nh, nkv, hd, 0.25, 10000.0, 1e-6)
+    print(f"[gpu] fp16 attention, sharp heads, hd={hd} heads={nh}/{nkv} T={T}", flush=True)
+    t = syn.make_full_attn_tensors(s, 30 + T, weight_dtype=np.float16, norm_noise=0.1)
+    for name in ("self_attn.q_norm.weight", "self_attn.k_norm.weight"):
+        t[name] = t[name] * np.float32(3.0)
+    x = syn.make_inputs(31 + T, T, s.hidden)
+    layer = DeviceFullAttnLayer.from_host(mi355x, t, nh, nkv, hd, s.rotary_dim, s.rope_theta,
+                                          stream)
+    try:
+        layer.forward_numpy(x, s.eps)
+        v = layer.runner.views(layer.desc(s.eps), T)
+        od, kw = nh * hd, nkv * hd
+
+        def read(p, dt, n):
+            return read_device(mi355x, p, dt, T * n, stream).reshape(T, n).astype(np.float64)
+
+        qg, act = read(v.qg, np.float32, 2 * od), read(v.act, np.float16, od)
+        k, vv = read(v.k, np.float32, kw), read(v.v, np.float32, kw)
+    finally:
+        layer.close()
+    assert np.all(np.isfinite(act))
+    hidden = np.triu(np.ones((T, T), bool), 1)
+    spread = 0.0
+    for h in range(nh):
+        c = slice(h * hd, (h + 1) * hd)
+        kc = slice(h // (nh // nkv) * hd, (h // (nh // nkv) + 1) * hd)
+        sc = np.where(hidden, -np.inf, qg[:, c] @ k[:, kc].T / np.sqrt(hd))
+        size = np.where(hidden, 0, np.abs(qg[:, c]) @ np.abs(k[:, kc]).T / np.sqrt(hd))
+        d = size.max(axis=1, keepdims=True) * (2.0 ** -10 + hd * 2.0 ** -24)
+        p = np.exp(sc - sc.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        gate = 1 / (1 + np.exp(-qg[:, od:][:, c]))
+        want, mag = p @ vv[:, kc] * gate, p @ np.abs(vv[:, kc]) * gate
+        tol = mag * (np.expm1(2 * d) + 2 * 2.0 ** -11 + 2.0 ** -13) * 1.01 + 2.0 ** -11 * np.abs(want) \
+            + T * 2.0 ** -25 * np.abs(vv[:, kc]).max() + 1e-7
+        assert np.all(np.abs(act[:, c] - want) <= tol)
+        spread = max(spread, sc[-1].max() - sc[-1].min())
+    assert spread > 22.0  # twice what fp16 probabilities hold above a reference
