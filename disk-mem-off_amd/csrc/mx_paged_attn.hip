@@ -319,21 +319,6 @@ __device__ __forceinline__ half8_t pa_i8x8(int2_t v) {
   return (half8_t){h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
-// 16 int8 -> 16 fp16 of 1152 + q, exact: byte q + 128 under exponent 0x64 reads as 1024 + (q + 128).
-__device__ __forceinline__ void pa_i8_biased(int4_t v, half8_t& lo, half8_t& hi) {
-  int4_t a, b;
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    const uint32_t u = (uint32_t)v[d] ^ 0x80808080u;
-    const int p0 = (int)__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-    const int p1 = (int)__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    (d < 2 ? a : b)[2 * (d & 1)] = p0;
-    (d < 2 ? a : b)[2 * (d & 1) + 1] = p1;
-  }
-  lo = __builtin_bit_cast(half8_t, a);
-  hi = __builtin_bit_cast(half8_t, b);
-}
-
 // ------------------------------------------------------------------------------------
 // LDS tiles of 32 rows of RB bytes (RB = 64 .. 512, the padded row), row-major, a row's 16-byte
 // chunks permuted by an XOR so that the fragment reads use every bank once: 8 lanes of a
@@ -631,16 +616,6 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
 #pragma unroll
   for (int cc = 0; cc < NC; ++cc)
     if (qdim(cc) >= c.hd) qf[cc] = (half8_t)(half_t)0.f;
-  // Int8 keys meet the queries as 1152 + q (pa_i8_biased): 1152 times the sum of the row's queries
-  // comes off the score.
-  float bias = 0.f;
-  if constexpr (DT == MX_DT_I8) {
-#pragma unroll
-    for (int cc = 0; cc < NC; ++cc)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) bias += (float)qf[cc][e];
-    bias = -1152.f * pa_rowsum(bias);
-  }
   // The last key that every row of the tile sees (rows past the last repeat it), and that any does.
   const int all = t.pos0 + t.row0 / a.group, any = t.kend - 1;
   // MORE: a tile follows.  Its copies are issued without a branch, so that the compiler's own waits
@@ -655,13 +630,13 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
     for (int s = 0; s < 2; ++s) {
       const char* p0 = kbuf + klane + s * 16 * RB;
       const char* p1 = kbuf + (klane ^ (CPR > 4 ? 64 : 0)) + s * 16 * RB;
-      float4_t x[2] = {{bias, bias, bias, bias}, {0.f, 0.f, 0.f, 0.f}};
+      float4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         const int4_t kf = *(const int4_t*)((n & 1 ? p1 : p0) + 64 * (n & ~1));
         if constexpr (DT == MX_DT_I8) {
           half8_t lo, hi;
-          pa_i8_biased(kf, lo, hi);
+          mx_i8_to_f16(kf, lo, hi);
           x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qf[2 * n], x[0], 0, 0, 0);
           x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qf[2 * n + 1], x[1], 0, 0, 0);
         } else {
