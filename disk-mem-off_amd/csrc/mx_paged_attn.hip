@@ -467,7 +467,7 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
       const bool out = MASK && (16 * b + r > lim || !((on >> b) & 1));
       float v;
       if constexpr (DT == MX_DT_I8) {
-        const float w = fmaxf(vq[r], 1e-30f);
+        const float w = vq[r] < 1e-30f ? 1e-30f : vq[r];  // a NaN stays, which fmaxf would drop
         inv[4 * b + r] = out ? 0.f : __builtin_amdgcn_rcpf(w);
         v = __builtin_fmaf(sc[b][r], rs * kq[r], __builtin_amdgcn_logf(w));
       } else {

@@ -179,11 +179,13 @@ __global__ __launch_bounds__(256) void k_pk_append(PkCache c, PkBatch b, PkRowAr
       if (act && valid && stored) pk_store4<true>(pool, c.dt == MX_DT_F32, at * c.hd + i, o);
       continue;
     }
-    float m = valid ? fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w))) : 0.f;
+    // As bits: an infinity or a NaN is larger than every number, and makes the row's scale NaN.
+    auto size = [](float v) { return (int)(__float_as_uint(v) & 0x7FFFFFFFu); };
+    int m = valid ? max(max(size(o.x), size(o.y)), max(size(o.z), size(o.w))) : 0;
 #pragma unroll
-    for (int d = 1; d < LPR; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    for (int d = 1; d < LPR; d *= 2) m = max(m, __shfl_xor(m, d));
     if (kind == 0) continue;  // the shuffles needed every lane
-    const float scale = m > 0.f ? m / 127.f : 1.f;
+    const float scale = m >= 0x7F800000 ? __builtin_nanf("") : m > 0 ? __uint_as_float((uint32_t)m) / 127.f : 1.f;
     auto q8 = [&](float v) {
       return (uint32_t)((int)fminf(fmaxf(rintf(v / scale), -127.f), 127.f) & 255);
     };

@@ -491,8 +491,8 @@ int mx_gated_delta_scan_ws(const float* q, const float* kb, const float* v,
 
 /* The keys and values of one layer, in pages of page_size tokens:
  * k, v [n_pages, n_kv_heads, page_size, head_dim] of dtype F32, F16 or I8 (16-byte aligned);
- * int8 rows stand for int8 * scale with one fp32 scale (finite, >= 0) per row in k_scale, v_scale
- * [n_pages, n_kv_heads, page_size] (16-byte aligned; NULL for the other types).
+ * int8 rows stand for int8 * scale with one fp32 scale (finite and >= 0, or NaN: a row of NaN) per row
+ * in k_scale, v_scale [n_pages, n_kv_heads, page_size] (16-byte aligned; NULL for the other types).
  * page_size: 16, 32, 64, 128 or 256.  head_dim: a multiple of 8 (I8: 16), <= 256.      */
 typedef struct MxKvCache {
   void* k;
@@ -531,8 +531,8 @@ typedef struct MxPagedBatch {
  * one is given), then the rotate-half rotary embedding of the first rotary_dim dims at the
  * row's position, angles formed in 64 bits (position * theta^(-2 j / rotary_dim)).  q goes
  * to q_out (F32 with an F32 cache, else F16; q and q_out NULL: no queries), k and v to their
- * pages; int8 rows get scale max|row| / 127 (1 for a row of zeros).  Rows at a negative
- * position are left out.                                                               */
+ * pages; int8 rows get scale max|row| / 127 (1 for a row of zeros; NaN for a row with a NaN or an
+ * infinity in it, which then reads as NaN).  Rows at a negative position are left out.  */
 typedef struct MxKvRows {
   const void* q;
   const void* k;

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 import _serving as sv
-from moe_mi355x.paged_kv import PagedKvCache, attn_args
+from moe_mi355x.paged_kv import PagedKvCache, append_args, attn_args
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,39 @@ def test_int8_scores_keep_their_digits_under_a_common_offset(mi355x, stream, hd,
     got = attend(mi355x, stream, b, q, k, v, ks, vs)
     want, mag, big = sv.attention(b, q[:b.used], sv.values(k, ks), sv.values(v, vs), nkv, 1.0)
     assert np.all(np.abs(got - want) <= rounded(want, mag, big, max(lens)))
+
+
+@pytest.mark.parametrize("news,lens", [([7, 3], [40, 20]), ([40, 9], [100, 9])])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_int8_rows_that_are_not_finite_read_as_nan(mi355x, stream, news, lens, what):
+    """A key and a value with one element that is no number, appended to int8 pages: their rows get a
+    NaN scale, the tokens that see them are NaN, and all others are as if they were not there."""
+    say(f"int8 append and attention with {what}, {news}")
+    nh, nkv, hd, page = 4, 2, 64, 16
+    rng = np.random.default_rng(21)
+    b = sv.Batch(rng, news, lens, page, pad=1)
+    k0, ks0 = sv.pool_of(rng, b, nkv, hd, "int8", hole=0.02)
+    x = rng.standard_normal((2, b.rows, nkv, hd)).astype(np.float32)
+    x[0, news[0] - 2, 0, 5] = what              # a key of the first sequence, head 0
+    x[1, news[0] + news[1] - 1, 1, hd - 1] = what  # a value of the second, head 1
+    q = (rng.standard_normal((b.rows, nh, hd)) * 1.5).astype(np.float16)
+    with sv.Arrays(mi355x, stream) as ar:
+        bufs = tuple(ar.put(a) for a in (k0, k0, ks0, ks0))
+        cache = PagedKvCache(mi355x, 1, nkv, hd, b.n_pages, page_size=page, dtype="int8",
+                             buffers=[bufs])
+        cache.append(0, b.device(ar), append_args(k=ar.put(x[0]), v=ar.put(x[1]), n_kv_heads=nkv,
+                                                  head_dim=hd), stream)
+        k, v, ks, vs = (ar.get(p, a) for p, a in zip(bufs, (k0, k0, ks0, ks0)))
+    bad = np.zeros((2, b.n_pages, nkv, page), bool)
+    for i, seq, pos, h in ((0, 0, lens[0] - 2, 0), (1, 1, lens[1] - 1, 1)):
+        bad[i, b.table[seq, pos // page], h, pos % page] = True
+    assert np.array_equal(np.isnan(np.stack([ks, vs])), bad)
+    assert np.all(np.isfinite(np.stack([ks, vs])[~bad]))
+    got = attend(mi355x, stream, b, q, k, v, ks, vs, hd ** -0.5)
+    want, mag, big = sv.attention(b, q[:b.used], sv.values(k, ks), sv.values(v, vs), nkv, hd ** -0.5)
+    gone = np.zeros(got.shape, bool)
+    gone[news[0] - 2:news[0], :2] = True
+    gone[b.used - 1, 2:] = True
+    assert np.all(np.isnan(got[gone])) and np.all(np.isfinite(got[~gone]))
+    ok = np.abs(got - want) <= rounded(want, mag, big, max(lens))
+    assert np.all(ok[~gone])
