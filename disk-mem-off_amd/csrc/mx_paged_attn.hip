@@ -1451,6 +1451,8 @@ int check(const MxKvCache* cache, const MxPagedBatch* batch, int n_heads) {
   MX_TRY(pk_check_cache(cache));
   MX_TRY(pk_check_batch(batch));
   if (n_heads <= 0 || n_heads % cache->n_kv_heads) return MX_ERR_INVALID;
+  // (a key's number plus a range's length stays below 2^31)
+  if (batch->max_kv > (1 << 30)) return MX_ERR_UNSUPPORTED;
   return n_heads > 65535 || (long)n_heads * batch->rows >= (1l << 26) ? MX_ERR_UNSUPPORTED : MX_OK;
 }
 

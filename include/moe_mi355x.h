@@ -561,7 +561,8 @@ int mx_kv_append(const MxKvCache* cache, const MxPagedBatch* batch, const MxKvRo
  * elements (ldq, ldo, ldg), head after head.  Key/value head of query head h:
  * h / (n_heads / n_kv_heads).  Fp16 and int8 caches: products of fp16 operands with fp32
  * sums (probabilities rounded to fp16); fp32 caches: fp32 throughout.  q and gate 16-byte
- * aligned with row strides that keep it, out likewise.                                 */
+ * aligned with row strides that keep it, out likewise.  Besides the batch's limits: max_kv <= 2^30,
+ * n_heads <= 65535 and n_heads * rows < 2^26.                                          */
 typedef struct MxPagedAttn {
   const void* q;
   void* out;

@@ -284,3 +284,23 @@ def test_delta_workspaces():
     assert lib.mx_gated_delta_rule(ctypes.byref(d), None, need, None) == _lib.MX_ERR_WORKSPACE
     assert lib.mx_gated_delta_rule(ctypes.byref(d), A, need - 1, None) == _lib.MX_ERR_WORKSPACE
     assert lib.mx_gated_delta_rule(ctypes.byref(d), A + 8, need, None) == ALI
+
+
+@pytest.mark.parametrize("b,heads,kv_heads,rc", [
+    (dict(max_kv=(1 << 30) + 1), 4, 2, UNS),   # key numbers would pass 32 bits inside the kernels
+    (dict(max_kv=2 ** 31 - 1), 4, 2, UNS),
+    (dict(rows=1 << 22), 16, 2, UNS),          # 2^26 rows of heads
+    (dict(rows=1), 65536, 2, UNS),
+    (dict(rows=(1 << 22) - 1), 16, 2, 0), (dict(max_kv=1 << 30), 4, 2, 0), (dict(rows=1), 65535, 1, 0)])
+def test_sizes_behind_the_limits_of_attention_are_refused(b, heads, kv_heads, rc):
+    """The workspace query and the call agree on what is too large; at the limits the query answers."""
+    n = ctypes.c_size_t(77)
+    c, ba = cache(n_kv_heads=kv_heads, head_dim=8), batch(**b)
+    assert _lib.load().mx_paged_attn_workspace_size(ctypes.byref(c), ctypes.byref(ba), heads,
+                                                    ctypes.byref(n)) == rc
+    ld = heads * 8
+    if rc:
+        assert call_attn(c, ba, attn(n_heads=heads, ldq=ld, ldo=ld)) == rc
+    else:  # no workspace: refused before any launch
+        assert n.value > 0
+        assert call_attn(c, ba, attn(n_heads=heads, ldq=ld, ldo=ld)) == _lib.MX_ERR_WORKSPACE
