@@ -166,6 +166,23 @@ class PageTables:
         self._refs[p] = 1
         return p
 
+    def take_back(self, growth: Sequence[tuple[int, int]], copies: list[tuple[int, int]]) -> None:
+        """Undoes the last ``extend(growth)``, which gave ``copies``."""
+        source = {d: s for s, d in copies}
+        for seq, n in reversed(growth):
+            have = self._pages[seq]
+            self._len[seq] -= n
+            while len(have) > -(-self._len[seq] // self.page_size):
+                self._give(have.pop())
+            if have and have[-1] in source:
+                self._give(have[-1])
+                have[-1] = source[have[-1]]
+                self._refs[have[-1]] += 1
+
+    def _give(self, p: int) -> None:
+        self._refs[p] = 0
+        self._free.append(p)
+
     def free(self, seq: int) -> None:
         """Forgets the sequence; pages no other sequence has become free."""
         back = []
@@ -182,13 +199,17 @@ class PageTables:
         used = [p for p in range(self.n_pages) if self._refs[p]]
         holes = [p for p in range(len(used)) if not self._refs[p]]
         moves = list(zip([p for p in used if p >= len(used)], holes))
+        self.move(moves)
+        return moves
+
+    def move(self, moves: list[tuple[int, int]]) -> None:
+        """Used pages to free places, (from, to), in the tables."""
         to = dict(moves)
         for s, d in moves:
             self._refs[d], self._refs[s] = self._refs[s], 0
         for have in self._pages.values():
             have[:] = [to.get(p, p) for p in have]
-        self._free = list(range(self.n_pages - 1, len(used) - 1, -1))
-        return moves
+        self._free = [p for p in range(self.n_pages - 1, -1, -1) if not self._refs[p]]
 
 
 # ---- the cache -------------------------------------------------------------------------------
@@ -278,14 +299,32 @@ class PagedKvCache:
         self.tables.free(seq)
 
     def compact(self, stream: Any) -> None:
-        """Used pages to the front of the pools; batches made before are void."""
-        self._copy(self.tables.compact(), stream)
+        """Used pages to the front of the pools; batches made before are void.  Waits for the
+        stream; where a device call fails, the tables stay as they were."""
+        moves = self.tables.compact()
+        try:
+            self._copy(moves, stream)
+        except BaseException:
+            self.tables.move([(d, s) for s, d in moves])
+            raise
 
     def batch(self, growth: Iterable[tuple[int, int]], stream: Any) -> _lib.MxPagedBatch:
         """Grows the sequences by their new rows (copying part-filled pages they share) and
-        uploads the tables of a call on them; the last batch of the cache is void then."""
+        uploads the tables of a call on them; the last batch of the cache is void then.
+
+        The call waits for the stream, and tables that no longer fit are allocated anew, at another
+        address: a graph, or a step that must not stall the host, takes :func:`paged_batch` with
+        device arrays of the caller's.  Where a device call fails no sequence has grown."""
         growth = [(s, int(n)) for s, n in growth]
-        self._copy(self.tables.extend(growth), stream)
+        copies = self.tables.extend(growth)
+        try:
+            self._copy(copies, stream)
+            return self._tables(growth, stream)
+        except BaseException:
+            self.tables.take_back(growth, copies)
+            raise
+
+    def _tables(self, growth: list[tuple[int, int]], stream: Any) -> _lib.MxPagedBatch:
         pages = [self.tables.pages(s) for s, _ in growth]
         n, mp = len(growth), max([1, *(len(p) for p in pages)])
         starts = np.concatenate([[0], np.cumsum([m for _, m in growth])]).astype(np.int32)

@@ -9,6 +9,7 @@ import pytest
 
 from moe_mi355x import _lib, delta_rule, paged_kv
 from moe_mi355x.paged_kv import PagedKvCache, PageTables
+from moe_mi355x.types import DeviceBuffer
 
 A = 1 << 12  # an aligned address that is never read
 
@@ -304,3 +305,109 @@ def test_sizes_behind_the_limits_of_attention_are_refused(b, heads, kv_heads, rc
     else:  # no workspace: refused before any launch
         assert n.value > 0
         assert call_attn(c, ba, attn(n_heads=heads, ldq=ld, ldo=ld)) == _lib.MX_ERR_WORKSPACE
+
+
+# ---- failing device calls --------------------------------------------------------------------
+
+class FailingBackend:
+    """Device calls that work until the ``fail``-th of them."""
+
+    def __init__(self, fail=None):
+        self.left, self.live, self.next = fail, {}, 1 << 20
+
+    def _count(self):
+        if self.left is not None:
+            self.left -= 1
+            if self.left < 0:
+                raise RuntimeError("device call failed")
+
+    def alloc_device(self, nbytes):
+        self._count()
+        self.next += -(-nbytes // 256) * 256
+        self.live[self.next] = nbytes
+        return DeviceBuffer(handle=self.next, nbytes=nbytes, backend="failing")
+
+    def free_device(self, buf):
+        del self.live[buf.handle]
+
+    def copy_h2d_ptr_async(self, *args):
+        self._count()
+
+    def synchronize_stream(self, stream):
+        self._count()
+
+
+def state(t):
+    return (list(t._refs), list(t._free), {s: list(p) for s, p in t._pages.items()}, dict(t._len))
+
+
+def test_extend_can_be_taken_back():
+    """From any state, with shared part-filled pages, whole new pages and growth of nothing."""
+    rng = np.random.default_rng(8)
+    t = PageTables(40, 4)
+    tried = 0
+    for _ in range(3000):
+        seqs = list(t._pages)
+        what = rng.integers(5)
+        if what == 0 and len(seqs) < 7:
+            t.add()
+        elif what == 1 and seqs and len(seqs) < 7:
+            t.fork(int(rng.choice(seqs)))
+        elif what == 2 and len(seqs) > 2:
+            t.free(int(rng.choice(seqs)))
+        elif seqs:
+            growth = [(int(s), int(rng.integers(0, 9))) for s in rng.permutation(seqs)[:4]]
+            before = state(t)
+            try:
+                copies = t.extend(growth)
+            except RuntimeError:
+                assert state(t) == before
+                continue
+            t.take_back(growth, copies)
+            assert state(t) == before
+            tried += bool(copies)
+            t.extend(growth)
+    assert tried > 50
+
+
+@pytest.mark.parametrize("fail", range(12))
+def test_a_failing_device_call_leaves_the_sequences_as_they_were(monkeypatch, fail):
+    monkeypatch.setattr(paged_kv, "copy_pages", lambda *a: be._count())
+    be = FailingBackend()
+    c = PagedKvCache(be, 1, 1, 16, 300, page_size=16, buffers=[(A, A, None, None)])
+    a = c.add()
+    c.batch([(a, 20)], None)
+    b = c.fork(a)
+    d = c.add()
+    before = state(c.tables)
+    be.left = fail  # a copied page, new pages, larger tables
+    try:
+        c.batch([(a, 1), (b, 30), (d, 4000)], None)
+    except RuntimeError:
+        assert state(c.tables) == before
+        be.left = None
+        c.batch([(a, 1), (b, 30), (d, 4000)], None)
+    else:
+        assert be.left >= 0 and c.tables.length(d) == 4000
+    be.left = None
+    c.close()
+    assert not be.live
+
+
+@pytest.mark.parametrize("fail", range(5))
+def test_a_failing_compaction_moves_nothing(monkeypatch, fail):
+    monkeypatch.setattr(paged_kv, "copy_pages", lambda *a: be._count())
+    be = FailingBackend()
+    c = PagedKvCache(be, 1, 1, 16, 30, page_size=16, buffers=[(A, A, None, None)])
+    a, b = c.add(), c.add()
+    c.batch([(a, 40), (b, 50)], None)
+    c.free(a)
+    before = state(c.tables)
+    be.left = fail
+    try:
+        c.compact(None)
+    except RuntimeError:
+        assert state(c.tables) == before
+        be.left = None
+        c.compact(None)
+    assert sorted(c.tables.pages(b)) == [0, 1, 2, 3]
