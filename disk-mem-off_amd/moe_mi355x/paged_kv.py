@@ -243,13 +243,17 @@ class PagedKvCache:
         sizes = [rows * head_dim * _ESZ[dtype]] * 2 + [rows * 4 if dtype == "int8" else 0] * 2
         if buffers is None:
             buffers = []
-            for _ in range(n_layers):
-                got = []
-                for size in sizes:
-                    if size:
-                        self._owned.append(backend.alloc_device(size))
-                    got.append(int(self._owned[-1].handle) if size else None)
-                buffers.append(tuple(got))
+            try:
+                for _ in range(n_layers):
+                    got = []
+                    for size in sizes:
+                        if size:
+                            self._owned.append(backend.alloc_device(size))
+                        got.append(int(self._owned[-1].handle) if size else None)
+                    buffers.append(tuple(got))
+            except BaseException:
+                self.close()
+                raise
         self.layers = [_lib.MxKvCache(*b, n_pages, page_size, n_kv_heads, head_dim, _DT[dtype])
                        for b in buffers]
         per = page_size * n_kv_heads

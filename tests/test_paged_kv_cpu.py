@@ -411,3 +411,11 @@ def test_a_failing_compaction_moves_nothing(monkeypatch, fail):
         be.left = None
         c.compact(None)
     assert sorted(c.tables.pages(b)) == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("fail", range(8))
+def test_a_cache_that_does_not_fit_leaves_nothing_behind(fail):
+    be = FailingBackend(fail)
+    with pytest.raises(RuntimeError):
+        PagedKvCache(be, 3, 1, 16, 4, page_size=16, dtype="int8")
+    assert not be.live
