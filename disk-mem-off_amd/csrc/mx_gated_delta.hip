@@ -610,7 +610,7 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
 //
 // A column's factor 2^e of the state's planes has to be known before all waves have the new state: from
 // the bound e^G max|S| + 64 max|k| max|c u|, whose maxima went through LDS before (k's rows are
-// scaled to 2^15, c u's are below 2^15 of their factor).  It may exceed the maximum by 2^10 before
+// scaled to 2^15, c u's are below 2^15 of their factor).  It may exceed the maximum by 2^15 before
 // the 2^-39 above reaches fp32's own 2^-24.
 //
 // A NaN or infinity in x (a NaN in v is one of its column, in k of every column) would meet the zeros

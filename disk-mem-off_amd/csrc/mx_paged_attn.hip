@@ -841,9 +841,7 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
 //
 // Row tiles of a key/value head run on the XCDs that its keys are dealt to.
 // ------------------------------------------------------------------------------------
-#ifndef PA_PD
-#define PA_PD 2  // LDS fragment reads in flight ahead of the MFMAs
-#endif
+constexpr int kAheadReads = 2;  // LDS fragment reads in flight ahead of the MFMAs
 
 template <int RB, int DT, int QS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -977,13 +975,13 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
     for (int u = 0; u < QS; ++u)
 #pragma unroll
       for (int s = 0; s < 2; ++s) sc[u][s] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    int4_t fr[PA_PD];
+    int4_t fr[kAheadReads];
 #pragma unroll
-    for (int i = 0; i < PA_PD && i < 2 * NK; ++i) fr[i] = kfrag(i);
+    for (int i = 0; i < kAheadReads && i < 2 * NK; ++i) fr[i] = kfrag(i);
 #pragma unroll
     for (int i = 0; i < 2 * NK; ++i) {
-      const int4_t kf = fr[i % PA_PD];
-      if (i + PA_PD < 2 * NK) fr[i % PA_PD] = kfrag(i + PA_PD);
+      const int4_t kf = fr[i % kAheadReads];
+      if (i + kAheadReads < 2 * NK) fr[i % kAheadReads] = kfrag(i + kAheadReads);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (DT == MX_DT_I8) {
         half8_t lo, hi;
@@ -1384,10 +1382,12 @@ int plan(const MxKvCache* c, const MxPagedBatch* b, int nh, PaPlan* p) {
   // take longer: 2 x 500 tokens 16.1 us in ranges of 64, 19.5 of 128.
   p->least = p->kind == kF32 ? 64 : own && keys <= 256 ? 256 : 128;
   p->most = own ? kKeysMax : 1 << 30;
-  // Items of a head: ranges of len >= least keys, where len >= (sum of keys) / target or is `most`.
+  // Items of a head, as pa_schedule comes to them: the tiles' ceil(keys / len) add up to at most tiles +
+  // (keys of the tiles) / len, and len is above nkv (keys of the tiles) / target, or `most`; one or
+  // two roundings of its 32-bit sum do not matter, since the extra are counted twice.
   const long capped = own ? tiles * (keys / kKeysMax) : 0;
   const long fine = tiles * (keys / p->least);
-  const long extra = 2 * (p->target / nkv + 1);  // (the schedule may count on half the target)
+  const long extra = 2 * (p->target / nkv + 1);
   long slots = tiles + (extra > capped ? extra : capped);
   if (slots > tiles + fine) slots = tiles + fine;
   const long ranges = (keys + p->least - 1) / p->least;
