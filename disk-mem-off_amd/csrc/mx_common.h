@@ -88,13 +88,14 @@ __device__ __forceinline__ void mx_swap16(float& x, float& y) {
 __device__ __forceinline__ void mx_swap32(float& x, float& y) {
   asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
 }
-// Max over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+// Max over the lanes l, l ^ 16, l ^ 32, l ^ 48; NaN where one is (fmaxf would quiet both operands first,
+// since nothing is known of what the swaps give).
 __device__ __forceinline__ float mx_rowmax4(float v) {
   float x = v, y = v;
   mx_swap16(x, y);
-  x = y = fmaxf(x, y);
+  x = y = __builtin_elementwise_maximum(x, y);
   mx_swap32(x, y);
-  return fmaxf(x, y);
+  return __builtin_elementwise_maximum(x, y);
 }
 
 // Reference silu: x / (1 + exp(-x))  (_common.py:83-84).
