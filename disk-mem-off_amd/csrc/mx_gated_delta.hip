@@ -601,7 +601,7 @@ __global__ __launch_bounds__(256, FULL && sizeof(XT) == 2 ? 4 : 3) void k_gd_pre
 // A sequence's chunks in order, 16 columns of a head's state per block.  Wave rt has the tokens 16 rt ..
 // of the chunk and the rows 16 SL rt .. of the state, in accumulators.  Per chunk three barriers:
 //   the state's planes to LDS  | k^T S and q^T S; x to LDS, k to LDS  | u = T x to LDS  | o and S
-// Bound by these steps one after the other: a chunk takes 2.3 us where a CU has one block and 3.5 with
+// Bound by these steps one after the other: a chunk takes 2.3 us where a CU has one block and 3.3 with
 // two (heads of 128 x 128, fp16).  Tried and slower: 32 columns per block of 8 waves (442 us
 // against 380 for 4 prompts of up to 2600 tokens, early on), and 8 waves for 16 columns, four
 // of them for k and T and four for q and P (180 us against 147).

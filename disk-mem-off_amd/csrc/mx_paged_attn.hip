@@ -508,7 +508,8 @@ __device__ __forceinline__ half8_t pa_softmax(float4_t (&sc)[2], float rs, const
 // would be 16 rows x 16 bytes per quarter wave, a cache line each); the next tile's keys are on
 // their way from the moment this tile's scores are formed, its values from the moment this
 // tile's are used.  No barrier until the waves' sums are put together at the end.  64 sequences of 8000
-// fp16 tokens, 16 heads over 2 of 256: 185 us with the join, 5.7 TB/s; two of 913 tokens 11.8 us, launches.
+// fp16 tokens, 16 heads over 2 of 256: 185 us with the join, 5.7 TB/s; two of 913 tokens 11.7 us, launches; 40
+// ragged ones of up to 12000 int8 tokens 32 us, of which 27.5 here (3.3 TB/s, 76 bytes of scratch per lane).
 // ------------------------------------------------------------------------------------
 constexpr int kKeysMax = 4096;  // keys of a split: 64 sub-tile page ids per wave
 
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(256, RB < 512 ? 2 : 1) void k_pa_keys(PkCache c, Pk
 // lie.  One wave per (row, head), or WIDE, a block's four waves, a quarter of the ranges each: a
 // decode step has few rows of many ranges, whose sums were written by other XCDs and take a
 // microsecond or two to fetch (40 rows of up to 35 ranges: 11.4 us with one wave, 5.0 with four).
-// Bound by the sums' bytes where there are many rows: 2048 rows of 16 heads in two ranges 24 us.
+// Bound by the sums' bytes where there are many rows: 2048 rows of 16 heads in two ranges 21 us.
 // ------------------------------------------------------------------------------------
 template <typename OT, bool WIDE>
 __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a, PaSched sp) {
@@ -837,7 +838,8 @@ __global__ __launch_bounds__(256) void k_pa_join(PkCache c, PkBatch b, PaArgs a,
 // copied straight into two LDS buffers by the buffer loads' LDS mode; a wave's copies of tile t + 1
 // are issued behind the barrier that opens tile t.  Each fragment read from LDS feeds QS query
 // sets.  A wave computes up to its own last key and then only keeps the copies going.  2048 rows over 8192
-// tokens, 16 heads over 2 of 256: 260 us with the join, 0.92 PFLOP/s.
+// tokens, 16 heads over 2 of 256: 259 us with the join, 0.93 PFLOP/s.  Two sets of 256 fp16 dims take all 256
+// registers and 12 bytes of scratch.
 //
 // Row tiles of a key/value head run on the XCDs that its keys are dealt to.
 // ------------------------------------------------------------------------------------
@@ -1124,7 +1126,7 @@ void k_pa_rows(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
 // rows, keys dealt to the waves 16 at a time, keys in registers, values through the wave's LDS
 // buffers.  The MFMA k-slot of lane group g at step r is key 4 g + r on both operands.  Bound by those
 // instructions (a sixteenth of fp16's rate) and, in small calls, by their latency: 3 x 130 rows over 1500 tokens,
-// 32 heads over 8 of 128: 134 us, 68 TFLOP/s.
+// 32 heads over 8 of 128: 131 us, 70 TFLOP/s.  Heads of 256 dims: 60 bytes of scratch.
 // ------------------------------------------------------------------------------------
 template <int DP, bool DIRECT>
 __global__ __launch_bounds__(256, DP < 256 ? 2 : 1) void k_pa_f32(PkCache c, PkBatch b, PaArgs a, PaSched sp, int per) {
