@@ -64,10 +64,11 @@ struct Args {
   Seg seg[kSegs];
 };
 
-// The scaled sum: the same roundings in every kernel, whatever is added to it.
+// The scaled sum: the same roundings in every kernel, whatever is added to it.  sw first: sum sw lies between 2^-24 and
+// 2^46, while sx sw may leave the range of fp32 (sx is down to 2^-126) where the result does not.
 __device__ __forceinline__ float scaled(int sum, float sx, float sw) {
 #pragma clang fp contract(off)
-  return (float)sum * (sx * sw);
+  return (float)sum * sw * sx;
 }
 
 // Four columns of row m from column n on, res added.
