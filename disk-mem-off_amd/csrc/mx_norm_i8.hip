@@ -155,10 +155,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_norm_i8(const NormArgs a)
       top = fmax(top, part[1][w]);
     }
   }
-  const double r = a.norm ? 1.0 / sqrt(ss / (double)H + (double)a.eps) : 1.0;
+  // A row of zeros stays one where eps is 0.
+  const double mean = ss / (double)H + (double)a.eps;
+  const double r = !a.norm ? 1.0 : mean == 0.0 ? 0.0 : 1.0 / sqrt(mean);
   float s = (float)(top * r / 127.0);
   const bool lost = !(top <= DBL_MAX) || !(s <= FLT_MAX);
-  s = lost ? __builtin_nanf("") : top == 0.0 ? 1.f : fmaxf(s, FLT_MIN);
+  s = lost ? __builtin_nanf("") : top * r == 0.0 ? 1.f : fmaxf(s, FLT_MIN);
   const double step = lost ? 0.0 : r / (double)s;
   if (a.qs && t == 0) a.qs[row] = s;
 #pragma unroll

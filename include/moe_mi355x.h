@@ -654,10 +654,10 @@ int mx_gated_delta_rule(const MxGatedDelta* args, void* workspace, size_t worksp
  *   v = x + res;  y = v / sqrt(mean(v^2) + eps) * norm_w  (norm 0: y = v)
  *   s = max|y| / 127;  q = rint(y / s)
  * worked out in 64 bits from the inputs, so that a code next to a border is the definition's; s is
- * rounded to fp32 before the division (1 for a row of zeros, at least 2^-126 for others; NaN for a
- * row with a NaN or an infinity in it, whose codes are 0 and stand for NaN).  Rows of x_dtype
- * (F32 / F16) and, of the residual stream, res_dtype; sum = v in res_dtype may be res (or x, of the same
- * type and stride), h16 is y in fp16.  res, sum, norm_w, h16 may be NULL, and q with q_scale too where
+ * rounded to fp32 before the division (1 for a row of zeros, which stays one where eps is 0 too; at least
+ * 2^-126 for others; NaN for a row with a NaN or an infinity in it, whose codes are 0 and stand for NaN).
+ * Rows of x_dtype (F32 / F16) and, of the residual stream, res_dtype; sum = v in res_dtype may be res (or x,
+ * of the same type and stride), h16 is y in fp16.  res, sum, norm_w, h16 may be NULL, and q with q_scale too where
  * h16 is not; no other two arrays may overlap.  Row strides in elements, every array on a boundary of its
  * element; hidden <= 16384, rows < 2^24.                                                                         */
 typedef struct MxNormRows {

@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_projection import Case, say
+from test_gpu_projection import Case, check_norm, norm64, run_norm, say
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,29 @@ def test_scales_at_both_ends_of_fp32(mi355x, stream, rows):
     err = np.abs(got[small] - want[small])
     assert np.all(err <= 3.01 * 2.0 ** -24 * np.abs(want[small]) + 2.0 ** -150)
     assert np.all(got[:, [5, 7]] == 0)
+
+
+@pytest.mark.parametrize("rows,hidden", [(3, 200), (5, 2048), (300, 2051), (300, 5120)])
+def test_a_row_of_zeros_stays_one_without_eps(mi355x, stream, rows, hidden):
+    """eps 0 divides a row of zeros by its own norm: it is zeros, with a scale of 1, as with any other eps; the rows
+    beside it are the definition's."""
+    say(f"zeros without eps, {rows} x {hidden}")
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((rows, hidden)).astype(np.float32)
+    res = rng.standard_normal((rows, hidden)).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(hidden)).astype(np.float32)
+    x[1], x[2] = 0, -res[2]
+    res[1] = 0
+    q, s, h, total = got = run_norm(mi355x, stream, x, res, w, eps=0.0)
+    for r in (1, 2):
+        assert s[r] == 1 and not q[r].any() and not h[r].any() and not total[r].any()
+    others = np.delete(np.arange(rows), [1, 2])
+    v, y = norm64(x[others], res[others], w, True, 0.0)
+    check_norm(y, v, tuple(a[others] for a in got), np.float32)
+
+
+def test_an_infinite_eps_leaves_rows_of_zeros(mi355x, stream):
+    say("infinite eps")
+    x = np.random.default_rng(3).standard_normal((4, 256)).astype(np.float32)
+    q, s, h, total = run_norm(mi355x, stream, x, None, None, eps=np.inf)
+    assert np.all(s == 1) and not q.any() and not h.any() and np.array_equal(total, x)
