@@ -17,6 +17,7 @@ namespace {
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxHidden = 1024 * 16;  // 1024 threads of 16 values (of 32: spills)
+constexpr int kLaunchRows = 1 << 21;   // a launch holds less than 2^32 threads, a row takes up to 1024
 
 struct NormArgs {
   const void* x;
@@ -315,14 +316,23 @@ extern "C" int mx_add_rmsnorm_i8(const MxNormRows* args, void* stream) {
       (uintptr_t)n->q_scale % 4 || (uintptr_t)n->h16 % 2)
     return MX_ERR_ALIGNMENT;
   if (n->rows == 0) return MX_OK;
-  const NormArgs a{n->x,   n->res,   n->sum,   n->norm_w, n->q,    n->q_scale,   (half_t*)n->h16, n->ldx,     n->ldres,
-                   n->ldsum, n->ldq, n->ldh, n->rows,   n->hidden, n->x_dtype, n->res_dtype,    n->param_dtype, n->norm,
-                   n->eps};
+  NormArgs a{n->x,   n->res,   n->sum,   n->norm_w, n->q,    n->q_scale,   (half_t*)n->h16, n->ldx,     n->ldres,
+             n->ldsum, n->ldq, n->ldh, n->rows,   n->hidden, n->x_dtype, n->res_dtype,    n->param_dtype, n->norm,
+             n->eps};
   auto on = [](const void* p, long ld, int e) { return !p || ((uintptr_t)p % (4 * e) == 0 && ld % 4 == 0); };
   const bool vec = H % 4 == 0 && on(n->x, n->ldx, xs) && on(n->res, n->ldres, rs) && on(n->sum, n->ldsum, rs) &&
                    on(n->norm_w, 0, ps) && on(n->q, n->ldq, 1) && on(n->h16, n->ldh, 2);
-  mx_clear_error();
-  if (vec) launch_rows<true>(a, (hipStream_t)stream);
-  else launch_rows<false>(a, (hipStream_t)stream);
-  return mx_launch_status();
+  for (long r0 = 0; r0 < n->rows; r0 += kLaunchRows) {
+    a.rows = (int)(n->rows - r0 < kLaunchRows ? n->rows - r0 : kLaunchRows);
+    a.x = (const char*)n->x + r0 * n->ldx * xs;
+    if (n->res) a.res = (const char*)n->res + r0 * n->ldres * rs;
+    if (n->sum) a.sum = (char*)n->sum + r0 * n->ldsum * rs;
+    if (n->q) a.q = n->q + r0 * n->ldq, a.qs = n->q_scale + r0;
+    if (n->h16) a.h16 = (half_t*)n->h16 + r0 * n->ldh;
+    mx_clear_error();
+    if (vec) launch_rows<true>(a, (hipStream_t)stream);
+    else launch_rows<false>(a, (hipStream_t)stream);
+    MX_TRY(mx_launch_status());
+  }
+  return MX_OK;
 }

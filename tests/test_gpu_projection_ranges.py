@@ -4,6 +4,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+import _serving as sv
+from moe_mi355x import projection as pj
 from test_gpu_projection import Case, check_norm, norm64, run_norm, say
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +57,24 @@ def test_an_infinite_eps_leaves_rows_of_zeros(mi355x, stream):
     x = np.random.default_rng(3).standard_normal((4, 256)).astype(np.float32)
     q, s, h, total = run_norm(mi355x, stream, x, None, None, eps=np.inf)
     assert np.all(s == 1) and not q.any() and not h.any() and np.array_equal(total, x)
+
+
+def test_norm_of_more_rows_than_a_launch_holds(mi355x, stream):
+    """Wide rows whose threads are more than 2^32 (103 GB): the first and last rows of every launch."""
+    rows, hidden = (1 << 22) + 3, 8196
+    say(f"norm {rows} x {hidden}")
+    look = sorted({0, 1, rows - 1, *(r + d for r in (1 << 21, 1 << 22) for d in (-1, 0))})
+    x = np.random.default_rng(5).standard_normal((len(look), hidden)).astype(np.float16)
+    w = (1 + 0.3 * np.random.default_rng(6).standard_normal(hidden)).astype(np.float32)
+    with sv.Arrays(mi355x, stream) as ar:
+        ar.held += [mi355x.alloc_device(rows * n) for n in (2 * hidden, hidden, 4)]
+        px, pq, ps = (int(b.handle) for b in ar.held)
+        for i, r in enumerate(look):
+            mi355x.copy_h2d_ptr_async(px + 2 * hidden * r, x[i].ctypes.data, x[i].nbytes, stream)
+        mi355x.synchronize_stream(stream)
+        pj.add_rmsnorm_i8(pj.norm_args(px, rows=rows, hidden=hidden, q=pq, q_scale=ps, norm_w=ar.put(w), dtype="float16"),
+                          stream)
+        q = np.stack([ar.get(pq + hidden * r, np.zeros(hidden, np.int8)) for r in look])
+        s = np.concatenate([ar.get(ps + 4 * r, np.zeros(1, np.float32)) for r in look])
+    v, y = norm64(x, None, w, True, 1e-6)
+    check_norm(y, v, (q, s, None, None), np.float16)
