@@ -26,6 +26,7 @@ constexpr int kMaxK = 1 << 16;
 constexpr int kMaxRank = 128;
 constexpr int kReadRank = 64;           // ranks from which a tile's rows do not read b themselves
 constexpr int kMaxLd = 1 << 22;        // 256 rows stay within a descriptor's 2 GiB
+constexpr long kMaxThreads = (1l << 32) - 1;  // of a launch
 
 __device__ __forceinline__ rsrc_t make_rsrc(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, 0x00020000);
@@ -894,7 +895,7 @@ template <int BM, int BN, int WM, int WN, int NS, int OCC, bool ADAPTERS = true>
 int launch_tiles(Args& a, hipStream_t s) {
   Tiles ts = {};
   const long blocks = number<BM, BN>(a, &ts);
-  if (blocks > INT_MAX / 4) return MX_ERR_UNSUPPORTED;
+  if (blocks * (BM / WM) * (BN / WN) * 64 > kMaxThreads) return MX_ERR_UNSUPPORTED;
   auto* kern = k_tiles<false, BM, BN, WM, WN, NS, OCC>;
   if constexpr (ADAPTERS) {
     if (a.low.id) kern = k_tiles<true, BM, BN, WM, WN, NS, OCC>;
@@ -992,7 +993,8 @@ int launch_many(Args& a, int mix, hipStream_t s) {
   if (tiles(64, 64) <= 256) return launch_tiles<64, 64, 32, 16, 4, 2>(a, s);
   if (tiles(128, 64) <= 256) return launch_tiles<128, 64, 32, 32, 3, 1>(a, s);
   if (tiles(64, 64) <= 512) return launch_tiles<64, 64, 32, 16, 4, 2>(a, s);  // two per CU
-  if (a.rank < kReadRank && mix > 2 * a.rank && a.M <= 1024) return launch_tiles<128, 64, 32, 32, 3, 1>(a, s);
+  if (a.rank < kReadRank && mix > 2 * a.rank && a.M <= 1024 && tiles(128, 64) * 512 <= kMaxThreads)
+    return launch_tiles<128, 64, 32, 32, 3, 1>(a, s);
   if (a.M <= kRowsMax) return launch_tiles<64, 128, 32, 32, 3, 1, false>(a, s);  // (with adapters: k_rows)
   if (tiles(128, 128) <= 256) return launch_tiles<128, 128, 64, 32, 4, 1>(a, s);
   if (tiles(256, 128) <= 256) return launch_tiles<256, 128, 64, 64, 3, 1>(a, s);

@@ -78,3 +78,35 @@ def test_norm_of_more_rows_than_a_launch_holds(mi355x, stream):
         s = np.concatenate([ar.get(ps + 4 * r, np.zeros(1, np.float32)) for r in look])
     v, y = norm64(x, None, w, True, 1e-6)
     check_norm(y, v, (q, s, None, None), np.float16)
+
+
+def test_adapters_of_more_columns_than_a_launch_holds(mi355x, stream):
+    """Four segments of the most columns there may be, 125 GB in all: 128 x 64 tiles, which as many adapters take
+    otherwise, would be 2^32 threads.  Whole numbers; the first and last columns of every segment."""
+    rows, k, n, rank, n_ad, edge = 897, 16, (1 << 24) - 1, 8, 17, 70
+    say(f"adapters alone, {rows} rows onto 4 x {n}")
+    rng = np.random.default_rng(8)
+    x = rng.integers(-2, 3, (rows, k)).astype(np.float16)
+    a = rng.integers(-2, 3, (n_ad, rank, k)).astype(np.float16)
+    ids = np.full(rows, 3, np.int32)
+    ids[[5, 896]], ids[7] = 16, -1
+    edges = {c: rng.integers(-2, 3, (n_ad, edge, rank)).astype(np.float16) for c in (0, n - edge)}
+    with sv.Arrays(mi355x, stream) as ar:
+        ar.held += [mi355x.alloc_device(size) for size in [2 * n_ad * n * rank] + [2 * rows * n] * 4]
+        pb, *py = (int(b.handle) for b in ar.held)
+        for c, b in edges.items():
+            for i in (3, 16):
+                mi355x.copy_h2d_ptr_async(pb + 2 * rank * (i * n + c), b[i].ctypes.data, b[i].nbytes, stream)
+        mi355x.synchronize_stream(stream)
+        pa = ar.put(a)
+        args = pj.projection_args([pj.segment(y, n, a=pa, b=pb) for y in py], rows=rows, k=k)
+        ad = pj.adapter_args(ar.put(x), ar.put(np.arange(rows + 1, dtype=np.int32)), ar.put(ids),
+                             ar.put(np.ones(n_ad, np.float32)), n_seqs=rows, n_adapters=n_ad, rank=rank, k=k)
+        need = pj.workspace_bytes(args, ad)
+        pj.project(args, stream, adapters=ad, workspace=(ar.put(np.zeros(need, np.uint8)), need))
+        for r in (0, 5, 7, 127, 128, 640, 895, 896):
+            t = x[r].astype(np.float64) @ a[ids[r]].astype(np.float64).T if ids[r] >= 0 else np.zeros(rank)
+            for c, b in edges.items():
+                want = t @ b[ids[r]].astype(np.float64).T
+                for y in py:
+                    assert np.array_equal(ar.get(y + 2 * (r * n + c), np.zeros(edge, np.float16)), want)
