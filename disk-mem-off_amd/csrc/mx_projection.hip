@@ -372,7 +372,7 @@ __global__ __launch_bounds__(64 * W) void k_adapter_t(const LowArgs p) {
 #pragma unroll
       for (int h = 0; h < H; ++h) red[wave][mi][h][lane] = acc[mi][h];
     __syncthreads();
-    // A wave finishes 16 ranks of 16 rows, or 32 with their common factor.  Ranks past the last are zero.
+    // A wave finishes 16 ranks of 16 rows, or 32 with their common factor.  Ranks past the last are zeros.
     constexpr int HF = PLANES ? 2 : 1;
     static_assert(H % HF == 0, "whole parts");
     for (int part = wave; part < MT * H / HF; part += W) {
@@ -383,6 +383,8 @@ __global__ __launch_bounds__(64 * W) void k_adapter_t(const LowArgs p) {
         v[h] = red[0][mi][h0 + h][lane];
 #pragma unroll
         for (int w = 1; w < W; ++w) v[h] += red[w][mi][h0 + h][lane];
+        // (rows of zeros by an infinity in x are NaN)
+        if (r0 + 16 * (h0 + h) + 4 * g >= p.rank) v[h] = (float4_t){0.f, 0.f, 0.f, 0.f};
       }
       int own = id[0];
 #pragma unroll

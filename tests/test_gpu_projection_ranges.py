@@ -110,3 +110,22 @@ def test_adapters_of_more_columns_than_a_launch_holds(mi355x, stream):
                 want = t @ b[ids[r]].astype(np.float64).T
                 for y in py:
                     assert np.array_equal(ar.get(y + 2 * (r * n + c), np.zeros(edge, np.float16)), want)
+
+
+@pytest.mark.parametrize("rank", [8, 40, 72, 128])
+@pytest.mark.parametrize("rows,each", [(20, 9), (90, 40), (200, 1), (700, 300)])
+def test_an_infinity_in_a_row_reaches_its_outputs_as_one(mi355x, stream, rows, each, rank):
+    """Adapters of positive weights, so that the definition's output is that infinity and no NaN, with ranks that fill
+    no whole tile; the other rows do not see it."""
+    say(f"infinite rows, {rows} rows, rank {rank}")
+    lens = [each] * (rows // each)
+    c = Case(6, rows, 272, [70], np.float32, lens=lens, ids=[i % 5 for i in range(len(lens))], rank=rank, n_adapters=5,
+             base=False, res=True)
+    c.a[0] = np.abs(c.a[0]) + np.float16(0.01)
+    c.b[0] = np.abs(c.b[0]) + np.float16(0.01)
+    clean = c.run(mi355x, stream)[0]
+    c.x[3, 7], c.x[6, 271] = np.inf, -np.inf
+    got = c.run(mi355x, stream)[0]
+    assert np.all(got[3] == np.inf) and np.all(got[6] == -np.inf)
+    others = np.delete(np.arange(rows), [3, 6])
+    assert np.all(np.isfinite(clean)) and np.array_equal(got[others], clean[others])
