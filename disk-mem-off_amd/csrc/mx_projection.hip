@@ -26,6 +26,7 @@ constexpr int kMaxK = 1 << 16;
 constexpr int kMaxRank = 128;
 constexpr int kReadRank = 64;           // ranks from which a tile's rows do not read b themselves
 constexpr int kMaxLd = 1 << 22;        // 256 rows stay within a descriptor's 2 GiB
+constexpr float kLo = 2048.f;          // the low plane of t, times this
 constexpr long kMaxThreads = (1l << 32) - 1;  // of a launch
 
 __device__ __forceinline__ rsrc_t make_rsrc(const void* base, uint32_t bytes) {
@@ -45,7 +46,7 @@ struct Seg {
   int t;       // which of the t arrays (-1: no adapters)
 };
 
-// What k_adapter_t leaves.  For k_rows: t alpha in fp32, [seg][row][rr].  For k_tiles: t 2^s = hi + lo as two fp16
+// What k_adapter_t leaves.  For k_rows: t alpha in fp32, [seg][row][rr].  For k_tiles: t 2^s = hi + lo / kLo as two fp16
 // planes, [seg][64 ranks][plane][row][64], and alpha 2^-s, [seg][row][rr / 32], s per 32 ranks such that the largest is
 // in [2^13, 2^14).
 struct Low {
@@ -276,9 +277,11 @@ __device__ __forceinline__ void adapters_of(const LowArgs& p, int t0, int (&id)[
   }
 }
 
-// A row's 8 ranks per lane group (32 in all) as two fp16 planes: v = (hi + lo) times the returned power of two, the
-// largest of hi + lo in [2^13, 2^14).  22 bits of the largest and, down to 2^-24 of it, of the others.  An infinity
-// or a NaN stays in hi.
+// A row's 8 ranks per lane group (32 in all) as two fp16 planes: v = hi + lo / kLo times the returned power of two, the
+// largest in [2^13, 2^14).  The low plane keeps the magnitude of the high one, so both hold 11 bits and a sign down to
+// 2^-27 of the largest: v is off by 2^-23 of itself there, and by 2^-49 of the largest below.  (Unscaled, the low
+// plane would be subnormal from 2^-16 of the largest on, and columns that meet only small ranks would lose their
+// digits.)  An infinity or a NaN stays in hi.
 __device__ __forceinline__ float split(const float4_t (&v)[2], half8_t& hi, half8_t& lo) {
   float top = 0.f;
 #pragma unroll
@@ -292,7 +295,7 @@ __device__ __forceinline__ float split(const float4_t (&v)[2], half8_t& hi, half
   for (int k = 0; k < 8; ++k) {
     const float u = ldexpf(v[k >> 2][k & 3], s);
     hi[k] = (half_t)u;
-    const float left = u - (float)hi[k];
+    const float left = (u - (float)hi[k]) * kLo;
     lo[k] = left - left == 0.f ? (half_t)left : (half_t)0.f;
   }
   return ldexpf(1.f, -s);
@@ -515,7 +518,7 @@ __device__ __forceinline__ int wave_min(int v) {
 // adapter's rows of b are staged in LDS as the product's operands are, 64 ranks (128 bytes) at a time, and a row
 // takes its own adapter's product.  Where the rows have many adapters and MANY, every lane reads its row's b itself.
 // 3099 rows of rank 64 onto 9216 columns: 87 us, without adapters 68; staging and products take turns. hi and lo are
-// multiplied in turn into one sum: 22 bits of t, where hi alone would be off by half a step of fp16.
+// multiplied in turn into one sum: t to 2^-23, where hi alone would be off by half a step of fp16.
 template <bool MANY, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void add_adapters(const Args& p, const Seg& sg, char* lds, int m0, int n0,
                                              float4_t (&v)[WM / 16][WN / 16]) {
@@ -562,7 +565,7 @@ __device__ __forceinline__ void add_adapters(const Args& p, const Seg& sg, char*
               for (int e = 0; e < 4; ++e) {
                 const half8_t bv = *(const half8_t*)(b + (long)min(nw + 16 * ni + 4 * g + e, N - 1) * rank + r);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) d[ni][e] = fmaf((float)hi[k] + (float)lo[k], (float)bv[k], d[ni][e]);
+                for (int k = 0; k < 8; ++k) d[ni][e] = fmaf(fmaf((float)lo[k], 1.f / kLo, (float)hi[k]), (float)bv[k], d[ni][e]);
               }
           }
           const float fac = p.low.fac[((long)sg.t * M + m) * nks + ks];
@@ -630,7 +633,7 @@ __device__ __forceinline__ void add_adapters(const Args& p, const Seg& sg, char*
 #pragma unroll
           for (int ni = 0; ni < NF; ++ni) {
             float4_t d = {0.f, 0.f, 0.f, 0.f};
-            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ni], lo, d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ni], lo, d, 0, 0, 0) * (1.f / kLo);
             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ni], hi, d, 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < 4; ++e)

@@ -722,8 +722,9 @@ typedef struct MxProjection {
 /* Adapters of the sequences of a call (device arrays): rows q_start[b] .. q_start[b + 1] - 1 take adapter
  * ids[b]; an id outside [0, n_adapters) is none, and rows behind the last sequence have none.  q_start
  * ascends from 0, n_seqs <= 65535.  x: fp16 rows [rows, k] (mx_add_rmsnorm_i8's h16), 16-byte aligned,
- * stride a multiple of 8 below 2^22.  rank: a multiple of 8, <= 128 (adapters of fewer: rows of zeros).  t is held
- * with 22 bits.  Non-finite weights of an adapter reach its own rows only.              */
+ * stride a multiple of 8 below 2^22.  rank: a multiple of 8, <= 128 (adapters of fewer: rows of zeros).  t is
+ * summed in fp32; up to 64 rows it is held in fp32, more rows hold it to 2^-23 of itself and 2^-49 of the largest
+ * of its 32 ranks.  Non-finite weights of an adapter reach its own rows only, as infinities or NaN.   */
 typedef struct MxAdapters {
   const void* x;
   const int32_t* q_start; /* [n_seqs + 1]                                               */

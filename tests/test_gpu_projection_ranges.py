@@ -129,3 +129,33 @@ def test_an_infinity_in_a_row_reaches_its_outputs_as_one(mi355x, stream, rows, e
     assert np.all(got[3] == np.inf) and np.all(got[6] == -np.inf)
     others = np.delete(np.arange(rows), [3, 6])
     assert np.all(np.isfinite(clean)) and np.array_equal(got[others], clean[others])
+
+
+@pytest.mark.parametrize("rows,each", [(60, 30), (90, 45), (200, 1), (700, 300)])
+@pytest.mark.parametrize("rank", [16, 48])
+def test_small_ranks_beside_loud_ones_keep_their_digits(mi355x, stream, rows, each, rank):
+    """Every other rank 2^-24 of its neighbour, and columns that only the small ranks reach.  t is exact in fp32 (whole
+    numbers below 2^24 times a power of two) and held to 2^-23 of itself; its products are summed in fp32, a rounding
+    or a truncation for each."""
+    say(f"small ranks, {rows} rows, rank {rank}")
+    k, n, n_ad = 64, 70, 3
+    lens = [each] * (rows // each)
+    c = Case(5, rows, k, [n], np.float32, lens=lens, ids=[i % n_ad for i in range(len(lens))], rank=rank, n_adapters=n_ad,
+             base=False, res=True)
+    rng = np.random.default_rng(11)
+    c.x = rng.integers(-1023, 1024, (rows, k)).astype(np.float16)
+    few = (rng.integers(0, 8, (n_ad, rank, k)) == 0) * rng.integers(-255, 256, (n_ad, rank, k))
+    few[:, 1::2] *= 2
+    c.a[0] = (few * np.where(np.arange(rank) % 2, 2.0 ** -24, 1.0)[:, None]).astype(np.float16)
+    assert np.array_equal(c.a[0][:, 1::2].astype(np.float64) * 2.0 ** 24, few[:, 1::2])  # subnormal, exact
+    c.b[0][:, 1::2, 0::2] = 0
+    c.res[0][:] = 0
+    c.alpha[:] = 1
+    got = c.run(mi355x, stream)[0].astype(np.float64)
+    for a, r in c.adapter_rows():
+        t = c.x[r].astype(np.float64) @ c.a[0][a].astype(np.float64).T
+        assert np.abs(t[:, 0::2]).max() < 2 ** 24 and np.abs(t[:, 1::2]).max() < 1
+        for cols in (slice(0, None, 2), slice(1, None, 2)):
+            b = c.b[0][a, cols].astype(np.float64)
+            size = np.abs(t) @ np.abs(b).T
+            assert np.all(np.abs(got[r, cols] - t @ b.T) <= (1 + rank + 4) * 2.0 ** -23 * size)
