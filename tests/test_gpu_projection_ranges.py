@@ -6,7 +6,7 @@ import pytest
 
 import _serving as sv
 from moe_mi355x import projection as pj
-from test_gpu_projection import Case, check_norm, norm64, run_norm, say
+from test_gpu_projection import SHAPES, Case, check_norm, norm64, run_norm, say
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,70 @@ def test_small_ranks_beside_loud_ones_keep_their_digits(mi355x, stream, rows, ea
             b = c.b[0][a, cols].astype(np.float64)
             size = np.abs(t) @ np.abs(b).T
             assert np.all(np.abs(got[r, cols] - t @ b.T) <= (1 + rank + 4) * 2.0 ** -23 * size)
+
+
+def long_ring_case(rows, ns, **kw):
+    """Nine stages of the reduction, the last in part: every ring of slots comes round, and ends inside a stage.  Whole
+    numbers: 1104 products of 100 x 100 at most, times 1/8, and what the adapters add, stay below 2^24 steps of 1/8."""
+    c = Case(rows, rows, 1104, ns, np.float32, whole=True, **kw)
+    rng = np.random.default_rng(rows + 1)
+    c.q = rng.integers(-100, 101, c.q.shape).astype(np.int8)
+    c.w = [rng.integers(-100, 101, w.shape).astype(np.int8) for w in c.w]
+    return c
+
+
+@pytest.mark.parametrize("rows,ns", SHAPES)
+def test_every_tile_over_many_stages(mi355x, stream, rows, ns):
+    say(f"many stages, {rows} rows -> {ns}")
+    c = long_ring_case(rows, ns)
+    for i, o in enumerate(c.run(mi355x, stream)):
+        assert np.array_equal(o, c.want(i)[0])
+
+
+@pytest.mark.parametrize("rows,ns", SHAPES)
+@pytest.mark.parametrize("rank,n_adapters,each", [(8, 33, 1), (72, 3, 70)])
+def test_every_adapted_tile_over_many_stages(mi355x, stream, rows, ns, rank, n_adapters, each):
+    say(f"many stages, adapted, {rows} rows -> {ns} rank={rank}")
+    rng = np.random.default_rng(rows * rank)
+    lens = []
+    while sum(lens) < rows - 3:
+        lens.append(min(int(rng.integers(0, 2 * each + 1)), rows - 3 - sum(lens)))
+    c = long_ring_case(rows, ns, lens=lens, ids=rng.integers(-1, n_adapters, len(lens)).tolist(), rank=rank,
+                       n_adapters=n_adapters)
+    for i, o in enumerate(c.run(mi355x, stream)):
+        assert np.array_equal(o, c.want(i)[0])
+
+
+@pytest.mark.parametrize("rows", [2, 13, 40, 64, 70, 130])
+def test_sums_past_24_bits_that_cancel(mi355x, stream, rows):
+    """The longest reduction in runs of +127 x 127 and -127 x 127, inside a quarter of it and across, with small codes in
+    between: partial sums reach 2^29, the sums stay below 2^24.  fp32 sums of 64 products each miss them."""
+    say(f"cancelling sums, {rows} rows")
+    k, n = 65536, 20
+    c = Case(9, rows, k, [n], np.float32)
+    rng = np.random.default_rng(9)
+    sign = rng.choice([-127, 127], (1, k))
+    c.w[0] = np.where(rng.random((n, k)) < 0.002, rng.integers(-127, 128, (n, k)), sign).astype(np.int8)
+    runs = np.stack([np.where(np.arange(k) // run % 2, -1, 1) for run in (32768, 8192, 2048, 16384)])
+    c.q = np.where(rng.random((rows, k)) < 0.002, rng.integers(-127, 128, (rows, k)),
+                   runs[np.arange(rows) % 4] * sign).astype(np.int8)
+    c.qs[:], c.ws = 1, [np.ones(n, np.float16)]
+    part = np.einsum("rsk,nsk->srn", c.q.reshape(rows, -1, 64).astype(np.float64), c.w[0].reshape(n, -1, 64).astype(np.float64),
+                     optimize=True)
+    want = part.sum(0)  # whole numbers, exact
+    near = np.zeros((rows, n), np.float32)
+    for p in part.astype(np.float32):
+        near += p
+    assert np.abs(want).max() < 2 ** 24 and np.abs(part.cumsum(0)).max() > 2 ** 28
+    assert np.mean(near != want) > 0.4  # (the runs of 2048 stay below 2^25)
+    assert np.array_equal(c.run(mi355x, stream)[0], want)
+
+
+@pytest.mark.parametrize("rows", [3, 90])
+def test_the_largest_sum(mi355x, stream, rows):
+    """-128 x -128 over the longest reduction: 2^30, within int32."""
+    say(f"largest sum, {rows} rows")
+    c = Case(9, rows, 65536, [20], np.float32)
+    c.q[:], c.w[0][:] = -128, -128
+    c.qs[:], c.ws = 1, [np.ones(20, np.float16)]
+    assert np.all(c.run(mi355x, stream)[0] == 2.0 ** 30)
