@@ -97,15 +97,21 @@ extern "C" int mx_quantize_rows_i8(const void* w, int32_t w_dtype, int32_t rows,
                                    int8_t* q, void* scale, void* stream) {
   if (!w || !q || !scale || rows < 0 || cols <= 0) return MX_ERR_INVALID;
   if (rows == 0) return MX_OK;
-  mx_clear_error();
+  if (w_dtype != MX_DT_F32 && w_dtype != MX_DT_F16) return MX_ERR_INVALID;
   hipStream_t s = (hipStream_t)stream;
-  if (w_dtype == MX_DT_F32)
-    hipLaunchKernelGGL(k_quantize_rows<float>, dim3(rows), dim3(256), 0, s, (const float*)w,
-                       (int)cols, q, (half_t*)scale);
-  else if (w_dtype == MX_DT_F16)
-    hipLaunchKernelGGL(k_quantize_rows<half_t>, dim3(rows), dim3(256), 0, s, (const half_t*)w,
-                       (int)cols, q, (half_t*)scale);
-  else
-    return MX_ERR_INVALID;
-  return mx_launch_status();
+  constexpr int kLaunchRows = 1 << 23;  // a launch holds less than 2^32 threads
+  for (size_t r0 = 0; r0 < (size_t)rows; r0 += kLaunchRows) {
+    const unsigned n = rows - r0 < kLaunchRows ? (unsigned)(rows - r0) : kLaunchRows;
+    int8_t* qr = q + r0 * cols;
+    half_t* sr = (half_t*)scale + r0;
+    mx_clear_error();
+    if (w_dtype == MX_DT_F32)
+      hipLaunchKernelGGL(k_quantize_rows<float>, dim3(n), dim3(256), 0, s, (const float*)w + r0 * cols, (int)cols, qr,
+                         sr);
+    else
+      hipLaunchKernelGGL(k_quantize_rows<half_t>, dim3(n), dim3(256), 0, s, (const half_t*)w + r0 * cols, (int)cols,
+                         qr, sr);
+    MX_TRY(mx_launch_status());
+  }
+  return MX_OK;
 }

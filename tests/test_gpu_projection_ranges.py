@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import _serving as sv
+from moe_mi355x import _lib
 from moe_mi355x import projection as pj
 from test_gpu_projection import SHAPES, Case, check_norm, norm64, run_norm, say
 
@@ -226,3 +227,19 @@ def test_the_largest_sum(mi355x, stream, rows):
     c.q[:], c.w[0][:] = -128, -128
     c.qs[:], c.ws = 1, [np.ones(20, np.float16)]
     assert np.all(c.run(mi355x, stream)[0] == 2.0 ** 30)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_more_weight_rows_than_a_launch_holds(mi355x, stream, dtype):
+    say(f"weights of 2^24 + 5 rows, {dtype.__name__}")
+    rows, cols = (1 << 24) + 5, 4
+    w = np.random.default_rng(2).standard_normal((rows, cols), dtype=np.float32).astype(dtype)
+    q, s = np.full((rows, cols), 99, np.int8), np.zeros(rows, np.float16)
+    with sv.Arrays(mi355x, stream) as ar:
+        pq, ps = ar.put(q), ar.put(s)
+        _lib.check(_lib.load().mx_quantize_rows_i8(ar.put(w), _lib.MX_DT_F16 if dtype is np.float16 else _lib.MX_DT_F32,
+                                                   rows, cols, pq, ps, stream), "mx_quantize_rows_i8")
+        q, s = ar.get(pq, q), ar.get(ps, s)
+    w = w.astype(np.float32)
+    assert np.array_equal(s, (np.abs(w).max(1) / np.float32(127)).astype(np.float16))
+    assert np.array_equal(q, np.clip(np.rint(w / s[:, None].astype(np.float32)), -127, 127))
