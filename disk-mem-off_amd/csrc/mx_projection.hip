@@ -103,9 +103,8 @@ __device__ __forceinline__ void store4(const Seg& sg, bool f16, long m, int n, f
   }
 }
 
-// A wave's tile, rows m + 16 mi and columns n + 16 ni; `whole`: all its columns are there, on boundaries
-// of four.  A row's residuals are loaded
-// while the row before is stored.
+// A wave's tile, rows m + 16 mi and columns n + 16 ni; `whole`: all its columns are there, on boundaries of four.  A
+// row's residuals are loaded while the row before is stored.
 template <typename T, int MF, int NF>
 __device__ __forceinline__ void store_tile(const Seg& sg, int m, int n, int M, bool whole, const float4_t (&v)[MF][NF]) {
   typedef T t4 __attribute__((ext_vector_type(4)));
@@ -228,7 +227,7 @@ struct WaveRing {
 // all rows of the block, and a row keeps its own's (columns of the product do not mix, so another adapter's NaN stays
 // away).  blockIdx.z deals the adapters of a tile to blocks.  Bound by latency: finding the adapters, the first
 // copies and the sums of the W waves follow one another (48 rows of 20 adapters, three segments of rank 16 of 2048:
-// 7.3 us; 3099 rows of rank 64: 16.7, 0.3 PFLOP/s).  The MFMA sums are fp32.
+// 7.3 us; 3099 rows of rank 64: 17, 0.3 PFLOP/s).  The MFMA sums are fp32.
 // ------------------------------------------------------------------------------------
 struct LowArgs {
   const half_t* x;
@@ -517,8 +516,9 @@ __device__ __forceinline__ int wave_min(int v) {
 // v += alpha t b^T of a tile.  Adapter after adapter, lowest id first: the planes of t for the tile's rows and the
 // adapter's rows of b are staged in LDS as the product's operands are, 64 ranks (128 bytes) at a time, and a row
 // takes its own adapter's product.  Where the rows have many adapters and MANY, every lane reads its row's b itself.
-// 3099 rows of rank 64 onto 9216 columns: 87 us, without adapters 68; staging and products take turns. hi and lo are
-// multiplied in turn into one sum: t to 2^-23, where hi alone would be off by half a step of fp16.
+// 3099 rows of rank 64 onto 9216 columns: 92 us, without adapters 71; staging and products take turns.  lo and hi are
+// multiplied in turn into one sum, lo's scaled back in between (2 of the 92 us): t to 2^-23, where hi alone would be
+// off by half a step of fp16.
 template <bool MANY, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void add_adapters(const Args& p, const Seg& sg, char* lds, int m0, int n0,
                                              float4_t (&v)[WM / 16][WN / 16]) {
@@ -540,10 +540,10 @@ __device__ __forceinline__ void add_adapters(const Args& p, const Seg& sg, char*
   };
 
   if constexpr (MANY) {
-    // 128 rows onto 4096 columns, rank 16, in 64 x 64 tiles: 4 adapters 15.0 us staged, 16.0 read; 8 of them 18.0 and
-    // 16.4, 64 of them 35.7 and 16.9.  600 rows in 128 x 128 tiles: 16 adapters 31.8 and 32.6, 32 of them 44.3 and
-    // 33.7.  Rows of b of 64 ranks fill cache lines of their own, which every row of the tile reads again: 128 rows
-    // of 64 adapters onto 9216 columns 73.8 and 89.1 (48 ranks 70.5 and 60.4).
+    // Rows of 4096 onto 4096 columns, rank 16.  128 rows in 64 x 64 tiles: 4 adapters 14.8 us staged, 16.0 read; 8 of
+    // them 18.3 and 16.5, 64 of them 36.4 and 17.3.  600 rows in 128 x 128 tiles: 16 adapters 39.1 and 38.8, 32 of
+    // them 52.4 and 39.6.  Rows of b of 64 ranks fill cache lines of their own, which every row of the tile reads
+    // again: 128 rows of 64 adapters of 2048 onto 9216 columns 70.8 and 90.2 (48 ranks 74.3 and 57.1).
     const int most = rank * (BM * BN / 4096) * 3 / 8;
     int n = 0;
     if (rank < kReadRank)
@@ -810,7 +810,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, OCC) void k_tiles(const
 }
 
 // A block per CU, each with the same number of 256 x 256 tiles; what is left of them (ts.first on) in quarters.
-// Bound by the matrix units and the copies next to them: 4096 rows onto 9216 columns of 2048 83 us, 1.86 POP/s.
+// Bound by the matrix units and the copies next to them: 4096 rows onto 9216 columns of 2048 86 us, 1.80 POP/s.
 template <bool AD>
 __global__ __launch_bounds__(512, 1) void k_rounds(const Args p, const Tiles ts) {
   __shared__ __align__(1024) char lds[2 * 512 * kStage];
@@ -989,10 +989,14 @@ int launch_few(Args& a, hipStream_t s) {
 // small tiles on more CUs are faster (330 rows onto 2048 columns of 4096: 64 x 64 10.4 us, 128 x 128 16.4, 256 x 256
 // 26); past one round the larger tile's fewer copies per product count (1700 rows: 28.2, 19.4 and 28).  Past all of
 // them rounds of 256 x 256 (4096 rows onto 9216 of 2048: 90 us, 128 x 128 tiles 100), but tiles no higher than the
-// rows (128 rows onto 131072: 128 x 128 73 us, 84; 64 rows: 64 x 128 58, 64 x 64 68). `mix`: adapters that 128 rows
-// may have.  Where they are many, tiles whose rows can read b themselves (512 sequences of a row onto 9216 columns,
-// rank 16: of 64 adapters 58 us, 256 x 128 tiles 80; of 256 adapters 77, 172; of 16 50, 41; of 4 31, 28), up to 1024
-// rows (2048 of 4 adapters: 90 us, 66).
+// rows (128 rows onto 131072: 128 x 128 73 us, 84; 64 rows: 64 x 128 58, 64 x 64 68).
+//
+// `mix`: adapters that 128 rows may have, on the mean of the batch (where its long sequences lie the device knows alone).
+// Where they are many, tiles whose rows can read b themselves (512 sequences of a row onto 9216 columns, rank 16: of 64
+// adapters 54 us, 256 x 128 tiles 84; of 256 adapters 74, 180; of 16 48, 44; of 4 32, 29), up to 1024 rows (2048 of 4
+// adapters: 89 us, 67).  Tiles of more than 2048 outputs a wave take an adapter after the other, however many: 2048 rows of
+// 256 adapters 272 us (187 in 128 x 64 tiles), a prompt of 900 rows beside 100 sequences of a row, 64 adapters, 125 us
+// (1000 rows of one adapter 41).
 int launch_many(Args& a, int mix, hipStream_t s) {
   auto tiles = [&](int bm, int bn) { return column_blocks(a, bn) * mx_ceil_div(a.M, bm); };
   if (tiles(64, 64) <= 256) return launch_tiles<64, 64, 32, 16, 4, 2>(a, s);
