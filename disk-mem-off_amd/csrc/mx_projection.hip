@@ -25,8 +25,8 @@ constexpr int kRowsMax = 64;            // rows of k_rows
 constexpr int kMaxK = 1 << 16;
 constexpr int kMaxRank = 128;
 constexpr int kReadRank = 64;           // ranks from which a tile's rows do not read b themselves
-constexpr int kMaxLd = 1 << 22;        // 256 rows stay within a descriptor's 2 GiB
-constexpr float kLo = 2048.f;          // the low plane of t, times this
+constexpr int kMaxLd = 1 << 22;         // 256 rows stay within a descriptor's 2 GiB
+constexpr float kLo = 2048.f;           // the low plane of t is held times this
 constexpr long kMaxThreads = (1l << 32) - 1;  // of a launch
 
 __device__ __forceinline__ rsrc_t make_rsrc(const void* base, uint32_t bytes) {
@@ -278,7 +278,7 @@ __device__ __forceinline__ void adapters_of(const LowArgs& p, int t0, int (&id)[
 
 // A row's 8 ranks per lane group (32 in all) as two fp16 planes: v = hi + lo / kLo times the returned power of two, the
 // largest in [2^13, 2^14).  The low plane keeps the magnitude of the high one, so both hold 11 bits and a sign down to
-// 2^-27 of the largest: v is off by 2^-23 of itself there, and by 2^-49 of the largest below.  (Unscaled, the low
+// 2^-26 of the largest: v is off by 2^-23 of itself there, and by 2^-49 of the largest below.  (Unscaled, the low
 // plane would be subnormal from 2^-16 of the largest on, and columns that meet only small ranks would lose their
 // digits.)  An infinity or a NaN stays in hi.
 __device__ __forceinline__ float split(const float4_t (&v)[2], half8_t& hi, half8_t& lo) {
